@@ -258,6 +258,82 @@ int mc_generate_limits_dev(mc_batch* batch, const int32_t* d_prompts, const int3
                            const int32_t* d_max_tokens, int n_max, double temperature, uint32_t session0,
                            int32_t* d_out_tokens, float* d_out_probs);
 
+/* ---------------------------------------------------------------------------------------------
+ * A quantised key/value cache and the attention around it, for callers that run their own layers
+ * (the engine above keeps float32 rings of its own; nothing here has a counterpart in the
+ * reference). All of it works on device pointers and the caller's stream.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum { MC_F32 = 0, MC_F16 = 1, MC_BF16 = 2 } mc_dtype;
+
+/* Rows [row][head][head_dim] on the device, strides in elements; a head's dimensions are
+ * contiguous. Any strides, any alignment of the type. */
+typedef struct {
+  void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} mc_rows;
+
+typedef struct {
+  int sessions;
+  int heads;     /* key/value heads */
+  int head_dim;  /* a multiple of 16, 16 to 128 */
+  int bits;      /* 4 or 8 */
+  int slots;     /* positions held per session, at most 2^30 */
+  int sinks;     /* first positions of a session, never overwritten: [0, slots) */
+} mc_kv_spec;
+
+typedef struct mc_kv mc_kv;
+
+/* A cache of keys and values for `sessions` sessions of one layer, in device memory that the
+ * library owns. Position p of a session is held at place p while p < sinks, then in a ring of
+ * slots - sinks places: the cache holds the first `sinks` positions and the last slots - sinks.
+ * Each row of head_dim values is held as codes of `bits` bits with a scale and a center
+ * (bfloat16): center + scale * m, m an odd integer in [-15, 15] (4 bits) or an integer in
+ * [-127, 127] (8 bits). The center is the bfloat16 next to the middle of the row's extremes and
+ * the scale is rounded up, so |x - read back| <= scale (4 bits) or scale / 2 (8 bits), plus float32
+ * rounding. A row that is not all finite reads back as NaN; a masked one reaches no output. */
+int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out);
+/* Waits for the device's work and frees the cache. */
+int mc_kv_close(mc_kv* kv);
+/* Waits for the device's work; MC_INVALID_ARGUMENT if a call since the last check named a session
+ * or a position out of range (such rows are skipped, attention rows written as zero). */
+int mc_kv_error(mc_kv* kv);
+
+/* Quantises rows into the cache. Segment b is rows [row_start[b], row_start[b+1]) and goes to
+ * session sessions[b] (NULL: b) at positions pos0[b], pos0[b]+1, ...; row_start == NULL: one row
+ * per segment (n_rows == n_segments). Of a segment longer than the ring only the positions that
+ * stay are written. Segments of one call must not share a session's places. Arrays of the calls
+ * below and this one are device int32. Calls on one cache are ordered by the caller (one stream, or
+ * events); no call allocates or synchronizes, so they can be captured into a graph. */
+int mc_kv_write_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int n_rows, const int32_t* row_start,
+                    const int32_t* sessions, const int32_t* pos0, int n_segments, void* stream);
+
+/* Reads positions back as rows, laid out like mc_kv_write_dev's: segment b's rows are positions
+ * pos0[b], pos0[b]+1, ... of a session that has lens[b] positions so far. Positions that are not
+ * held (past lens[b], or overwritten since) and rows of no segment come back as zeros. */
+int mc_kv_read_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int n_rows, const int32_t* row_start,
+                   const int32_t* sessions, const int32_t* pos0, const int32_t* lens, int n_segments, void* stream);
+
+/* Attention of one query token per session over the cached positions: row i of q and out
+ * [n][q_heads][head_dim] belongs to session sessions[i] (NULL: i), which has lens[i] positions, the
+ * query's own the last. It sees the held positions p with p < sinks or p > lens[i] - 1 - window
+ * (window 0: every held one). out = softmax(scale q.k) v; query head h uses key/value head
+ * h / (q_heads / heads). A row that sees nothing (lens[i] <= 0) is zero. */
+int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out, int dtype, int q_heads, const int32_t* sessions,
+                     const int32_t* lens, int n, int window, float scale, void* stream);
+
+/* Causal attention of whole segments with the same mask, over keys and values as they are
+ * (prompts, before they go into the cache, or after mc_kv_read_dev has brought the past back).
+ * Segment b is queries [q_start[b], q_start[b+1]) and keys [k_start[b], k_start[b+1]); its queries
+ * are its last positions: query t of nq is position nk - nq + t. It sees keys j <= position with
+ * j < sinks or j > position - window (window 0: all of them). A row that sees nothing is zero;
+ * rows outside every segment are not written; a segment whose bounds leave the n_q or n_k rows is
+ * skipped. q_start and k_start NULL: one segment of all rows. head_dim 1 to 256. Runs on the
+ * current device. */
+int mc_window_attn_dev(const mc_rows* q, const mc_rows* k, const mc_rows* v, const mc_rows* out, int dtype, int q_heads,
+                       int kv_heads, int head_dim, int n_q, int n_k, const int32_t* q_start, const int32_t* k_start,
+                       int n_segments, int window, int sinks, float scale, void* stream);
+
 /* The int8 rate of this device's tensor pipe, the denominator of the INT8 roofline fractions (no
  * counterpart in the reference: a measurement). One CTA per multiprocessor issues back-to-back
  * tcgen05.mma kind::i8 instructions of the largest single-CTA shape (M 128, N 256, K 32) on

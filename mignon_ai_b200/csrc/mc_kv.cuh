@@ -1,0 +1,147 @@
+// The quantised key/value cache: its layout in memory, its quantiser and the positions it holds.
+//
+// A cache has `slots` places per session. Position p of a session lies at slot p while p < sinks
+// (the first positions are never overwritten) and at sinks + (p - sinks) % (slots - sinks) after
+// that: a ring behind pinned places. Every (session, head) owns one region
+//
+//   keys' codes | values' codes | keys' scales and centers | values' scales and centers
+//
+// with `cap` = slots rounded up to 64 places. Codes of four consecutive slots are interleaved, so
+// that a 16-byte load gives a lane one 32-bit word of each of the four, in the order in which the
+// operands of an 8-bit m16n8k32 MMA want them:
+//
+//   keys    word w of slot s is word (s / 4) * 4 * words + 4 * w + s % 4. 8 bits: word w holds
+//           dimensions 4w..4w+3. 4 bits: byte b of word w holds dimensions 8w + b (low) and
+//           8w + 4 + b (high). The contraction runs along the dimensions: a word is an operand.
+//   values  word (s / 4) * cb + n * ni + i (cb code bytes per slot) holds dimension 8i + n
+//           (8 bits, ni = dim / 8), or 16i + n (low) and 16i + 8 + n (high) (4 bits, ni = dim / 16),
+//           of four slots, slot s in byte s % 4. The contraction runs along the slots.
+//
+// A slot's scale and center are one word: scale in the low half, center in the high (bfloat16).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "mc_sm100.cuh"
+
+namespace mc {
+namespace kv {
+
+enum Dtype : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+constexpr int kMaxDim = 128;
+
+// Rows [row][head][dim] with element strides; the dimensions of a row are contiguous.
+struct Rows {
+  void* p;
+  long long row, head;
+};
+
+struct Cache {
+  int sessions, heads, dim, bits, slots, sinks, ring, cap;
+  int cb;              // code bytes of one slot's keys (and of its values): dim * bits / 8
+  long long region;    // bytes of one (session, head)
+  uint8_t* base;       // [session][head] regions
+  int* error;          // set when an index was out of range (that access is skipped)
+};
+
+__device__ __forceinline__ uint8_t* region_of(const Cache& c, int session, int head) {
+  return c.base + ((long long)session * c.heads + head) * c.region;
+}
+__device__ __forceinline__ long long values_offset(const Cache& c) { return (long long)c.cap * c.cb; }
+__device__ __forceinline__ long long params_offset(const Cache& c) { return 2ll * c.cap * c.cb; }
+
+__device__ __forceinline__ int slot_of(const Cache& c, int pos) {
+  return pos < c.sinks ? pos : c.sinks + (pos - c.sinks) % c.ring;
+}
+
+// The position that slot s holds in a session of `len` positions, or -1.
+__device__ __forceinline__ int position_of(const Cache& c, int s, int len) {
+  if (s < c.sinks) return s < len ? s : -1;
+  const int last = len - 1 - c.sinks, j = s - c.sinks;  // ring coordinates of the newest position and of s
+  if (j >= c.ring || last < 0) return -1;
+  const int back = last >= j ? (last - j) % c.ring : c.ring - (j - last);  // j - last < ring
+  const int p = last - back;
+  return p < 0 ? -1 : c.sinks + p;
+}
+
+// Whether a session of `len` positions still holds position pos.
+__device__ __forceinline__ bool is_held(const Cache& c, int pos, int len) {
+  return pos >= 0 && pos < len && (pos < c.sinks || pos >= len - c.ring);
+}
+
+template <class T>
+__device__ __forceinline__ float to_float(T x);
+template <>
+__device__ __forceinline__ float to_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// The quantiser of one row x of one head, from its extremes:
+//   center = bf16(hi / 2 + lo / 2), half = max(hi - center, center - lo),
+//   scale  = half / (15 or 127), rounded up to bfloat16 so that the codes reach both extremes
+//            (0 where half is below 2^-100: the row then reads back as its center),
+//   m      = the odd integer of [-15, 15] (4 bits) or the integer of [-127, 127] (8 bits) next to
+//            (x - center) / scale.
+// The row reads back as center + scale * m. The products scale * m are exact in float32 (8 by at
+// most 8 bits), so a fused and a separate multiply-add give the same value. A row that is not all
+// finite, or whose center or scale leaves bfloat16's range, reads back as NaN (scale NaN).
+struct Quant {
+  float scale, center, inv;
+};
+
+__device__ __forceinline__ Quant quant_of(float hi, float lo, bool finite, int bits) {
+  Quant q;
+  q.center = __bfloat162float(__float2bfloat16_rn(__fadd_rn(__fmul_rn(0.5f, hi), __fmul_rn(0.5f, lo))));
+  const float half = fmaxf(__fsub_rn(hi, q.center), __fsub_rn(q.center, lo));
+  const float step = __fmul_rn(half, bits == 4 ? 1.0f / 15.0f : 1.0f / 127.0f);
+  q.scale = __uint_as_float((__float_as_uint(step) + 0xFFFFu) & 0xFFFF0000u);
+  if (half < 0x1p-100f) q.scale = 0.f;
+  q.inv = q.scale > 0.f ? __fdiv_rn(1.0f, q.scale) : 0.f;
+  if (!finite || !(fabsf(q.center) <= 3.4e38f) || !(q.scale <= 3.4e38f)) {
+    q.scale = __int_as_float(0x7FFF0000);
+    q.center = 0.f;
+    q.inv = 0.f;
+  }
+  return q;
+}
+
+__device__ __forceinline__ uint32_t param_word(const Quant& q) {
+  return (__float_as_uint(q.scale) >> 16) | (__float_as_uint(q.center) & 0xFFFF0000u);
+}
+__device__ __forceinline__ float param_scale(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float param_center(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// The code of x: 4 bits: a nibble c in two's complement, m = 2c + 1; 8 bits: m itself.
+__device__ __forceinline__ int code_of(const Quant& q, float x, int bits) {
+  const float t = __fmul_rn(__fsub_rn(x, q.center), q.inv);
+  if (bits == 4) return (int)fminf(fmaxf(floorf(__fmul_rn(0.5f, t)), -8.f), 7.f);
+  return (int)fminf(fmaxf(rintf(t), -127.f), 127.f);
+}
+
+// The segment of row r: the last b with start[b] <= r (null starts: one row per segment), or -1.
+__device__ __forceinline__ int segment_of(const int* start, int n, int r) {
+  if (!start) return r < n ? r : -1;
+  if (r < start[0] || r >= start[n]) return -1;
+  int lo = 0, hi = n;  // start[lo] <= r < start[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= r) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace kv
+}  // namespace mc
