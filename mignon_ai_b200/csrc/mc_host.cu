@@ -53,6 +53,27 @@ bool make_tmap_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t co
   return true;
 }
 
+bool make_tmap_16(CUtensorMap* map, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1,
+                  uint64_t s2, uint32_t box1, uint32_t box2) {
+  auto fn = encode_fn();
+  if (!fn) {
+    set_error(kCudaError, "cuTensorMapEncodeTiled is not available from the driver");
+    return false;
+  }
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {s1, s2};
+  cuuint32_t box[3] = {64, box1, box2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(kCudaError, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+    return false;
+  }
+  return true;
+}
+
 int check_device_error(cudaStream_t stream) {
   int code = 0;
   MC_CUDA(cudaMemcpyFromSymbolAsync(&code, g_device_error, sizeof(int), 0, cudaMemcpyDeviceToHost, stream));

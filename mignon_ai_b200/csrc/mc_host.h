@@ -37,6 +37,12 @@ enum Status : int {
 bool make_tmap_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch,
                   uint32_t box_cols, uint32_t box_rows);
 
+// Encodes a 3-D tiled tensor map over 16-bit elements [d2][d1][d0] (d0 contiguous, byte strides s1
+// and s2) with box {64, box1, box2} and the 128-byte swizzle; reads past an extent give zeros.
+// Returns false (with the error recorded) if the driver rejects it.
+bool make_tmap_16(CUtensorMap* map, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1,
+                  uint64_t s2, uint32_t box1, uint32_t box2);
+
 // Reads and clears the device error word of the current device; non-zero codes become
 // kDeviceTimeout with a message.
 int check_device_error(cudaStream_t stream);

@@ -1,5 +1,6 @@
 // Kernels of the quantised key/value cache (mc_kv.cuh): quantising rows as they are written,
 // reading them back, and one query token's attention over a session's cached positions.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <new>
@@ -7,6 +8,7 @@
 #include "../../include/mignon_cuda.h"
 #include "mc_host.h"
 #include "mc_kv.cuh"
+#include "mc_kv_attend.cuh"
 
 namespace mc {
 namespace kv {
@@ -159,103 +161,6 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_consta
   }
 }
 
-// ------------------------------------------------------------------------------------------------
-// Attention of one query token over the cache: one warp per (session, query head)
-// ------------------------------------------------------------------------------------------------
-struct AttendArgs {
-  Cache c;
-  Rows q, out;
-  int n, q_heads, group, window;
-  const int *sess, *lens;
-  float scale;  // of the scores, times log2(e)
-};
-
-template <class T>
-__global__ void __launch_bounds__(kCacheThreads) attend_kernel(const __grid_constant__ AttendArgs a) {
-  __shared__ float qs[kCacheThreads / 32][kMaxDim];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
-  const int b = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
-  if (b >= a.n) return;
-  const Cache& c = a.c;
-  const int dim = c.dim, bits = c.bits, cb = c.cb;
-  const T* q = static_cast<const T*>(a.q.p) + b * a.q.row + h * a.q.head;
-  T* out = static_cast<T*>(a.out.p) + b * a.out.row + h * a.out.head;
-  const int session = a.sess ? a.sess[b] : b;
-  const bool ok = (unsigned)session < (unsigned)c.sessions;
-  if (!ok) atomicExch(c.error, 1);
-  const int len = ok ? a.lens[b] : 0;
-  float qsum = 0.f;
-  for (int d = lane; d < dim; d += 32) {
-    qs[warp][d] = to_float<T>(q[d]);
-    qsum = __fadd_rn(qsum, qs[warp][d]);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) qsum = __fadd_rn(qsum, __shfl_xor_sync(~0u, qsum, o));
-  __syncwarp();
-  const uint8_t* region = region_of(c, ok ? session : 0, h / a.group);
-  const uint32_t* params = reinterpret_cast<const uint32_t*>(region + params_offset(c));
-  float top = -INFINITY, total = 0.f, acc[kMaxDim / 32] = {};
-  for (int t = 0; t < c.slots; t += 32) {
-    const int slot = t + lane;
-    const int pos = slot < c.slots ? position_of(c, slot, len) : -1;
-    const bool seen = pos >= 0 && (a.window <= 0 || pos < c.sinks || pos >= len - a.window);
-    if (!__any_sync(~0u, seen)) continue;
-    float s = -INFINITY, vscale = 0.f, vcenter = 0.f;
-    if (seen) {
-      const uint8_t* codes = region + (long long)(slot >> 2) * 4 * cb + 4 * (slot & 3);
-      float dot = 0.f;
-      for (int w = 0; w < cb / 4; ++w) {
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + 16 * w);
-        for (int e = 0; e < 32 / bits; ++e) {
-          const uint32_t byte = (word >> (8 * (e & 3))) & 255u;
-          const float m = bits == 4 ? (float)(2 * signed_nibble(byte, e >> 2) + 1) : (float)(int8_t)byte;
-          dot = __fmaf_rn(m, qs[warp][w * (32 / bits) + e], dot);
-        }
-      }
-      s = __fmul_rn(a.scale, __fmaf_rn(param_scale(params[slot]), dot, __fmul_rn(param_center(params[slot]), qsum)));
-      vscale = param_scale(params[c.cap + slot]);
-      vcenter = param_center(params[c.cap + slot]);
-    }
-    float m = s;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float other = __shfl_xor_sync(~0u, m, o);
-      m = m >= other || isnan(m) ? m : other;  // a NaN score stays
-    }
-    m = m >= top || isnan(m) ? m : top;
-    if (m == -INFINITY) continue;  // nothing but scores of minus infinity so far
-    const float keep = exp2f(__fsub_rn(top, m));
-    const float p = exp2f(__fsub_rn(s, m));
-    top = m;
-    total = __fmul_rn(total, keep) + p;  // per lane; summed over the lanes at the end
-#pragma unroll
-    for (int u = 0; u < kMaxDim / 32; ++u) acc[u] = __fmul_rn(acc[u], keep);
-    for (int j = 0; j < 32; ++j) {
-      const bool js = __shfl_sync(~0u, (int)seen, j);
-      const float pj = __shfl_sync(~0u, p, j), sj = __shfl_sync(~0u, vscale, j), cj = __shfl_sync(~0u, vcenter, j);
-      if (!js) continue;
-      const uint8_t* codes = region + values_offset(c) + (long long)((t + j) >> 2) * 4 * cb + ((t + j) & 3);
-      const int ni = cb / 8;
-#pragma unroll
-      for (int u = 0; u < kMaxDim / 32; ++u) {
-        const int d = lane + 32 * u;
-        if (d >= dim) break;
-        const uint32_t byte = codes[4 * ((d % 8) * ni + (bits == 4 ? d / 16 : d / 8))];
-        const float m = bits == 4 ? (float)(2 * signed_nibble(byte, (d >> 3) & 1) + 1) : (float)(int8_t)byte;
-        acc[u] = __fmaf_rn(pj, __fmaf_rn(sj, m, cj), acc[u]);
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total = __fadd_rn(total, __shfl_xor_sync(~0u, total, o));
-#pragma unroll
-  for (int u = 0; u < kMaxDim / 32; ++u) {
-    const int d = lane + 32 * u;
-    if (d < dim) out[d] = from_float<T>(total == 0.f ? 0.f : __fdiv_rn(acc[u], total));
-  }
-}
-
 }  // namespace kv
 }  // namespace mc
 
@@ -265,7 +170,10 @@ __global__ void __launch_bounds__(kCacheThreads) attend_kernel(const __grid_cons
 struct mc_kv {
   int device = 0;
   mc::kv::Cache c{};
-  void* mem = nullptr;
+  void* mem = nullptr;       // error word, arrival counters, partial results, regions
+  int* arrived = nullptr;
+  float* partial = nullptr;
+  int n_sm = 0;
 };
 
 namespace mc {
@@ -326,10 +234,14 @@ extern "C" int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out) {
   c.cap = (s.slots + 63) / 64 * 64;
   c.cb = s.head_dim * s.bits / 8;
   c.region = 2ll * c.cap * (c.cb + 4);
-  const double need = (double)c.region * s.sessions * s.heads + 256;
+  // the workspace of mc_kv_attend_dev is part of the cache, so that no call allocates
+  const size_t head = 256 + kv::kMaxPartials * (sizeof(int) + kv::kAttendRows * (2 + s.head_dim) * sizeof(float));
+  const double need = (double)c.region * s.sessions * s.heads + (double)head;
   size_t bytes = 0;
   void* mem = nullptr;
-  if (need < 9e18) bytes = (size_t)c.region * s.sessions * s.heads + 256;
+  int n_sm = 0;
+  MC_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
+  if (need < 9e18) bytes = (size_t)c.region * s.sessions * s.heads + head;
   if (!bytes || cudaMalloc(&mem, bytes) != cudaSuccess) {
     (void)cudaGetLastError();
     return set_error(kOutOfMemory, "mc_kv_open: no room for a cache of " + std::to_string(need) + " bytes");
@@ -340,7 +252,7 @@ extern "C" int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out) {
     return set_error(kCudaError, std::string("mc_kv_open: cudaMemset: ") + cudaGetErrorString(e));
   }
   c.error = static_cast<int*>(mem);
-  c.base = static_cast<uint8_t*>(mem) + 256;
+  c.base = static_cast<uint8_t*>(mem) + head;  // a multiple of 256
   mc_kv* kv = new (std::nothrow) mc_kv;
   if (!kv) {
     cudaFree(mem);
@@ -349,6 +261,9 @@ extern "C" int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out) {
   kv->device = device;
   kv->c = c;
   kv->mem = mem;
+  kv->arrived = reinterpret_cast<int*>(static_cast<uint8_t*>(mem) + 256);
+  kv->partial = reinterpret_cast<float*>(kv->arrived + kv::kMaxPartials);
+  kv->n_sm = n_sm;
   *out = kv;
   return kOk;
 }
@@ -408,12 +323,23 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   if (n == 0) return kOk;
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
-  const AttendArgs a{kv->c, rows_of(q), rows_of(out), n, q_heads, q_heads / kv->c.heads, window, sessions, lens,
-                     scale * 1.4426950408889634f};
-  const long long blocks = ((long long)n * q_heads + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
+  const Cache& c = kv->c;
+  const int group = q_heads / c.heads, row_groups = (group + kAttendRows - 1) / kAttendRows;
+  const long long items = (long long)n * c.heads * row_groups;
+  // warps an item's slots are split over: enough for two waves of the 16 warps an SM holds, while
+  // each keeps two tiles of 64 slots
+  const int seen = window > 0 ? (int)std::min<long long>(c.slots, (long long)window + c.sinks) : c.slots;
+  const long long wanted = std::min<long long>((2ll * 16 * kv->n_sm + items - 1) / items, (seen + 127) / 128);
+  const bool split = wanted > 1;
+  int pieces = 1;
+  if (split) pieces = (int)std::max<long long>(1, std::min<long long>((wanted + kAttendWarps - 1) / kAttendWarps, kMaxPartials / items));
+  const AttendArgs a{c, rows_of(q), rows_of(out), n, q_heads, group, row_groups, window, dtype, pieces, sessions, lens,
+                     scale * 1.4426950408889634f, kv->partial, kv->arrived};
+  const long long blocks = split ? items : (items + kAttendWarps - 1) / kAttendWarps;
   if (blocks > INT_MAX) return set_error(kInvalidArgument, "mc_kv_attend_dev: too many rows");
-  void (*f)(AttendArgs) = dtype == kF32 ? attend_kernel<float> : dtype == kF16 ? attend_kernel<__half> : attend_kernel<__nv_bfloat16>;
-  f<<<(unsigned)blocks, kCacheThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  const int planes = dtype == kF32 ? 3 : 2;
+  auto f = c.bits == 4 ? attend_variant_of<4>(c.dim, planes, split) : attend_variant_of<8>(c.dim, planes, split);
+  f<<<dim3((unsigned)blocks, pieces), kAttendWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
   MC_CUDA(cudaGetLastError());
   return kOk;
 }

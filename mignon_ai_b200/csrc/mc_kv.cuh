@@ -96,7 +96,8 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { re
 //            (x - center) / scale.
 // The row reads back as center + scale * m. The products scale * m are exact in float32 (8 by at
 // most 8 bits), so a fused and a separate multiply-add give the same value. A row that is not all
-// finite, or whose center or scale leaves bfloat16's range, reads back as NaN (scale NaN).
+// finite, or whose center or scale leaves bfloat16's range, reads back as NaN (scale and
+// center NaN).
 struct Quant {
   float scale, center, inv;
 };
@@ -110,8 +111,7 @@ __device__ __forceinline__ Quant quant_of(float hi, float lo, bool finite, int b
   if (half < 0x1p-100f) q.scale = 0.f;
   q.inv = q.scale > 0.f ? __fdiv_rn(1.0f, q.scale) : 0.f;
   if (!finite || !(fabsf(q.center) <= 3.4e38f) || !(q.scale <= 3.4e38f)) {
-    q.scale = __int_as_float(0x7FFF0000);
-    q.center = 0.f;
+    q.scale = q.center = __int_as_float(0x7FFF0000);
     q.inv = 0.f;
   }
   return q;

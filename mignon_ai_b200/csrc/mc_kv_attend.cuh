@@ -127,7 +127,7 @@ __device__ __forceinline__ SlotSpan slot_span(const Cache& c, int len, int windo
 // gives every warp an item of its own, kAttendWarps one item to the CTA.
 template <int BITS, int DIM, int PLANES, int WPI>
 __global__ void __launch_bounds__(kAttendWarps * 32, 4) attend_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int HALVES = BITS == 4 ? 2 : 1;      // 32-slot halves of a tile
+  constexpr int HALVES = BITS == 4 && PLANES == 2 ? 2 : 1;  // 32-slot halves of a tile
   constexpr int TS = 32 * HALVES;
   constexpr int CB = DIM * BITS / 8;             // code bytes per slot
   constexpr int KS = (DIM + 31) / 32;            // MMA steps along the dimensions
@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 4) attend_kernel(const __gr
       big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
     }
     const float inv = row_inv_step(big);
-    // base 254: the first digit is in steps of big / 127; a row of non-finite queries stays so
-    qstep = __fmul_rn(__fmul_rn(row_step(big), a.scale), PLANES == 3 ? kOne / 254.0f : kOne / 254.0f);
+    // a non-finite query has no digits: its scores become NaN by qsum
+    qstep = __fmul_rn(__fmul_rn(row_step(big), a.scale), kOne / 254.0f);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       uint32_t u[8][3];
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 4) attend_kernel(const __gr
         pa[h][PLANES - 2][u] = __byte_perm(lo01, lo23, 0x7632);  // bytes 1
         if constexpr (PLANES == 3) {
           const uint32_t hi01 = __byte_perm(x[0], x[1], 0x0062), hi23 = __byte_perm(x[2], x[3], 0x0062);
-          pa[h][0][u] = __byte_perm(hi01, hi23, 0x5410) & 0x7F7F7F7Fu;  // bits 16-22
+          pa[h][0][u] = __byte_perm(hi01, hi23, 0x5410);  // bits 16-22
         }
       }
     // ---- the weighted values
