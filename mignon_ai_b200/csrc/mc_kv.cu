@@ -287,6 +287,8 @@ extern "C" int mc_kv_error(mc_kv* kv) {
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
   MC_CUDA(cudaDeviceSynchronize());
+  const int st = check_device_error(0);
+  if (st != kOk) return st;
   int code = 0;
   MC_CUDA(cudaMemcpy(&code, kv->c.error, sizeof(int), cudaMemcpyDeviceToHost));
   if (!code) return kOk;

@@ -3,107 +3,22 @@
 //   s_ij = scale q_i . k_j,  visible: j <= i and (j < sinks or j > i - window),
 //   o_i = sum_j softmax(s_i)_j v_j,  zero for a row that sees nothing.
 // A segment's queries are its last positions: query t of nq over nk keys is position nk - nq + t.
-#include "mc_kv.cuh"
+#include <type_traits>
+
+#include "mc_kv_attend.cuh"
+#include "mc_window_row.cuh"
+#include "mc_window_tc.cuh"
 
 namespace mc {
 namespace win {
 
-using kv::Rows;
-using kv::from_float;
-using kv::to_float;
-
-constexpr int kThreads = 256;
-constexpr int kMaxDim = 256;
-
-struct Args {
-  Rows q, k, v, out;
-  int n_q, n_k, n_seg, q_heads, heads, group, dim, window, sinks;
-  const int *q_start, *k_start;
-  float scale;  // of the scores, times log2(e)
-};
-
-// One query row by one warp, key by key: lane j scores keys j, j + 32, ..; then the lanes own
-// dimensions. Masked keys and values are not read, so whatever they hold reaches nothing.
-template <class T>
-__device__ void row_attention(const Args& a, int row, int h, int k0, int pos, float* qs) {
-  const int lane = threadIdx.x & 31, dim = a.dim, hk = h / a.group;
-  const T* q = static_cast<const T*>(a.q.p) + row * a.q.row + h * a.q.head;
-  T* out = static_cast<T*>(a.out.p) + row * a.out.row + h * a.out.head;
-  const T* k = static_cast<const T*>(a.k.p) + k0 * a.k.row + hk * a.k.head;
-  const T* v = static_cast<const T*>(a.v.p) + k0 * a.v.row + hk * a.v.head;
-  for (int d = lane; d < dim; d += 32) qs[d] = to_float<T>(q[d]);
-  __syncwarp();
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;  // first key of the window
-  const int sink_end = min(a.sinks, lo);                        // visible keys before it
-  float top = -INFINITY, total = 0.f, acc[kMaxDim / 32] = {};
-  const int n = sink_end + (pos + 1 - lo);
-  for (int t = 0; t < n; t += 32) {
-    const int i = t + lane;
-    const bool seen = i < n;
-    const int j = i < sink_end ? i : i - sink_end + lo;
-    float s = -INFINITY;
-    if (seen) {
-      float dot = 0.f;
-      for (int d = 0; d < dim; ++d) dot = __fmaf_rn(qs[d], to_float<T>(k[j * a.k.row + d]), dot);
-      s = __fmul_rn(dot, a.scale);
-    }
-    float m = s;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float other = __shfl_xor_sync(~0u, m, o);
-      m = m >= other || isnan(m) ? m : other;  // a NaN score stays
-    }
-    m = m >= top || isnan(m) ? m : top;
-    if (m == -INFINITY) continue;  // nothing but scores of minus infinity so far
-    const float keep = exp2f(__fsub_rn(top, m));
-    const float p = exp2f(__fsub_rn(s, m));
-    top = m;
-    total = __fmul_rn(total, keep) + p;  // per lane; summed over the lanes at the end
-#pragma unroll
-    for (int u = 0; u < kMaxDim / 32; ++u) acc[u] = __fmul_rn(acc[u], keep);
-    const int count = min(32, n - t);
-    for (int e = 0; e < count; ++e) {
-      const float pe = __shfl_sync(~0u, p, e);
-      const T* vr = v + __shfl_sync(~0u, j, e) * a.v.row;
-#pragma unroll
-      for (int u = 0; u < kMaxDim / 32; ++u) {
-        const int d = lane + 32 * u;
-        if (d < dim) acc[u] = __fmaf_rn(pe, to_float<T>(vr[d]), acc[u]);
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total = __fadd_rn(total, __shfl_xor_sync(~0u, total, o));
-#pragma unroll
-  for (int u = 0; u < kMaxDim / 32; ++u) {
-    const int d = lane + 32 * u;
-    if (d < dim) out[d] = from_float<T>(total == 0.f ? 0.f : __fdiv_rn(acc[u], total));
-  }
-}
-
-// The segment's queries and keys, with its bounds checked against the rows there are.
-struct Segment {
-  int q0, nq, k0, nk;
-};
-__device__ __forceinline__ Segment segment(const Args& a, int b) {
-  Segment s{0, a.n_q, 0, a.n_k};
-  if (a.q_start) {
-    s.q0 = a.q_start[b];
-    s.nq = a.q_start[b + 1] - s.q0;
-  }
-  if (a.k_start) {
-    s.k0 = a.k_start[b];
-    s.nk = a.k_start[b + 1] - s.k0;
-  }
-  if (s.q0 < 0 || s.nq < 0 || s.nq > a.n_q - s.q0 || s.k0 < 0 || s.nk < 0 || s.nk > a.n_k - s.k0) s = Segment{0, 0, 0, 0};
-  return s;
-}
+constexpr int kWindowRowThreads = 256;
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) row_kernel(const __grid_constant__ Args a) {
-  __shared__ float qs[kThreads / 32][kMaxDim];
+__global__ void __launch_bounds__(kWindowRowThreads) row_kernel(const __grid_constant__ Args a) {
+  __shared__ float qs[kWindowRowThreads / 32][kMaxDim];
   const int warp = threadIdx.x >> 5;
-  const long long item = (long long)blockIdx.x * (kThreads / 32) + warp;
+  const long long item = (long long)blockIdx.x * (kWindowRowThreads / 32) + warp;
   const int row = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
   if (row >= a.n_q) return;
   const int b = a.q_start ? kv::segment_of(a.q_start, a.n_seg, row) : 0;
@@ -111,6 +26,34 @@ __global__ void __launch_bounds__(kThreads) row_kernel(const __grid_constant__ A
   const Segment s = segment(a, b);
   if (s.nq == 0) return;
   row_attention<T>(a, row, h, s.k0, s.nk - s.nq + row - s.q0, qs[warp]);
+}
+
+// The tensor-core kernel takes head widths that are a multiple of its 16-wide products and rows that
+// TMA can fetch: 16-byte aligned addresses and strides.
+static bool tc_fits(const Args& a) {
+  auto fits = [](const Rows& r) {
+    return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.row % 8 == 0 && r.head % 8 == 0 && r.row > 0 && r.head > 0 &&
+           r.row < (1ll << 38) && r.head < (1ll << 38);
+  };
+  return a.dim % 16 == 0 && a.dim <= 128 && a.group <= 128 && a.n_k > 0 && fits(a.q) && fits(a.k) && fits(a.v);
+}
+
+template <class T>
+static int tc_launch(const Args& a, cudaStream_t stream) {
+  constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+  const int tokens = 128 / a.group;
+  TcArgs args{a, tokens, reinterpret_cast<uintptr_t>(a.out.p) % 16 == 0 && a.out.row % 8 == 0 && a.out.head % 8 == 0};
+  CUtensorMap mq, mk, mv;
+  if (!make_tmap_16(&mq, a.q.p, bf, a.dim, a.q_heads, a.n_q, 2 * a.q.head, 2 * a.q.row, a.group, tokens)) return kCudaError;
+  if (!make_tmap_16(&mk, a.k.p, bf, a.dim, a.heads, a.n_k, 2 * a.k.head, 2 * a.k.row, 1, kTcKeys)) return kCudaError;
+  if (!make_tmap_16(&mv, a.v.p, bf, a.dim, a.heads, a.n_k, 2 * a.v.head, 2 * a.v.row, 1, kTcKeys)) return kCudaError;
+  const size_t smem = tc_smem(a.dim);
+  MC_CUDA(cudaFuncSetAttribute(tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem(128)));
+  const long long tiles = a.n_q / tokens + (long long)a.n_seg;
+  if (tiles > INT_MAX || a.heads > 65535) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows or heads");
+  tc_kernel<T><<<dim3((unsigned)tiles, a.heads), kTcThreads, smem, stream>>>(mq, mk, mv, args);
+  MC_CUDA(cudaGetLastError());
+  return kOk;
 }
 
 }  // namespace win
@@ -137,10 +80,11 @@ extern "C" int mc_window_attn_dev(const mc_rows* q, const mc_rows* k, const mc_r
   if (n_q == 0 || n_segments == 0) return kOk;
   const Args a{kv::rows_of(q), kv::rows_of(k), kv::rows_of(v), kv::rows_of(out), n_q, n_k, n_segments, q_heads, kv_heads,
                q_heads / kv_heads, head_dim, window, sinks, q_start, k_start, scale * 1.4426950408889634f};
-  const long long blocks = ((long long)n_q * q_heads + kThreads / 32 - 1) / (kThreads / 32);
+  if (dtype != kv::kF32 && tc_fits(a)) return dtype == kv::kF16 ? tc_launch<__half>(a, (cudaStream_t)stream) : tc_launch<__nv_bfloat16>(a, (cudaStream_t)stream);
+  const long long blocks = ((long long)n_q * q_heads + kWindowRowThreads / 32 - 1) / (kWindowRowThreads / 32);
   if (blocks > INT_MAX) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows");
   void (*f)(Args) = dtype == kv::kF32 ? row_kernel<float> : dtype == kv::kF16 ? row_kernel<__half> : row_kernel<__nv_bfloat16>;
-  f<<<(unsigned)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  f<<<(unsigned)blocks, kWindowRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
   MC_CUDA(cudaGetLastError());
   return kOk;
 }

@@ -1,0 +1,297 @@
+// Window attention of 16-bit types on the 5th-generation tensor cores.
+//
+// A CTA takes 128 rows: TT = floor(128 / group) tokens times the group's query heads, which share
+// their keys and values, and walks the 128-key tiles that any of the rows sees. Per tile
+//   S = Q K^T      tcgen05 128 x 128 x dim, operands by TMA in the 128-byte swizzle, S in TMEM
+//   P = exp2(S - m) a thread owns a row (a TMEM lane): no exchange between threads
+//   O += P V       P from TMEM (over S's columns, 16-bit pairs), V as it lies in memory (MN-major)
+// The running maximum m is only raised when a row's tile maximum exceeds it by more than 8 (in
+// log2): until then the weights are at most 2^8 and nothing has to be rescaled; a raise rescales
+// O in TMEM. Weights are rounded to the operands' type for the product (as the output is), their sum
+// is not.
+//
+// Two CTAs share an SM (96 KB of operands and 256 TMEM columns each), so one's products run
+// under the other's exponentials: per tile the tensor pipe needs about 1000 cycles at dim 128 and
+// the exponentials as many.
+//
+// A hidden key's weight is an exact zero, but zero times an infinity or NaN among its values would
+// still reach the row. A row that comes out non-finite is therefore computed again key by key
+// (row_attention), which reads visible keys only.
+#pragma once
+#include "mc_window_row.cuh"
+
+namespace mc {
+namespace win {
+
+constexpr int kTcThreads = 192;          // 4 softmax warps, 1 TMA warp, 1 MMA warp
+constexpr int kTcKeys = 128;             // keys per tile
+constexpr int kTcBlock = 128 * 128;      // 128 rows x 64 16-bit values
+constexpr uint32_t kTcCols = 256;        // TMEM: S (P over it) | O
+
+struct TcArgs {
+  Args a;
+  int tokens;          // TT
+  int out_vec;         // output rows take 16-byte stores
+};
+
+constexpr size_t tc_smem(int dim) { return 1024 + 3 * (size_t)((dim + 63) / 64) * kTcBlock; }
+
+template <class T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kTcThreads, 2)
+tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+          const __grid_constant__ CUtensorMap mv, const __grid_constant__ TcArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[8];
+  __shared__ uint32_t tmem_slot;
+  __shared__ float redo[4][kMaxDim];
+  const Args& a = args.a;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int dim = a.dim, blocks = (dim + 63) / 64;
+  uint8_t* sq = smem;
+  uint8_t* sk = sq + blocks * kTcBlock;
+  uint8_t* sv = sk + blocks * kTcBlock;
+  uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 2, *s_full = bars + 3, *p_full = bars + 4,
+           *o_full = bars + 5, *v_free = bars + 6;
+
+  // ---- which tokens: tile ids are handed out so that segment b's begin at start / TT + b
+  const int tile_id = gridDim.x - 1 - blockIdx.x, hk = blockIdx.y, tt = args.tokens;
+  int b = 0;
+  if (a.q_start) {
+    int lo = 0, hi = a.n_seg;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.q_start[mid] / tt + mid <= tile_id) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+  }
+  const Segment seg = segment(a, b);
+  const int first = (tile_id - (a.q_start ? a.q_start[b] / tt + b : 0)) * tt;  // first token in the segment
+  if (first < 0 || first >= seg.nq) return;
+  const int tokens = min(tt, seg.nq - first);
+  const int pos0 = seg.nk - seg.nq + first, pos1 = pos0 + tokens - 1;  // positions of the first and last token
+  // tiles of keys: the sinks' (below the window) and the window's
+  const int win_lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+  const int win_tile = win_lo / kTcKeys;
+  const int sink_tiles = pos1 < 0 ? 0 : min(win_tile, (min(a.sinks, win_lo) + kTcKeys - 1) / kTcKeys);
+  const int n_tiles = pos1 < 0 ? 0 : sink_tiles + pos1 / kTcKeys - win_tile + 1;
+  auto tile_key = [&](int i) { return (i < sink_tiles ? i : win_tile + i - sink_tiles) * kTcKeys; };
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(k_full, 1);
+    mbar_init(v_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 128);
+    mbar_init(o_full, 1);
+    mbar_init(v_free, 1);
+    fence_barrier_init();
+  }
+  if (warp == 5) tmem_alloc(&tmem_slot, kTcCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t t_s = tmem, t_o = tmem + 128;
+  // rows [first, first + tokens) x group of the segment; the row of a thread
+  const int row_token = threadIdx.x / a.group, row_head = threadIdx.x % a.group;
+
+  if (warp == 4) {
+    if (lane == 0 && n_tiles > 0) {
+      bool ok = true;
+      mbar_arrive_expect_tx(q_full, (uint32_t)(blocks * tt * a.group * 128));
+      for (int c = 0; c < blocks; ++c) tma_load_3d(sq + c * kTcBlock, &mq, 64 * c, hk * a.group, seg.q0 + first, q_full);
+      int loads = 0;
+      for (int i = 0; i < n_tiles; ++i) {
+        const int key = seg.k0 + tile_key(i);
+        // the key buffer is free once the products of tile i - 1 are done: s_full's phase i - 1
+        if (i > 0 && !mbar_wait_or_abort(s_full, (i - 1) & 1, kErrWaitEmpty)) ok = false;
+        if (!ok) break;
+        mbar_arrive_expect_tx(k_full, (uint32_t)(blocks * kTcBlock));
+        for (int c = 0; c < blocks; ++c) tma_load_3d(sk + c * kTcBlock, &mk, 64 * c, hk, key, k_full);
+        if (i > 0 && !mbar_wait_or_abort(v_free, (i - 1) & 1, kErrWaitEmpty)) ok = false;
+        ++loads;
+        if (!ok) break;
+        mbar_arrive_expect_tx(v_full, (uint32_t)(blocks * kTcBlock));
+        for (int c = 0; c < blocks; ++c) tma_load_3d(sv + c * kTcBlock, &mv, 64 * c, hk, key, v_full);
+      }
+      // after a wait that gave up: never leave with copies in flight into this CTA's memory
+      if (!ok) {
+        mbar_wait(q_full, 0, kErrWaitFull);
+        if (loads > 0) mbar_wait(k_full, (loads - 1) & 1, kErrWaitFull);
+        if (loads > 1) mbar_wait(v_full, (loads - 2) & 1, kErrWaitFull);
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0 && n_tiles > 0) {
+      constexpr bool kBf = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+      const uint32_t id_s = idesc_f16(128, kTcKeys, kBf, false), id_o = idesc_f16(128, dim, kBf, true);
+      const uint64_t dq = smem_desc_sw128(sq), dk = smem_desc_sw128(sk), dv = smem_desc_sw128_mn(sv, kTcBlock);
+      auto scores = [&]() {
+        for (int k = 0; k < dim / 16; ++k) {
+          const uint64_t off = (uint64_t)((k >> 2) * (kTcBlock >> 4) + (k & 3) * 2);
+          mma_f16(t_s, dq + off, dk + off, id_s, k > 0);
+        }
+        mma_commit(s_full);
+      };
+      bool ok = mbar_wait_or_abort(q_full, 0, kErrWaitFull) && mbar_wait_or_abort(k_full, 0, kErrWaitFull);
+      if (ok) scores();
+      for (int i = 0; ok && i < n_tiles; ++i) {
+        ok = mbar_wait_or_abort(p_full, i & 1, kErrWaitAccFree) && mbar_wait_or_abort(v_full, i & 1, kErrWaitFull);
+        if (!ok) break;
+        tc_fence_after();
+        for (int k = 0; k < kTcKeys / 16; ++k)
+          mma_f16_ts(t_o, t_s + 8 * k, dv + (uint64_t)k * (2048 >> 4), id_o, i > 0 || k > 0);
+        mma_commit(i + 1 < n_tiles ? v_free : o_full);
+        if (i + 1 < n_tiles) {
+          ok = mbar_wait_or_abort(k_full, (i + 1) & 1, kErrWaitFull);
+          if (ok) scores();  // after the products that read P from the same columns: MMAs run in order
+        }
+      }
+      if (!ok) {  // a wait gave up: the MMAs issued so far end before TMEM is freed
+        mma_commit(o_full);
+        mbar_wait(o_full, 0, kErrWaitAcc);
+      }
+    }
+  } else {
+    const int pos = pos0 + row_token;  // of this thread's row
+    const bool real = row_token < tokens;
+    const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+    const uint32_t lane_off = (uint32_t)(32 * warp) << 16;
+    float top = -INFINITY, total = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int key = tile_key(i);
+      ok = __all_sync(~0u, mbar_wait_or_abort(s_full, i & 1, kErrWaitAcc));
+      if (!ok) break;
+      tc_fence_after();
+      // visible: key + c in [lo, pos] or below the sinks (which never lie past pos)
+      const int c_lo = lo - key, c_hi = pos - key, c_sink = min(a.sinks, pos + 1) - key;
+      const bool whole = __all_sync(~0u, c_hi >= kTcKeys - 1 && (c_lo <= 0 || c_sink >= kTcKeys));
+      // S is read twice, 64 columns at a time: for the maximum, then for the weights
+      float s[64];
+      auto load = [&](int c0) {
+        tmem_ld32(t_s + lane_off + c0, *reinterpret_cast<uint32_t(*)[32]>(s));
+        tmem_ld32(t_s + lane_off + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+        tmem_wait_ld();
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (!((c0 + c >= c_lo && c0 + c <= c_hi) || c0 + c < c_sink)) s[c] = -INFINITY;
+        }
+      };
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c0 = 0; c0 < kTcKeys; c0 += 64) {
+        load(c0);
+#pragma unroll
+        for (int c = 0; c < 64; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+      }
+      const float m = __fmul_rn(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), a.scale);
+      if (__any_sync(~0u, m > top + 8.f || (top == -INFINITY && m > top))) {
+        const float raised = fmaxf(top, m);
+        const float keep = top == -INFINITY ? 0.f : exp2f(__fsub_rn(top, raised));
+        total = __fmul_rn(total, keep);
+        top = raised;
+        if (i > 0) {
+          for (int c = 0; c < dim; c += 16) {
+            uint32_t x[16];
+            tmem_ld16(t_o + lane_off + c, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__fmul_rn(__uint_as_float(x[e]), keep));
+            tmem_st16(t_o + lane_off + c, x);
+          }
+        }
+      }
+      const float shift = top == -INFINITY ? 0.f : top;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int c0 = 0; c0 < kTcKeys; c0 += 64) {
+        load(c0);
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = kv::exp2_fast(__fmaf_rn(s[c + 2 * e], a.scale, -shift));
+            const float p1 = kv::exp2_fast(__fmaf_rn(s[c + 2 * e + 1], a.scale, -shift));
+            sum[0] = __fadd_rn(sum[0], p0);
+            sum[1] = __fadd_rn(sum[1], p1);
+            p[e] = pack16<T>(p0, p1);
+          }
+          // columns (c0 + c) / 2.. of P lie over scores that have been read for the last time
+          tmem_st16(t_s + lane_off + (c0 + c) / 2, p);
+        }
+      }
+      total = __fadd_rn(total, __fadd_rn(sum[0], sum[1]));
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(p_full);
+    }
+    // ---- the output row
+    if (ok && n_tiles > 0) ok = __all_sync(~0u, mbar_wait_or_abort(o_full, 0, kErrWaitAcc));
+    if (ok) {
+      tc_fence_after();
+      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
+      const int row = seg.q0 + first + row_token, h = hk * a.group + row_head;
+      T* out = static_cast<T*>(a.out.p) + row * a.out.row + h * a.out.head;
+      float bad = 0.f;
+      for (int c = 0; c < dim; c += 16) {
+        uint32_t x[16];
+        if (n_tiles > 0) {
+          tmem_ld16(t_o + lane_off + c, x);
+          tmem_wait_ld();
+        }
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v0 = __uint_as_float(x[2 * e]), v1 = __uint_as_float(x[2 * e + 1]);
+          if (n_tiles == 0) v0 = v1 = 0.f;
+          bad = __fmaf_rn(v0, 0.f, __fmaf_rn(v1, 0.f, bad));  // NaN once a value is not finite
+          y[e] = pack16<T>(__fmul_rn(v0, inv), __fmul_rn(v1, inv));
+        }
+        if (real && args.out_vec) {
+          *reinterpret_cast<uint4*>(out + c) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+        } else if (real) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const T* pair = reinterpret_cast<const T*>(&y[e]);
+            out[c + 2 * e] = pair[0];
+            out[c + 2 * e + 1] = pair[1];
+          }
+        }
+      }
+      bad = __fmaf_rn(total, 0.f, bad);
+      uint32_t again = __ballot_sync(~0u, real && !(bad == 0.f));
+      while (again) {
+        const int l = __ffs(again) - 1, r = 32 * warp + l;
+        again &= again - 1;
+        row_attention<T>(a, seg.q0 + first + r / a.group, hk * a.group + r % a.group, seg.k0, pos0 + r / a.group, redo[warp]);
+        __syncwarp();
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, kTcCols);
+}
+
+}  // namespace win
+}  // namespace mc
