@@ -8,6 +8,7 @@
 #include "mc_kv_attend.cuh"
 #include "mc_window_row.cuh"
 #include "mc_window_tc.cuh"
+#include "mc_window_tile.cuh"
 
 namespace mc {
 namespace win {
@@ -56,6 +57,21 @@ static int tc_launch(const Args& a, cudaStream_t stream) {
   return kOk;
 }
 
+template <class T>
+static int tile_launch(const Args& a, cudaStream_t stream) {
+  int dimp = 0;
+  auto f = tile_variant<T>(a.dim, &dimp);
+  const size_t smem = tile_smem(dimp);
+  MC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const long long tiles = a.n_q / (kTileRows / a.group) + (long long)a.n_seg;
+  if (tiles > INT_MAX || a.heads > 65535) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows or heads");
+  auto aligned = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.row % 4 == 0 && r.head % 4 == 0; };
+  const TileArgs args{a, std::is_same<T, float>::value && a.dim % 4 == 0 && aligned(a.k) && aligned(a.v)};
+  f<<<dim3((unsigned)tiles, a.heads), kTileThreads, smem, stream>>>(args);
+  MC_CUDA(cudaGetLastError());
+  return kOk;
+}
+
 }  // namespace win
 }  // namespace mc
 
@@ -81,6 +97,11 @@ extern "C" int mc_window_attn_dev(const mc_rows* q, const mc_rows* k, const mc_r
   const Args a{kv::rows_of(q), kv::rows_of(k), kv::rows_of(v), kv::rows_of(out), n_q, n_k, n_segments, q_heads, kv_heads,
                q_heads / kv_heads, head_dim, window, sinks, q_start, k_start, scale * 1.4426950408889634f};
   if (dtype != kv::kF32 && tc_fits(a)) return dtype == kv::kF16 ? tc_launch<__half>(a, (cudaStream_t)stream) : tc_launch<__nv_bfloat16>(a, (cudaStream_t)stream);
+  if (a.dim <= kTileMaxDim && a.group <= kTileRows)
+    return dtype == kv::kF32   ? tile_launch<float>(a, (cudaStream_t)stream)
+           : dtype == kv::kF16 ? tile_launch<__half>(a, (cudaStream_t)stream)
+                               : tile_launch<__nv_bfloat16>(a, (cudaStream_t)stream);
+  // wider heads and groups: a warp per row
   const long long blocks = ((long long)n_q * q_heads + kWindowRowThreads / 32 - 1) / (kWindowRowThreads / 32);
   if (blocks > INT_MAX) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows");
   void (*f)(Args) = dtype == kv::kF32 ? row_kernel<float> : dtype == kv::kF16 ? row_kernel<__half> : row_kernel<__nv_bfloat16>;

@@ -96,5 +96,17 @@ __device__ __forceinline__ Segment segment(const Args& a, int b) {
   return s;
 }
 
+// The tiled kernels hand out tiles of tt tokens so that segment b's begin at start[b] / tt + b: each
+// segment has room for all of its own, and a tile finds its segment by bisection.
+__device__ __forceinline__ int tile_segment(const int* start, int n, int tt, int tile) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] / tt + mid <= tile) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
 }  // namespace win
 }  // namespace mc

@@ -67,18 +67,8 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
   uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 2, *s_full = bars + 3, *p_full = bars + 4,
            *o_full = bars + 5, *v_free = bars + 6;
 
-  // ---- which tokens: tile ids are handed out so that segment b's begin at start / TT + b
   const int tile_id = gridDim.x - 1 - blockIdx.x, hk = blockIdx.y, tt = args.tokens;
-  int b = 0;
-  if (a.q_start) {
-    int lo = 0, hi = a.n_seg;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.q_start[mid] / tt + mid <= tile_id) lo = mid;
-      else hi = mid;
-    }
-    b = lo;
-  }
+  const int b = a.q_start ? tile_segment(a.q_start, a.n_seg, tt, tile_id) : 0;
   const Segment seg = segment(a, b);
   const int first = (tile_id - (a.q_start ? a.q_start[b] / tt + b : 0)) * tt;  // first token in the segment
   if (first < 0 || first >= seg.nq) return;

@@ -1,0 +1,290 @@
+// Window attention of float32 (and of 16-bit rows that TMA cannot fetch) on m16n8k8 tf32 MMAs.
+//
+// A float32 operand x is cut into hi = x with the low 13 bits cleared (tf32, 11 significant bits)
+// and lo = x - hi (exact); a product is hi*hi + hi*lo + lo*hi, whose error, about 2^-22 of
+// |a||b|, is float32's own size. 16-bit operands are exact in tf32 and their weights need no more
+// than tf32's bits before a 16-bit output: one product.
+//
+// A CTA of four warps takes 64 rows (tokens x the query heads that share a key/value head), a warp
+// 16 of them; keys and values of 64 positions at a time are staged as float32 in shared memory,
+// the next keys in flight behind the softmax and the value product, the next values behind the
+// score product (cp.async where rows are 16-byte aligned float32). Scores stay in
+// registers: the layout in which an MMA leaves them is the one its A operand wants if the k order
+// of the value product is taken as (2c, 2c + 1) for a thread's (c, c + 4). Row strides of dim + 8 and
+// dim + 4 floats keep the operands' shared loads free of bank conflicts.
+//
+// What bounds it: the three products at the legacy tensor rate (275 TFLOP/s of tf32 measured, so 92
+// of float32). Warps skip the 8-key columns that none of their 16 rows sees.
+#pragma once
+#include "mc_window_row.cuh"
+
+namespace mc {
+namespace win {
+
+constexpr int kTileThreads = 128;
+constexpr int kTileRows = 64;
+constexpr int kTileKeys = 64;
+constexpr int kTileMaxDim = 128;
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void cut(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xFFFFE000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
+}
+
+// d += a x b with a's and b's parts (PRODUCTS 1: the high parts alone)
+template <int PRODUCTS>
+__device__ __forceinline__ void mma_cut(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
+  uint32_t bh0, bl0, bh1, bl1;
+  cut(b0, bh0, bl0);
+  cut(b1, bh1, bl1);
+  if constexpr (PRODUCTS == 3) {
+    mma_tf32(d, al, bh0, bh1);
+    mma_tf32(d, ah, bl0, bl1);
+  }
+  mma_tf32(d, ah, bh0, bh1);
+}
+
+struct TileArgs {
+  Args a;
+  int vec;  // float32 rows of keys and values, 16-byte aligned, of a multiple of 4 dimensions
+};
+
+__device__ __forceinline__ void copy16_async(float* dst, const float* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Rows [0, count) of 64 staged with stride S, zeros past count and past the head's width.
+template <class T, int DIMP, int S>
+__device__ __forceinline__ void stage(float* dst, const T* src, long long stride, int count, int dim, bool vec) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (vec) {
+#pragma unroll 4
+      for (int e = threadIdx.x; e < kTileKeys * DIMP / 4; e += kTileThreads) {
+        const int j = e / (DIMP / 4), d = 4 * (e % (DIMP / 4));
+        const bool in = j < count && d < dim;
+        copy16_async(dst + j * S + d, src + (in ? j * stride + d : 0), in);
+      }
+      return;
+    }
+  }
+#pragma unroll 4
+  for (int e = threadIdx.x; e < kTileKeys * DIMP; e += kTileThreads) {
+    const int j = e / DIMP, d = e % DIMP;
+    dst[j * S + d] = j < count && d < dim ? to_float<T>(src[j * stride + d]) : 0.f;
+  }
+}
+
+inline size_t tile_smem(int dimp) { return (size_t)kTileKeys * (2 * dimp + 12) * sizeof(float) + 4 * kMaxDim * sizeof(float); }
+
+// DIMP: the head width rounded up to 16, 32, 64, 96 or 128 (dimensions past the width are zeros).
+template <class T, int DIMP>
+__global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(const __grid_constant__ TileArgs args) {
+  const Args& a = args.a;
+  constexpr int PRODUCTS = std::is_same<T, float>::value ? 3 : 1;
+  constexpr int KD = DIMP / 8;                   // MMA steps along the dimensions
+  constexpr int NK = kTileKeys / 8;              // 8-key columns of a tile
+  constexpr int SK = DIMP + 8, SV = DIMP + 4;    // row strides of the staged keys and values
+  extern __shared__ float sm[];
+  float* sk = sm;
+  float* sv = sk + kTileKeys * SK;
+  float* redo = sv + kTileKeys * SV;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+
+  const int tt = kTileRows / a.group, tile_id = gridDim.x - 1 - blockIdx.x, hk = blockIdx.y;
+  const int b = a.q_start ? tile_segment(a.q_start, a.n_seg, tt, tile_id) : 0;
+  const Segment seg = segment(a, b);
+  const int first = (tile_id - (a.q_start ? a.q_start[b] / tt + b : 0)) * tt;  // first token in the segment
+  if (first < 0 || first >= seg.nq) return;
+  const int tokens = min(tt, seg.nq - first);
+  const int base = seg.nk - seg.nq + first;  // position of the first token
+
+  // the warp's rows 16w + r and 16w + r + 8: tokens and heads, positions, bounds of what they see
+  int pos[2], lo[2], row[2], head[2];
+  bool real[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = 16 * warp + r + 8 * e, token = i / a.group;
+    real[e] = token < tokens;
+    pos[e] = real[e] ? base + token : -1;
+    lo[e] = a.window > 0 ? max(0, pos[e] - a.window + 1) : 0;
+    row[e] = seg.q0 + first + token;
+    head[e] = hk * a.group + i % a.group;
+  }
+  // positions of the CTA's and of the warp's first and last real rows
+  const int last_token = min(tokens - 1, (16 * warp + 15) / a.group), first_token = 16 * warp / a.group;
+  const int w_hi = first_token < tokens ? base + last_token : -1;
+  const int w_lo = a.window > 0 ? max(0, base + first_token - a.window + 1) : 0;  // the warp's first windowed key
+  const int cta_hi = base + tokens - 1, cta_lo = a.window > 0 ? max(0, base - a.window + 1) : 0;
+  const int win_tile = cta_lo / kTileKeys;
+  const int sink_tiles = cta_hi < 0 ? 0 : min(win_tile, (min(a.sinks, cta_lo) + kTileKeys - 1) / kTileKeys);
+  const int n_tiles = cta_hi < 0 ? 0 : sink_tiles + cta_hi / kTileKeys - win_tile + 1;
+
+  // ---- the queries' parts: step s, thread (r, c): dimensions 8s + 2c (a0, a1) and 8s + 2c + 1 (a2, a3)
+  float q[KD][4];
+#pragma unroll
+  for (int s = 0; s < KD; ++s)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int d = 8 * s + 2 * c + u;
+        float x = 0.f;
+        if (real[e] && d < a.dim) x = to_float<T>(static_cast<const T*>(a.q.p)[row[e] * a.q.row + head[e] * a.q.head + d]);
+        q[s][2 * u + e] = PRODUCTS == 3 ? __fmul_rn(x, a.scale) : x;  // 16-bit values stay exact in tf32
+      }
+  float o[DIMP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DIMP / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+  float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f};
+
+  const T* kbase = static_cast<const T*>(a.k.p) + seg.k0 * a.k.row + hk * a.k.head;
+  const T* vbase = static_cast<const T*>(a.v.p) + seg.k0 * a.v.row + hk * a.v.head;
+  auto tile_key = [&](int i) { return (i < sink_tiles ? i : win_tile + i - sink_tiles) * kTileKeys; };
+  auto load = [&](int i, bool values) {  // keys past cta_hi are seen by no row and stay zero
+    if (i < n_tiles) {
+      const int key = tile_key(i), count = min(kTileKeys, cta_hi + 1 - key);
+      if (values) stage<T, DIMP, SV>(sv, vbase + key * a.v.row, a.v.row, count, a.dim, args.vec);
+      else stage<T, DIMP, SK>(sk, kbase + key * a.k.row, a.k.row, count, a.dim, args.vec);
+    }
+    copies_commit();
+  };
+  load(0, false);
+  load(0, true);
+  for (int i = 0; i < n_tiles; ++i) {
+    const int key = tile_key(i);
+    // 8-key columns that some row of the warp sees
+    const int n_end = w_hi < key ? 0 : min(NK, (w_hi - key) / 8 + 1);
+    const int n_begin = key < a.sinks ? 0 : max(0, (w_lo - key) / 8);
+    copies_wait<1>();
+    __syncthreads();
+    float s[NK][4];
+#pragma unroll
+    for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KD; ++k) {
+      uint32_t ah[4], al[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) cut(q[k][e], ah[e], al[e]);
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        if (n < n_begin || n >= n_end) continue;
+        const float2 x = *reinterpret_cast<const float2*>(&sk[(8 * n + r) * SK + 8 * k + 2 * c]);
+        mma_cut<PRODUCTS>(s[n], ah, al, x.x, x.y);
+      }
+    }
+    __syncthreads();
+    load(i + 1, false);
+    // ---- what each row sees, its maximum, its weights. s[n][2e + u]: row e, key 8n + 2c + u
+    float keep[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j_lo = lo[e] - key - 2 * c, j_hi = pos[e] - key - 2 * c, j_sink = min(a.sinks, pos[e] + 1) - key - 2 * c;
+      float m = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int j = 8 * n + u;
+          if (n < n_begin || n >= n_end || !((j >= j_lo && j <= j_hi) || j < j_sink)) s[n][2 * e + u] = -INFINITY;
+          else if (PRODUCTS == 1) s[n][2 * e + u] = __fmul_rn(s[n][2 * e + u], a.scale);
+          m = fmaxf(m, s[n][2 * e + u]);
+        }
+      m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+      m = fmaxf(m, top[e]);
+      keep[e] = top[e] == -INFINITY ? 0.f : kv::exp2_fast(__fsub_rn(top[e], m));
+      top[e] = m;
+      const float shift = m == -INFINITY ? 0.f : m;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float p = kv::exp2_fast(__fsub_rn(s[n][2 * e + u], shift));
+          s[n][2 * e + u] = p;
+          sum = __fadd_rn(sum, p);
+        }
+      total[e] = __fmaf_rn(total[e], keep[e], sum);
+    }
+#pragma unroll
+    for (int d = 0; d < DIMP / 8; ++d) {
+      o[d][0] = __fmul_rn(o[d][0], keep[0]), o[d][1] = __fmul_rn(o[d][1], keep[0]);
+      o[d][2] = __fmul_rn(o[d][2], keep[1]), o[d][3] = __fmul_rn(o[d][3], keep[1]);
+    }
+    copies_wait<1>();
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      if (n < n_begin || n >= n_end) continue;
+      uint32_t ph[4], pl[4];
+      cut(s[n][0], ph[0], pl[0]);
+      cut(s[n][2], ph[1], pl[1]);
+      cut(s[n][1], ph[2], pl[2]);
+      cut(s[n][3], ph[3], pl[3]);
+#pragma unroll
+      for (int d = 0; d < DIMP / 8; ++d) {
+        const float* x = &sv[(8 * n + 2 * c) * SV + 8 * d + r];
+        mma_cut<PRODUCTS>(o[d], ph, pl, x[0], x[SV]);
+      }
+    }
+    __syncthreads();
+    load(i + 1, true);
+  }
+  // ---- the output rows: o[d][2e + u] is row e, dimension 8d + 2c + u
+  uint32_t again[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float sum = total[e];
+    sum = __fadd_rn(sum, __shfl_xor_sync(~0u, sum, 1));
+    sum = __fadd_rn(sum, __shfl_xor_sync(~0u, sum, 2));
+    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum);
+    float bad = __fmul_rn(sum, 0.f);
+    T* out = static_cast<T*>(a.out.p) + row[e] * a.out.row + head[e] * a.out.head;
+#pragma unroll
+    for (int d = 0; d < DIMP / 8; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float x = __fmul_rn(o[d][2 * e + u], inv);
+        bad = __fmaf_rn(x, 0.f, bad);  // NaN once a value is not finite
+        if (real[e] && 8 * d + 2 * c + u < a.dim) out[8 * d + 2 * c + u] = from_float<T>(x);
+      }
+    again[e] = __ballot_sync(~0u, real[e] && !(bad == 0.f));
+  }
+  // a non-finite row may have met a hidden key's infinity or NaN times its weight of zero: key by key
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    for (int i = 0; i < 8; ++i) {
+      if (!(again[e] & (0xFu << (4 * i)))) continue;
+      const int at = 16 * warp + 8 * e + i;
+      __syncwarp();
+      row_attention<T>(a, seg.q0 + first + at / a.group, hk * a.group + at % a.group, seg.k0, base + at / a.group,
+                       redo + warp * kMaxDim);
+    }
+}
+
+template <class T>
+inline void (*tile_variant(int dim, int* dimp))(TileArgs) {
+  *dimp = dim <= 16 ? 16 : dim <= 32 ? 32 : dim <= 48 ? 48 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
+  switch (*dimp) {
+    case 16: return tile_kernel<T, 16>;
+    case 32: return tile_kernel<T, 32>;
+    case 48: return tile_kernel<T, 48>;
+    case 64: return tile_kernel<T, 64>;
+    case 96: return tile_kernel<T, 96>;
+    default: return tile_kernel<T, 128>;
+  }
+}
+
+}  // namespace win
+}  // namespace mc
