@@ -16,75 +16,93 @@ namespace kv {
 constexpr int kCacheThreads = 256;
 
 // ------------------------------------------------------------------------------------------------
-// Write and read: one warp per (row, head), keys then values
+// Write and read
+//
+// Both move a row's codes between its dtype and the interleaved layout. A segment's rows go four
+// at a time: the rows of one group of slots (four consecutive slots, the first a multiple of
+// four), eight lanes to a row, a lane eight consecutive dimensions of it (and the eight 64 further
+// on). Then every access is a full word or vector: the keys' words of four rows are 16 consecutive
+// bytes, and the values' words, which hold one dimension of four rows, are made by a byte
+// transpose over the four rows' lanes (two shuffles). Rows that do not fill a group (the ends of a
+// segment, the two sides of a ring's end, single tokens) go one at a time by a whole warp.
+//
+// Bound by memory: the rows' bytes and the codes'.
 // ------------------------------------------------------------------------------------------------
 struct RowArgs {
   Cache c;
   Rows k, v;
   int n_rows, n_seg;
   const int *start, *sess, *pos0, *lens;
+  int vec;  // rows are aligned for 16-byte accesses of eight elements
 };
 
+// The last i of [0, n) for which `at_most` holds, by a whole warp with 32 probes a round (0 if it
+// holds nowhere; it must not hold again after it failed).
+template <class F>
+__device__ __forceinline__ int last_at_most(int n, F at_most) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const bool below = at < hi && (lane == 0 || at_most(at));
+    lo += (31 - __clz(__ballot_sync(~0u, below))) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+// Where a row goes or comes from: its session and slot, slot -1 for none.
 struct RowPlace {
   int session, slot;
 };
 
-// The warp's row: its session and slot; slot -1 where nothing is to be done.
-__device__ __forceinline__ RowPlace write_place(const RowArgs& a, int row) {
-  RowPlace w{0, -1};
-  const int b = segment_of(a.start, a.n_seg, row);
-  if (b < 0) return w;
-  const int first = a.start ? a.start[b] : row, rows = a.start ? a.start[b + 1] - first : 1;
-  w.session = a.sess ? a.sess[b] : b;
+// Row `row` of segment b, whose first row is `first` of `rows`.
+template <bool WRITE>
+__device__ __forceinline__ RowPlace place(const RowArgs& a, int b, int first, int rows, int row) {
+  RowPlace w{a.sess ? a.sess[b] : b, -1};
   const int pos0 = a.pos0[b];
   if ((unsigned)w.session >= (unsigned)a.c.sessions || pos0 < 0 || pos0 > INT_MAX - rows) {
     atomicExch(a.c.error, 1);
+    w.session = 0;
     return w;
   }
   const int pos = pos0 + (row - first);
-  // a segment longer than the ring: only the positions that it leaves behind are written
-  if (is_held(a.c, pos, pos0 + rows)) w.slot = slot_of(a.c, pos);
+  // writing a segment longer than the ring: only the positions that it leaves behind
+  if (is_held(a.c, pos, WRITE ? pos0 + rows : a.lens[b])) w.slot = slot_of(a.c, pos);
   return w;
 }
 
+__device__ __forceinline__ int signed_nibble(uint32_t byte, int high) { return (int)(byte << (high ? 24 : 28)) >> 28; }
+
+// One row by a warp: lanes own dimensions lane + 32u. `cs` holds kMaxDim codes of the warp's.
 template <class T>
-__global__ void __launch_bounds__(kCacheThreads) write_kernel(const __grid_constant__ RowArgs a) {
-  __shared__ int8_t codes[kCacheThreads / 32][kMaxDim];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
-  const int row = (int)(item / a.c.heads), head = (int)(item % a.c.heads);
-  if (row >= a.n_rows) return;
-  const RowPlace w = write_place(a, row);
-  if (w.slot < 0) return;
-  const int dim = a.c.dim, bits = a.c.bits, cb = a.c.cb;
+__device__ void write_row(const RowArgs& a, int row, int head, RowPlace w, int8_t* cs) {
+  const int lane = threadIdx.x & 31, dim = a.c.dim, bits = a.c.bits, cb = a.c.cb;
   uint8_t* region = region_of(a.c, w.session, head);
-  int8_t* cs = codes[warp];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const Rows& r = which ? a.v : a.k;
     const T* x = static_cast<const T*>(r.p) + row * r.row + head * r.head;
     float v[kMaxDim / 32];
-    float hi = -INFINITY, lo = INFINITY, bad = 0.f;
+    float hi = -INFINITY, lo = INFINITY;
 #pragma unroll
     for (int u = 0; u < kMaxDim / 32; ++u) {
       const int d = lane + 32 * u;
       if (d >= dim) break;
       v[u] = to_float<T>(x[d]);
-      hi = fmaxf(hi, v[u]);
-      lo = fminf(lo, v[u]);
-      bad = __fmaf_rn(v[u], 0.f, bad);  // NaN once an element is not finite
+      hi = max_nan(hi, v[u]);
+      lo = min_nan(lo, v[u]);
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-      bad = __fadd_rn(bad, __shfl_xor_sync(~0u, bad, o));
+      hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
+      lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
     }
-    const Quant q = quant_of(hi, lo, bad == 0.f, bits);
+    const Quant q = quant_of(hi, lo, bits);
 #pragma unroll
     for (int u = 0; u < kMaxDim / 32; ++u) {
       const int d = lane + 32 * u;
-      if (d < dim) cs[d] = (int8_t)code_of(q, v[u], bits);
+      if (d < dim) cs[d] = (int8_t)code_bits(q, v[u], bits);
     }
     __syncwarp();
     const int g = w.slot >> 2, s = w.slot & 3;
@@ -111,30 +129,12 @@ __global__ void __launch_bounds__(kCacheThreads) write_kernel(const __grid_const
   }
 }
 
-__device__ __forceinline__ int signed_nibble(uint32_t byte, int high) {
-  return (int)(byte << (high ? 24 : 28)) >> 28;
-}
-
 template <class T>
-__global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_constant__ RowArgs a) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
-  const int row = (int)(item / a.c.heads), head = (int)(item % a.c.heads);
-  if (row >= a.n_rows) return;
-  const int b = segment_of(a.start, a.n_seg, row);
-  int session = 0, pos = 0;
-  bool held = b >= 0;  // rows of no segment, and positions that are not held, come back as zeros
-  if (held) {
-    session = a.sess ? a.sess[b] : b;
-    const int ahead = a.start ? row - a.start[b] : 0;
-    held = (unsigned)session < (unsigned)a.c.sessions && a.pos0[b] >= 0 && a.pos0[b] <= INT_MAX - ahead;
-    if (!held) atomicExch(a.c.error, 1);
-    pos = held ? a.pos0[b] + ahead : 0;
-    held = held && is_held(a.c, pos, a.lens[b]);
-  }
-  const int dim = a.c.dim, bits = a.c.bits, cb = a.c.cb;
-  const int slot = held ? slot_of(a.c, pos) : 0, g = slot >> 2, s = slot & 3;
-  const uint8_t* region = region_of(a.c, held ? session : 0, head);
+__device__ void read_row(const RowArgs& a, int row, int head, RowPlace w) {
+  const int lane = threadIdx.x & 31, dim = a.c.dim, bits = a.c.bits, cb = a.c.cb;
+  const bool held = w.slot >= 0;
+  const int slot = held ? w.slot : 0, g = slot >> 2, s = slot & 3;
+  const uint8_t* region = region_of(a.c, w.session, head);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const Rows& r = which ? a.v : a.k;
@@ -146,18 +146,240 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_consta
     for (int d = lane; d < dim; d += 32) {
       float m = 0.f;
       if (held) {
+        uint32_t byte;
         if (which == 0) {
-          const int word = bits == 4 ? d / 8 : d / 4;
-          const uint32_t byte = codes[16 * word + 4 * s + d % 4];
-          m = bits == 4 ? (float)(2 * signed_nibble(byte, (d >> 2) & 1) + 1) : (float)(int8_t)byte;
+          byte = codes[16 * (bits == 4 ? d / 8 : d / 4) + 4 * s + d % 4];
         } else {
-          const int ni = cb / 8, n = d % 8, i = bits == 4 ? d / 16 : d / 8;
-          const uint32_t byte = codes[4 * (n * ni + i) + s];
-          m = bits == 4 ? (float)(2 * signed_nibble(byte, (d >> 3) & 1) + 1) : (float)(int8_t)byte;
+          byte = codes[4 * ((d % 8) * (cb / 8) + (bits == 4 ? d / 16 : d / 8)) + s];
         }
+        m = bits == 4 ? (float)(2 * signed_nibble(byte, (d >> (which ? 3 : 2)) & 1) + 1) : (float)(int8_t)byte;
       }
       y[d] = from_float<T>(held ? __fmaf_rn(scale, m, center) : 0.f);
     }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8], bool vec) {
+  if (vec) {
+    alignas(16) T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_float<T>(x[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(e)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = from_float<T>(x[i]);
+  }
+}
+
+// 4 x 4 bytes transposed over the four rows' lanes (s = lane / 8): lane s gives the bytes n of its
+// row and gets the bytes of dimension n = s, row 0's lowest. Its own inverse.
+__device__ __forceinline__ uint32_t transpose_bytes(uint32_t x, int s) {
+  uint32_t y = __shfl_xor_sync(~0u, x, 8);
+  x = s & 1 ? __byte_perm(y, x, 0x7351) : __byte_perm(x, y, 0x6240);  // rows 2t, 2t + 1 of n = s % 2 and s % 2 + 2
+  y = __shfl_xor_sync(~0u, x, 16);
+  return s & 2 ? __byte_perm(y, x, 0x7632) : __byte_perm(x, y, 0x5410);
+}
+
+// The four rows of one group of slots, lane (s, c): row s, dimensions 8c.. and 64 + 8c..
+template <class T, int BITS>
+__device__ void write_group(const RowArgs& a, int row0, int head, int session, int slot0) {
+  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
+  uint8_t* region = region_of(a.c, session, head);
+  uint32_t* params = reinterpret_cast<uint32_t*>(region + params_offset(a.c));
+  float x[2][2][8];
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const Rows& r = which ? a.v : a.k;
+    const T* p = static_cast<const T*>(r.p) + (row0 + s) * r.row + head * r.head;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (c0 + 8 * u < chunks) load8<T>(x[which][u], p + 8 * (c0 + 8 * u), a.vec);
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (c0 + 8 * u < chunks) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hi = max_nan(hi, x[which][u][e]), lo = min_nan(lo, x[which][u][e]);
+      }
+#pragma unroll
+    for (int o = 1; o <= 4; o <<= 1) {
+      hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
+      lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
+    }
+    const Quant q = quant_of(hi, lo, BITS);
+    uint32_t* out = reinterpret_cast<uint32_t*>(region + (which ? values_offset(a.c) : 0) + (long long)(slot0 >> 2) * 4 * cb);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (8 * u >= chunks) break;  // uniform
+      const int chunk = c0 + 8 * u;
+      const bool in = chunk < chunks;
+      uint32_t code[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) code[e] = code_bits(q, in ? x[which][u][e] : 0.f, BITS);
+      const uint32_t b0 = pack_low_bytes(code[0], code[1], code[2], code[3]);
+      const uint32_t b1 = pack_low_bytes(code[4], code[5], code[6], code[7]);
+      if (which == 0) {
+        if constexpr (BITS == 4) {
+          if (in) out[4 * chunk + s] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
+        } else if (in) {
+          out[8 * chunk + s] = b0;
+          out[8 * chunk + 4 + s] = b1;
+        }
+      } else if constexpr (BITS == 4) {
+        // even chunks (low nibbles) keep dimensions n = 0..3 of the pair, odd ones (high) n = 4..7
+        const bool odd = chunk & 1;
+        const uint32_t got = __shfl_xor_sync(~0u, odd ? b0 : b1, 1);
+        const uint32_t low = odd ? got : b0, high = odd ? b1 : got;
+        const uint32_t word = transpose_bytes((low & 0x0F0F0F0Fu) | ((high << 4) & 0xF0F0F0F0u), s);
+        if (in) out[(4 * (chunk & 1) + s) * (cb / 8) + (chunk >> 1)] = word;
+      } else {
+        const uint32_t w0 = transpose_bytes(b0, s), w1 = transpose_bytes(b1, s);
+        if (in) {
+          out[s * (cb / 8) + chunk] = w0;
+          out[(4 + s) * (cb / 8) + chunk] = w1;
+        }
+      }
+    }
+    if (c0 == 0) params[(which ? a.c.cap : 0) + slot0 + s] = param_word(q);
+  }
+}
+
+// Four codes as they are in bytes biased by 128: 2^23 + byte is a float whose low byte it is.
+__device__ __forceinline__ void decode4(float* x, uint32_t biased, float scale, float center) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float m = __fsub_rn(__uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7440 + e)), 8388736.0f);
+    x[e] = __fmaf_rn(scale, m, center);
+  }
+}
+
+template <class T, int BITS>
+__device__ void read_group(const RowArgs& a, int row0, int head, int session, int slot0) {
+  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
+  const uint8_t* region = region_of(a.c, session, head);
+  const uint32_t* params = reinterpret_cast<const uint32_t*>(region + params_offset(a.c)) + slot0 + s;
+  uint32_t w[2][2][2] = {};
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(region + (which ? values_offset(a.c) : 0) + (long long)(slot0 >> 2) * 4 * cb);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int chunk = c0 + 8 * u;
+      if (chunk >= chunks) break;
+      if constexpr (BITS == 4) {
+        w[which][u][0] = __ldg(in + (which ? (4 * (chunk & 1) + s) * (cb / 8) + (chunk >> 1) : 4 * chunk + s));
+      } else {
+        w[which][u][0] = __ldg(in + (which ? s * (cb / 8) + chunk : 8 * chunk + s));
+        w[which][u][1] = __ldg(in + (which ? (4 + s) * (cb / 8) + chunk : 8 * chunk + 4 + s));
+      }
+    }
+  }
+  const uint32_t param[2] = {__ldg(params), __ldg(params + a.c.cap)};
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const Rows& r = which ? a.v : a.k;
+    T* p = static_cast<T*>(r.p) + (row0 + s) * r.row + head * r.head;
+    // nibbles come as bytes 16c + 8 = 8m, so their scale is an eighth
+    const float scale = __fmul_rn(param_scale(param[which]), BITS == 4 ? 0.125f : 1.0f), center = param_center(param[which]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (8 * u >= chunks) break;  // uniform
+      const int chunk = c0 + 8 * u;
+      uint32_t b0, b1;
+      if constexpr (BITS == 4) {
+        const uint32_t word = w[which][u][0];
+        if (which == 0) {
+          b0 = low_codes(word), b1 = high_codes(word);
+        } else {
+          const uint32_t mine = transpose_bytes(word, s), other = __shfl_xor_sync(~0u, mine, 1);
+          b0 = chunk & 1 ? high_codes(other) : low_codes(mine);
+          b1 = chunk & 1 ? high_codes(mine) : low_codes(other);
+        }
+      } else {
+        b0 = which ? transpose_bytes(w[which][u][0], s) : w[which][u][0];
+        b1 = which ? transpose_bytes(w[which][u][1], s) : w[which][u][1];
+      }
+      float y[8];
+      decode4(y, b0 ^ 0x80808080u, scale, center);
+      decode4(y + 4, b1 ^ 0x80808080u, scale, center);
+      if (chunk < chunks) store8<T>(p + 8 * chunk, y, a.vec);
+    }
+  }
+}
+
+// One warp per (group of slots, head) of the segments. Segment b's groups have numbers from
+// start[b] / 4 + 2b on: room for its rows / 4 + 2, and it has no more whatever its first slot.
+template <class T, bool WRITE>
+__global__ void __launch_bounds__(kCacheThreads) segment_kernel(const __grid_constant__ RowArgs a) {
+  __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
+  const long long group = item / a.c.heads;
+  const int head = (int)(item % a.c.heads);
+  if constexpr (!WRITE) {  // rows before the first segment and after the last come back as zeros
+    const int lo = max(0, min(a.start[0], a.n_rows)), hi = max(lo, min(a.start[a.n_seg], a.n_rows));
+    for (long long e = item; e < (long long)(lo + a.n_rows - hi) * a.c.heads; e += (long long)gridDim.x * (kCacheThreads / 32)) {
+      const int i = (int)(e / a.c.heads);
+      read_row<T>(a, i < lo ? i : hi + i - lo, (int)(e % a.c.heads), RowPlace{0, -1});
+    }
+  }
+  const int b = last_at_most(a.n_seg, [&](int i) { return (a.start[i] >> 2) + 2ll * i <= group; });
+  const int first = a.start[b], rows = a.start[b + 1] - first;
+  const long long at = group - ((first >> 2) + 2ll * b);
+  if (rows <= 0 || first < 0 || rows > a.n_rows - first || at < 0) return;
+  const int offset = a.pos0[b] >= 0 ? slot_of(a.c, a.pos0[b]) & 3 : 0;  // of the segment's first row in its group
+  const long long begin = max(0ll, 4 * at - offset), end = min((long long)rows, 4 * at - offset + 4);
+  if (begin >= end) return;
+  const int row0 = first + (int)begin, count = (int)(end - begin);
+  // rows by lane: lane 8s + c asks for row s
+  const int s = lane >> 3;
+  const RowPlace p = place<WRITE>(a, b, first, rows, row0 + min(s, count - 1));
+  const int slot0 = __shfl_sync(~0u, p.slot, 0);
+  if (__all_sync(~0u, count == 4 && slot0 >= 0 && (slot0 & 3) == 0 && p.slot == slot0 + s)) {
+    if (a.c.bits == 4) {
+      if constexpr (WRITE) write_group<T, 4>(a, row0, head, p.session, slot0);
+      else read_group<T, 4>(a, row0, head, p.session, slot0);
+    } else {
+      if constexpr (WRITE) write_group<T, 8>(a, row0, head, p.session, slot0);
+      else read_group<T, 8>(a, row0, head, p.session, slot0);
+    }
+    return;
+  }
+  for (int i = 0; i < count; ++i) {
+    const RowPlace q{p.session, __shfl_sync(~0u, p.slot, 8 * i)};
+    if constexpr (WRITE) {
+      if (q.slot >= 0) write_row<T>(a, row0 + i, head, q, codes[warp]);
+    } else {
+      read_row<T>(a, row0 + i, head, q);
+    }
+  }
+}
+
+// One warp per (row, head): rows that are a segment of their own (no starts), and short segments.
+template <class T, bool WRITE>
+__global__ void __launch_bounds__(kCacheThreads) single_kernel(const __grid_constant__ RowArgs a) {
+  __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
+  const int warp = threadIdx.x >> 5;
+  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
+  const int row = (int)(item / a.c.heads), head = (int)(item % a.c.heads);
+  if (row >= a.n_rows) return;
+  RowPlace w{0, -1};
+  if (!a.start) {
+    w = place<WRITE>(a, row, row, 1, row);
+  } else if (row >= a.start[0] && row < a.start[a.n_seg]) {
+    const int b = last_at_most(a.n_seg, [&](int i) { return a.start[i] <= row; });
+    const int first = a.start[b], rows = a.start[b + 1] - first;
+    if (first >= 0 && row - first < rows && rows <= a.n_rows - first) w = place<WRITE>(a, b, first, rows, row);
+  }
+  if constexpr (WRITE) {
+    if (w.slot >= 0) write_row<T>(a, row, head, w, codes[warp]);
+  } else {
+    read_row<T>(a, row, head, w);
   }
 }
 
@@ -182,6 +404,18 @@ namespace kv {
 static bool rows_ok(const mc_rows* r) { return r && r->data; }
 static Rows rows_of(const mc_rows* r) { return Rows{r->data, (long long)r->row_stride, (long long)r->head_stride}; }
 
+template <bool SEGMENTS, class T>
+static void (*row_kernel_of(bool write))(RowArgs) {
+  if constexpr (SEGMENTS) return write ? segment_kernel<T, true> : segment_kernel<T, false>;
+  else return write ? single_kernel<T, true> : single_kernel<T, false>;
+}
+template <bool SEGMENTS>
+static void (*row_variant(int dtype, bool write))(RowArgs) {
+  return dtype == kF32   ? row_kernel_of<SEGMENTS, float>(write)
+         : dtype == kF16 ? row_kernel_of<SEGMENTS, __half>(write)
+                         : row_kernel_of<SEGMENTS, __nv_bfloat16>(write);
+}
+
 static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int n_rows,
                       const int32_t* start, const int32_t* sess, const int32_t* pos0, const int32_t* lens, int n_seg,
                       cudaStream_t stream) {
@@ -194,12 +428,17 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
   if (n_rows == 0 || n_seg == 0) return kOk;
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
-  const RowArgs a{kv->c, rows_of(k), rows_of(v), n_rows, n_seg, start, sess, pos0, lens};
-  const long long blocks = ((long long)n_rows * kv->c.heads + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
+  const int size = dtype == kF32 ? 4 : 2;
+  auto aligned = [&](const mc_rows* r) {  // for the 16-byte accesses of eight elements
+    return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
+  };
+  const RowArgs a{kv->c, rows_of(k), rows_of(v), n_rows, n_seg, start, sess, pos0, lens, aligned(k) && aligned(v)};
+  // Groups of slots pay once a segment has rows to fill them: GROUPS_RULE
+  const bool groups = start && n_rows >= 4ll * n_seg;
+  const long long warps = (groups ? n_rows / 4 + 2ll * n_seg : (long long)n_rows) * kv->c.heads;
+  const long long blocks = (warps + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
   if (blocks > INT_MAX) return set_error(kInvalidArgument, std::string(name) + ": too many rows");
-  void (*f)(RowArgs) = nullptr;
-  if (write) f = dtype == kF32 ? write_kernel<float> : dtype == kF16 ? write_kernel<__half> : write_kernel<__nv_bfloat16>;
-  else f = dtype == kF32 ? read_kernel<float> : dtype == kF16 ? read_kernel<__half> : read_kernel<__nv_bfloat16>;
+  auto f = groups ? row_variant<true>(dtype, write) : row_variant<false>(dtype, write);
   f<<<(unsigned)blocks, kCacheThreads, 0, stream>>>(a);
   MC_CUDA(cudaGetLastError());
   return kOk;
@@ -328,20 +567,26 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   const Cache& c = kv->c;
   const int group = q_heads / c.heads, row_groups = (group + kAttendRows - 1) / kAttendRows;
   const long long items = (long long)n * c.heads * row_groups;
-  // warps an item's slots are split over: enough for two waves of the 16 warps an SM holds, while
-  // each keeps two tiles of 64 slots
+  // Warps an item's slots are split over: as many as fill the 12 warps of every SM, while each keeps
+  // two tiles of 64 slots.
   const int seen = window > 0 ? (int)std::min<long long>(c.slots, (long long)window + c.sinks) : c.slots;
-  const long long wanted = std::min<long long>((2ll * 16 * kv->n_sm + items - 1) / items, (seen + 127) / 128);
+  const long long warps = 12ll * kv->n_sm, wanted = std::min<long long>(warps / items, (seen + 127) / 128);
   const bool split = wanted > 1;
   int pieces = 1;
-  if (split) pieces = (int)std::max<long long>(1, std::min<long long>((wanted + kAttendWarps - 1) / kAttendWarps, kMaxPartials / items));
-  const AttendArgs a{c, rows_of(q), rows_of(out), n, q_heads, group, row_groups, window, dtype, pieces, sessions, lens,
-                     scale * 1.4426950408889634f, kv->partial, kv->arrived};
-  const long long blocks = split ? items : (items + kAttendWarps - 1) / kAttendWarps;
-  if (blocks > INT_MAX) return set_error(kInvalidArgument, "mc_kv_attend_dev: too many rows");
+  if (split)
+    pieces = (int)std::max<long long>(1, std::min<long long>({wanted / kAttendWarps, kMaxPartials / items, kMaxPieces}));
+  const int size = dtype == kF32 ? 4 : 2;
+  auto aligned = [&](const mc_rows* r) {
+    return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
+  };
+  const AttendArgs a{c, rows_of(q), rows_of(out), n, q_heads, group, row_groups, window, dtype, aligned(q) && aligned(out),
+                     pieces, sessions, lens, scale * 1.4426950408889634f, kv->partial, kv->arrived};
+  if (items > INT_MAX) return set_error(kInvalidArgument, "mc_kv_attend_dev: too many rows");
+  const long long blocks = split ? items : std::min<long long>((items + kAttendWarps - 1) / kAttendWarps, warps / kAttendWarps);
   const int planes = dtype == kF32 ? 3 : 2;
-  auto f = c.bits == 4 ? attend_variant_of<4>(c.dim, planes, split) : attend_variant_of<8>(c.dim, planes, split);
-  f<<<dim3((unsigned)blocks, pieces), kAttendWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  const AttendVariant f = c.bits == 4 ? attend_variant_of<4>(c.dim, planes, split) : attend_variant_of<8>(c.dim, planes, split);
+  MC_CUDA(cudaFuncSetAttribute(f.f, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
+  f.f<<<dim3((unsigned)blocks, pieces), kAttendWarps * 32, f.smem, static_cast<cudaStream_t>(stream)>>>(a);
   MC_CUDA(cudaGetLastError());
   return kOk;
 }

@@ -102,7 +102,19 @@ struct Quant {
   float scale, center, inv;
 };
 
-__device__ __forceinline__ Quant quant_of(float hi, float lo, bool finite, int bits) {
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// hi and lo by max_nan and min_nan: either is not finite once an element is not.
+__device__ __forceinline__ Quant quant_of(float hi, float lo, int bits) {
   Quant q;
   q.center = __bfloat162float(__float2bfloat16_rn(__fadd_rn(__fmul_rn(0.5f, hi), __fmul_rn(0.5f, lo))));
   const float half = fmaxf(__fsub_rn(hi, q.center), __fsub_rn(q.center, lo));
@@ -110,7 +122,7 @@ __device__ __forceinline__ Quant quant_of(float hi, float lo, bool finite, int b
   q.scale = __uint_as_float((__float_as_uint(step) + 0xFFFFu) & 0xFFFF0000u);
   if (half < 0x1p-100f) q.scale = 0.f;
   q.inv = q.scale > 0.f ? __fdiv_rn(1.0f, q.scale) : 0.f;
-  if (!finite || !(fabsf(q.center) <= 3.4e38f) || !(q.scale <= 3.4e38f)) {
+  if (!(fabsf(hi) < INFINITY) || !(fabsf(lo) < INFINITY) || !(fabsf(q.center) < INFINITY) || !(q.scale < INFINITY)) {
     q.scale = q.center = __int_as_float(0x7FFF0000);
     q.inv = 0.f;
   }
@@ -123,25 +135,17 @@ __device__ __forceinline__ uint32_t param_word(const Quant& q) {
 __device__ __forceinline__ float param_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float param_center(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
-// The code of x: 4 bits: a nibble c in two's complement, m = 2c + 1; 8 bits: m itself.
-__device__ __forceinline__ int code_of(const Quant& q, float x, int bits) {
+// The code of x in the low bits of a word: 4 bits: c = floor(t / 2) of t = (x - center) / scale, m = 2c + 1
+// (a nibble in two's complement); 8 bits: m = t rounded to the nearest integer, ties to even. |t| stays below 16
+// or 127.5, so adding 1.5 * 2^24 rounded down (whose float spacing is 2), or 1.5 * 2^23, leaves them there.
+__device__ __forceinline__ uint32_t code_bits(const Quant& q, float x, int bits) {
   const float t = __fmul_rn(__fsub_rn(x, q.center), q.inv);
-  if (bits == 4) return (int)fminf(fmaxf(floorf(__fmul_rn(0.5f, t)), -8.f), 7.f);
-  return (int)fminf(fmaxf(rintf(t), -127.f), 127.f);
+  return __float_as_uint(bits == 4 ? __fadd_rd(t, 25165824.0f) : __fadd_rn(t, 12582912.0f));
 }
 
-// The segment of row r: the last b with start[b] <= r (null starts: one row per segment), or -1.
-__device__ __forceinline__ int segment_of(const int* start, int n, int r) {
-  if (!start) return r < n ? r : -1;
-  if (r < start[0] || r >= start[n]) return -1;
-  int lo = 0, hi = n;  // start[lo] <= r < start[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] <= r) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
+// A word of nibbles c (two's complement) as bytes 16c + 8 = 8m: the low and the high nibbles.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) | 0x08080808u; }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return (w & 0xF0F0F0F0u) | 0x08080808u; }
 
 }  // namespace kv
 }  // namespace mc

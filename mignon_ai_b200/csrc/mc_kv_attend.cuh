@@ -30,11 +30,13 @@ namespace kv {
 constexpr int kAttendWarps = 4;
 constexpr int kAttendRows = 8;          // query heads of one item
 constexpr int kMaxPartials = 2048;      // partial results (items x pieces) that fit the workspace
+constexpr int kMaxPieces = 128;         // pieces of one item
 
 struct AttendArgs {
   Cache c;
   Rows q, out;
   int n, q_heads, group, row_groups, window, dtype;
+  int vec;               // rows of q and out take 16-byte (eight elements) and pair accesses
   int pieces;            // CTAs an item's slots are split over
   const int *sess, *lens;
   float scale;           // of the scores, times log2(e)
@@ -54,25 +56,58 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A word of nibbles c (two's complement) as bytes 16c + 8 = 8m: the low and the high nibbles.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) | 0x08080808u; }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return (w & 0xF0F0F0F0u) | 0x08080808u; }
-
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-__device__ __forceinline__ float load_element(const void* p, long long i, int dtype) {
-  if (dtype == kF32) return static_cast<const float*>(p)[i];
-  if (dtype == kF16) return __half2float(static_cast<const __half*>(p)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// Eight consecutive elements.
+template <class T>
+__device__ __forceinline__ void load8(float (&x)[8], const T* p, bool vec) {
+  if constexpr (sizeof(T) == 4) {
+    if (vec) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p)), v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+      return;
+    }
+  } else {
+    if (vec) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = to_float<T>(p[i]);
 }
+
+__device__ __forceinline__ void load_query(float (&x)[8], const void* p, long long i, int dtype, bool vec) {
+  if (dtype == kF32) load8<float>(x, static_cast<const float*>(p) + i, vec);
+  else if (dtype == kF16) load8<__half>(x, static_cast<const __half*>(p) + i, vec);
+  else load8<__nv_bfloat16>(x, static_cast<const __nv_bfloat16*>(p) + i, vec);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 __device__ __forceinline__ void store_element(void* p, long long i, int dtype, float x) {
   if (dtype == kF32) static_cast<float*>(p)[i] = x;
   else if (dtype == kF16) static_cast<__half*>(p)[i] = __float2half_rn(x);
   else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+}
+
+// Elements i and i + 1, i even.
+__device__ __forceinline__ void store_pair(void* p, long long i, int dtype, bool vec, float x, float y) {
+  if (!vec) {
+    store_element(p, i, dtype, x);
+    store_element(p, i + 1, dtype, y);
+  } else if (dtype == kF32) {
+    *reinterpret_cast<float2*>(static_cast<float*>(p) + i) = make_float2(x, y);
+  } else if (dtype == kF16) {
+    *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i) = __floats2half2_rn(x, y);
+  } else {
+    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + i) = __floats2bfloat162_rn(x, y);
+  }
 }
 
 template <int N>
@@ -80,18 +115,18 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const uint32_t* p) 
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      const uint4 x = reinterpret_cast<const uint4*>(p)[i];
       w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
     }
   } else if constexpr (N % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p) + i);
+      const uint2 x = reinterpret_cast<const uint2*>(p)[i];
       w[2 * i] = x.x, w[2 * i + 1] = x.y;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = __ldg(p + i);
+    for (int i = 0; i < N; ++i) w[i] = p[i];
   }
 }
 
@@ -123,292 +158,383 @@ __device__ __forceinline__ SlotSpan slot_span(const Cache& c, int len, int windo
   return s;
 }
 
-// WPI warps of a CTA share an item (a session's up to eight query heads of one key/value head): 1
-// gives every warp an item of its own, kAttendWarps one item to the CTA.
+constexpr int attend_slots(int bits, int planes) { return bits == 4 && planes == 2 ? 64 : 32; }
+constexpr int attend_stage_bytes(int bits, int dim, int planes) {
+  return attend_slots(bits, planes) * (2 * dim * bits / 8 + 8);
+}
+// Tiles in flight per warp: what fits three CTAs of four warps on an SM.
+constexpr int attend_stages(int bits, int dim, int planes) {
+  const int n = 71680 / (kAttendWarps * attend_stage_bytes(bits, dim, planes));
+  return n > 4 ? 4 : n < 2 ? 2 : n;
+}
+constexpr int attend_smem(int bits, int dim, int planes) {
+  const int ring = kAttendWarps * attend_stages(bits, dim, planes) * attend_stage_bytes(bits, dim, planes);
+  const int join = kAttendWarps * kAttendRows * (dim + 2) * 4;  // the warps' results, in the same place
+  return ring > join ? ring : join;
+}
+
+// Where a warp is in its work: an item (a session's up to eight query heads of one key/value head)
+// and a tile of its visible slots.
+struct AttendCursor {
+  long long item;
+  int t, end;
+  int tiles0, first1;
+  const uint8_t* region;
+};
+
+// WPI warps of a CTA share an item: 1 gives every warp items of its own, one after the other with
+// the next one's tiles already in flight; kAttendWarps gives the CTA one piece of one item.
 template <int BITS, int DIM, int PLANES, int WPI>
-__global__ void __launch_bounds__(kAttendWarps * 32, 4) attend_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int HALVES = BITS == 4 && PLANES == 2 ? 2 : 1;  // 32-slot halves of a tile
-  constexpr int TS = 32 * HALVES;
+__global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int TS = attend_slots(BITS, PLANES), HALVES = TS / 32;
   constexpr int CB = DIM * BITS / 8;             // code bytes per slot
   constexpr int KS = (DIM + 31) / 32;            // MMA steps along the dimensions
   constexpr int NI = BITS == 4 ? DIM / 16 : DIM / 8;  // value words of a group of slots per thread
   constexpr int NT = DIM / 8;                    // 8-column tiles of the output
   constexpr float kOne = BITS == 4 ? 0.125f : 1.0f;   // the MMA's codes are 8m (4 bits) or m
+  constexpr int STAGES = attend_stages(BITS, DIM, PLANES), STAGE = attend_stage_bytes(BITS, DIM, PLANES);
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kAttendWarps][STAGES];
   const Cache& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
+  uint8_t* ring = smem + warp * STAGES * STAGE;
+  uint64_t* bars = full[warp];
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
 
-  long long item = WPI == 1 ? (long long)blockIdx.x * kAttendWarps + warp : blockIdx.x;
-  const int piece = WPI == 1 ? 0 : blockIdx.y;
   const int per = c.heads * a.row_groups;
-  if (WPI == 1 && item >= (long long)a.n * per) return;
-  const int b = (int)(item / per), hr = (int)(item % per), head = hr / a.row_groups, rg = hr % a.row_groups;
-  const int rows = min(kAttendRows, a.group - rg * kAttendRows);  // query heads of this item
-  const int h0 = head * a.group + rg * kAttendRows;
-  int session = a.sess ? a.sess[b] : b, len = 0;
-  if ((unsigned)session < (unsigned)c.sessions) {
-    len = a.lens[b];
-  } else {
-    if (lane == 0) atomicExch(c.error, 1);
-    session = 0;
-  }
-  const SlotSpan span = slot_span<TS>(c, len, a.window);
+  const long long items = (long long)a.n * per, stride = WPI == 1 ? (long long)gridDim.x * kAttendWarps : items;
+  const int piece = WPI == 1 ? 0 : blockIdx.y;
   const int part = WPI == 1 ? 0 : piece * WPI + warp, parts = WPI == 1 ? 1 : a.pieces * WPI;
-  const int t_begin = (int)((long long)span.tiles * part / parts), t_end = (int)((long long)span.tiles * (part + 1) / parts);
 
-  // ---- the queries as digit planes: thread (r, cc) holds row r's dimensions 8w..8w+7, w = cc + 4i
-  uint32_t qa[KS][PLANES][2];
-  float qstep, qsum = 0.f;
-  {
-    float x[KS][8], big = 0.f;
-    const long long base = b * a.q.row + (h0 + r) * a.q.head;
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      const int w = cc + 4 * i;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[i][e] = r < rows && 8 * w < DIM ? load_element(a.q.p, base + 8 * w + e, a.dtype) : 0.f;
-        qsum = __fadd_rn(qsum, x[i][e]);
-        big = fmaxf(big, fabsf(x[i][e]));
-      }
+  auto open = [&](AttendCursor& u, SlotSpan& span) {
+    const int b = (int)(u.item / per), head = (int)(u.item % per) / a.row_groups;
+    int session = a.sess ? a.sess[b] : b, len = 0;
+    if ((unsigned)session < (unsigned)c.sessions) {
+      len = a.lens[b];
+    } else {
+      if (lane == 0) atomicExch(c.error, 1);
+      session = 0;
     }
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      qsum = __fadd_rn(qsum, __shfl_xor_sync(~0u, qsum, o));
-      big = fmaxf(big, __shfl_xor_sync(~0u, big, o));
-    }
-    const float inv = row_inv_step(big);
-    // a non-finite query has no digits: its scores become NaN by qsum
-    qstep = __fmul_rn(__fmul_rn(row_step(big), a.scale), kOne / 254.0f);
-#pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      uint32_t u[8][3];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) slice3_bits(x[i][e], inv, u[e][0], u[e][1], u[e][2]);
-#pragma unroll
-      for (int p = 0; p < PLANES; ++p) {
-        qa[i][p][0] = pack_low_bytes(u[0][p], u[1][p], u[2][p], u[3][p]);
-        qa[i][p][1] = pack_low_bytes(u[4][p], u[5][p], u[6][p], u[7][p]);
-      }
-    }
-    qsum = __fmul_rn(qsum, a.scale);
-  }
+    span = slot_span<TS>(c, len, a.window);
+    u.t = (int)((long long)span.tiles * part / parts);
+    u.end = (int)((long long)span.tiles * (part + 1) / parts);
+    u.tiles0 = span.tiles0;
+    u.first1 = span.first1;
+    u.region = region_of(c, session, head);
+  };
+  auto slot_at = [](const AttendCursor& u, int t) { return (t < u.tiles0 ? t : u.first1 + t - u.tiles0) * TS; };
 
-  const uint8_t* region = region_of(c, session, head);
-  const uint8_t* kcodes = region;
-  const uint8_t* vcodes = region + values_offset(c);
-  const uint32_t* kparam = reinterpret_cast<const uint32_t*>(region + params_offset(c));
-  const uint32_t* vparam = kparam + c.cap;
+  // ---- the producer's side: lane 0 copies the tiles of this warp's items in their order
+  AttendCursor next{WPI == 1 ? (long long)blockIdx.x * kAttendWarps + warp : (long long)blockIdx.x, 0, 0, 0, 0, nullptr};
+  AttendCursor cur = next;
+  int issued = 0;
+  SlotSpan scratch;
+  if (next.item < items) open(next, scratch);
+  auto issue = [&]() {
+    while (next.t >= next.end) {
+      if (next.item >= items) return;
+      next.item += stride;
+      if (next.item >= items) return;
+      open(next, scratch);
+    }
+    if (lane == 0) {
+      const int slot0 = slot_at(next, next.t), stage = issued % STAGES;
+      uint8_t* dst = ring + stage * STAGE;
+      const uint8_t* codes = next.region + (long long)slot0 * CB;
+      const uint8_t* params = next.region + params_offset(c) + (long long)slot0 * 4;
+      mbar_arrive_expect_tx(bars + stage, STAGE);
+      bulk_load(dst, codes, TS * CB, bars + stage);
+      bulk_load(dst + TS * CB, codes + values_offset(c), TS * CB, bars + stage);
+      bulk_load(dst + 2 * TS * CB, params, TS * 4, bars + stage);
+      bulk_load(dst + 2 * TS * CB + TS * 4, params + (long long)c.cap * 4, TS * 4, bars + stage);
+    }
+    ++issued;
+    ++next.t;
+  };
+  for (int i = 0; i < STAGES; ++i) issue();
 
+  int done = 0;
+  bool ok = true;  // false after a wait gave up
   float o[NT][2];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = 0.f;
-  float top = -INFINITY, total = 0.f, csum = 0.f;
+  float top, total, csum;
+  int b, rows, h0;
+  for (; cur.item < items; cur.item += stride) {
+    SlotSpan span;
+    open(cur, span);
+    b = (int)(cur.item / per);
+    const int hr = (int)(cur.item % per), head = hr / a.row_groups, rg = hr % a.row_groups;
+    rows = min(kAttendRows, a.group - rg * kAttendRows);  // query heads of this item
+    h0 = head * a.group + rg * kAttendRows;
 
-  for (int t = t_begin; t < t_end; ++t) {
-    const int slot0 = (t < span.tiles0 ? t : span.first1 + t - span.tiles0) * TS;
-    // ---- scores: s[h][i][u] of slot 32h + 8cc + 4u + i
-    float s[HALVES][4][2];
-    uint4 vp[HALVES][2];
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h) {
-      const int base = slot0 + 32 * h;
-      const uint4* kp4 = reinterpret_cast<const uint4*>(kparam + base + 8 * cc);
-      const uint4* vp4 = reinterpret_cast<const uint4*>(vparam + base + 8 * cc);
-      const uint4 kp[2] = {__ldg(kp4), __ldg(kp4 + 1)};
-      vp[h][0] = __ldg(vp4);
-      vp[h][1] = __ldg(vp4 + 1);
-      const uint8_t* kc = kcodes + (long long)(base / 4 + r) * 4 * CB;
-      int acc[4][4] = {}, acc3[4][4] = {};
+    // ---- the queries as digit planes: thread (r, cc) holds row r's dimensions 8w..8w+7, w = cc + 4i
+    uint32_t qa[KS][PLANES][2];
+    float qstep, qsum = 0.f;
+    {
+      float x[KS][8], big = 0.f;
+      const long long base = b * a.q.row + (h0 + r) * a.q.head;
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         const int w = cc + 4 * i;
-        uint32_t b0[4], b1[4];
-        if (DIM % 32 == 0 || 8 * w < DIM) {
-          if constexpr (BITS == 4) {
-            uint32_t x[4];
-            load_words<4>(x, reinterpret_cast<const uint32_t*>(kc + 16 * w));
+        const bool in = r < rows && 8 * w < DIM;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b0[j] = low_codes(x[j]), b1[j] = high_codes(x[j]);
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+        if (in) load_query(x[i], a.q.p, base + 8 * w, a.dtype, a.vec);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          qsum = __fadd_rn(qsum, x[i][e]);
+          big = fmaxf(big, fabsf(x[i][e]));
+        }
+      }
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) {
+        qsum = __fadd_rn(qsum, __shfl_xor_sync(~0u, qsum, x));
+        big = fmaxf(big, __shfl_xor_sync(~0u, big, x));
+      }
+      const float inv = row_inv_step(big);
+      // a non-finite query has no digits: its scores become NaN by qsum
+      qstep = __fmul_rn(__fmul_rn(row_step(big), a.scale), kOne / 254.0f);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        uint32_t u[8][3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) slice3_bits(x[i][e], inv, u[e][0], u[e][1], u[e][2]);
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) {
+          qa[i][p][0] = pack_low_bytes(u[0][p], u[1][p], u[2][p], u[3][p]);
+          qa[i][p][1] = pack_low_bytes(u[4][p], u[5][p], u[6][p], u[7][p]);
+        }
+      }
+      qsum = __fmul_rn(qsum, a.scale);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = 0.f;
+    top = -INFINITY, total = 0.f, csum = 0.f;
+
+    for (int t = cur.t; t < cur.end; ++t) {
+      const int slot0 = slot_at(cur, t), stage = done % STAGES;
+      ok = __all_sync(~0u, ok && mbar_wait_or_abort(bars + stage, (done / STAGES) & 1, kErrWaitFull));
+      if (!ok) break;
+      const uint8_t* kcodes = ring + stage * STAGE;
+      const uint8_t* vcodes = kcodes + TS * CB;
+      const uint32_t* kparam = reinterpret_cast<const uint32_t*>(vcodes + TS * CB);
+      const uint32_t* vparam = kparam + TS;
+      // ---- scores: s[h][i][u] of slot 32h + 8cc + 4u + i
+      float s[HALVES][4][2];
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        const uint4* kp4 = reinterpret_cast<const uint4*>(kparam + 32 * h + 8 * cc);
+        const uint4 kp[2] = {kp4[0], kp4[1]};
+        const uint8_t* kc = kcodes + (8 * h + r) * 4 * CB;
+        int acc[4][4] = {}, acc3[4][4] = {};
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          const int w = cc + 4 * i;
+          uint32_t b0[4], b1[4];
+          if (DIM % 32 == 0 || 8 * w < DIM) {
+            if constexpr (BITS == 4) {
+              uint32_t x[4];
+              load_words<4>(x, reinterpret_cast<const uint32_t*>(kc + 16 * w));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) b0[j] = low_codes(x[j]), b1[j] = high_codes(x[j]);
+            } else {
+              load_words<4>(b0, reinterpret_cast<const uint32_t*>(kc + 32 * w));
+              load_words<4>(b1, reinterpret_cast<const uint32_t*>(kc + 32 * w + 16));
+            }
           } else {
-            load_words<4>(b0, reinterpret_cast<const uint32_t*>(kc + 32 * w));
-            load_words<4>(b1, reinterpret_cast<const uint32_t*>(kc + 32 * w + 16));
-          }
-        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b0[j] = b1[j] = 0;
+            for (int j = 0; j < 4; ++j) b0[j] = b1[j] = 0;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_s8s8(acc[j], qa[i][0][0], qa[i][1][0], qa[i][0][1], qa[i][1][1], b0[j], b1[j]);
+            if constexpr (PLANES == 3) mma_s8s8(acc3[j], qa[i][2][0], 0u, qa[i][2][1], 0u, b0[j], b1[j]);
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          mma_s8s8(acc[j], qa[i][0][0], qa[i][1][0], qa[i][0][1], qa[i][1][1], b0[j], b1[j]);
-          if constexpr (PLANES == 3) mma_s8s8(acc3[j], qa[i][2][0], 0u, qa[i][2][1], 0u, b0[j], b1[j]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            // |first| <= 128 * 127 * 127, so 254 * first + second fits 32 bits
+            float f = (float)(acc[j][u] * 254 + acc[j][2 + u]);
+            if constexpr (PLANES == 3) f = __fmaf_rn((float)acc3[j][u], 1.0f / 254.0f, f);
+            const uint32_t w = word_of(kp[u], j);
+            s[h][j][u] = __fmaf_rn(__fmul_rn(f, qstep), param_scale(w), __fmul_rn(param_center(w), qsum));
+          }
         }
       }
+      const bool whole = slot0 + TS <= span.e0 || (slot0 >= span.s1 && slot0 + TS <= span.e1);
+      if (!whole) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+        for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          // |first| <= 128 * 127 * 127, so 254 * first + second fits 32 bits
-          float f = (float)(acc[j][u] * 254 + acc[j][2 + u]);
-          if constexpr (PLANES == 3) f = __fmaf_rn((float)acc3[j][u], 1.0f / 254.0f, f);
-          const uint4 k4 = kp[u];
-          const uint32_t w = j == 0 ? k4.x : j == 1 ? k4.y : j == 2 ? k4.z : k4.w;
-          s[h][j][u] = __fmaf_rn(__fmul_rn(f, qstep), param_scale(w), __fmul_rn(param_center(w), qsum));
-        }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int slot = slot0 + 32 * h + 8 * cc + 4 * u + j;
+              if (!(slot < span.e0 || (slot >= span.s1 && slot < span.e1))) s[h][j][u] = -INFINITY;
+            }
       }
-    }
-    const bool whole = slot0 + TS <= span.e0 || (slot0 >= span.s1 && slot0 + TS <= span.e1);
-    if (!whole) {
+      // ---- running maximum and sum (a row's slots are on the four threads of its quad)
+      float m = top;
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(s[h][j][0], s[h][j][1]));
+      m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+      if (__any_sync(~0u, m > top)) {
+        const float keep = top == -INFINITY ? 0.f : exp2_fast(__fsub_rn(top, m));
+        total = __fmul_rn(total, keep);
+        csum = __fmul_rn(csum, keep);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[i][0] = __fmul_rn(o[i][0], keep), o[i][1] = __fmul_rn(o[i][1], keep);
+        top = m;
+      }
+      // ---- weights p, their sum, and p * vscale in place of the scores
+      float pmax = 0.f;
+      const float shift = top == -INFINITY ? 0.f : top;  // nothing but scores of minus infinity so far
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        const uint4* vp4 = reinterpret_cast<const uint4*>(vparam + 32 * h + 8 * cc);
+        const uint4 vp[2] = {vp4[0], vp4[1]};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int slot = slot0 + 32 * h + 8 * cc + 4 * u + j;
-            if (!(slot < span.e0 || (slot >= span.s1 && slot < span.e1))) s[h][j][u] = -INFINITY;
+            const float p = exp2_fast(__fsub_rn(s[h][j][u], shift));
+            uint32_t w = word_of(vp[u], j);
+            if (!whole && s[h][j][u] == -INFINITY) w = 0;  // a hidden slot may hold a scale of NaN
+            total = __fadd_rn(total, p);
+            csum = __fmaf_rn(p, param_center(w), csum);
+            s[h][j][u] = __fmul_rn(p, param_scale(w));
+            pmax = fmaxf(pmax, s[h][j][u]);
           }
-    }
-    // ---- running maximum and sum (a row's slots are on the four threads of its quad)
-    float m = top;
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(s[h][j][0], s[h][j][1]));
-    m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
-    if (__any_sync(~0u, m > top)) {
-      const float keep = top == -INFINITY ? 0.f : exp2_fast(__fsub_rn(top, m));
-      total = __fmul_rn(total, keep);
-      csum = __fmul_rn(csum, keep);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) o[i][0] = __fmul_rn(o[i][0], keep), o[i][1] = __fmul_rn(o[i][1], keep);
-      top = m;
-    }
-    // ---- weights p, their sum, and p * vscale in place of the scores
-    float pmax = 0.f;
-    const float shift = top == -INFINITY ? 0.f : top;  // nothing but scores of minus infinity so far
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float p = exp2_fast(__fsub_rn(s[h][j][u], shift));
-          const uint4 v4 = vp[h][u];
-          uint32_t w = j == 0 ? v4.x : j == 1 ? v4.y : j == 2 ? v4.z : v4.w;
-          if (!whole && s[h][j][u] == -INFINITY) w = 0;  // a hidden slot may hold a scale of NaN
-          total = __fadd_rn(total, p);
-          csum = __fmaf_rn(p, param_center(w), csum);
-          s[h][j][u] = __fmul_rn(p, param_scale(w));
-          pmax = fmaxf(pmax, s[h][j][u]);
-        }
-    pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 1));
-    pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 2));
-    // below 1e-30 the inverse leaves float32's range: such weights count as nothing
-    constexpr float kFull = PLANES == 3 ? 8388607.0f : 65535.0f;
-    const float inv = pmax > 1e-30f ? __fdividef(kFull, pmax) : 0.f;
-    const float unit = __fmul_rn(pmax > 1e-30f ? pmax : 0.f, kOne / kFull);
-    // ---- the weights' bytes as A operands: plane 0 (highest) in rows 0-7, plane 1 in rows 8-15
-    uint32_t pa[HALVES][PLANES][2];
-#pragma unroll
-    for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t x[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __float_as_uint(fminf(__fmaf_rn(s[h][j][u], inv, 8388608.0f), 8388608.0f + kFull));
-        const uint32_t lo01 = __byte_perm(x[0], x[1], 0x5140), lo23 = __byte_perm(x[2], x[3], 0x5140);
-        pa[h][PLANES - 1][u] = __byte_perm(lo01, lo23, 0x5410);  // bytes 0
-        pa[h][PLANES - 2][u] = __byte_perm(lo01, lo23, 0x7632);  // bytes 1
-        if constexpr (PLANES == 3) {
-          const uint32_t hi01 = __byte_perm(x[0], x[1], 0x0062), hi23 = __byte_perm(x[2], x[3], 0x0062);
-          pa[h][0][u] = __byte_perm(hi01, hi23, 0x5410);  // bits 16-22
-        }
       }
-    // ---- the weighted values
-    constexpr int STEP = BITS == 4 ? (NI % 4 == 0 ? 4 : NI % 2 == 0 ? 2 : 1) : (NI % 4 == 0 ? 4 : 2);
-#pragma unroll
-    for (int i0 = 0; i0 < NI; i0 += STEP) {
-      uint32_t v[HALVES][2][STEP];
+      pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 1));
+      pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 2));
+      // below 1e-30 the inverse leaves float32's range: such weights count as nothing
+      constexpr float kFull = PLANES == 3 ? 8388607.0f : 65535.0f;
+      const float inv = pmax > 1e-30f ? __fdividef(kFull, pmax) : 0.f;
+      const float unit = __fmul_rn(pmax > 1e-30f ? pmax : 0.f, kOne / kFull);
+      // ---- the weights' bytes as A operands: plane 0 (highest) in rows 0-7, plane 1 in rows 8-15
+      uint32_t pa[HALVES][PLANES][2];
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          load_words<STEP>(v[h][u], reinterpret_cast<const uint32_t*>(
-                                        vcodes + (long long)(slot0 / 4 + 8 * h + 2 * cc + u) * 4 * CB) + r * NI + i0);
+        for (int u = 0; u < 2; ++u) {
+          uint32_t x[4];
 #pragma unroll
-      for (int i = 0; i < STEP; ++i) {
-#pragma unroll
-        for (int nib = 0; nib < (BITS == 4 ? 2 : 1); ++nib) {
-          int acc[4] = {}, acc3[4] = {};
-#pragma unroll
-          for (int h = 0; h < HALVES; ++h) {
-            uint32_t b0 = v[h][0][i], b1 = v[h][1][i];
-            if constexpr (BITS == 4) {
-              b0 = nib ? high_codes(b0) : low_codes(b0);
-              b1 = nib ? high_codes(b1) : low_codes(b1);
-            }
-            mma_u8s8(acc, pa[h][0][0], pa[h][1][0], pa[h][0][1], pa[h][1][1], b0, b1);
-            if constexpr (PLANES == 3) mma_u8s8(acc3, pa[h][2][0], 0u, pa[h][2][1], 0u, b0, b1);
+          for (int j = 0; j < 4; ++j)
+            x[j] = __float_as_uint(fminf(__fmaf_rn(s[h][j][u], inv, 8388608.0f), 8388608.0f + kFull));
+          const uint32_t lo01 = __byte_perm(x[0], x[1], 0x5140), lo23 = __byte_perm(x[2], x[3], 0x5140);
+          pa[h][PLANES - 1][u] = __byte_perm(lo01, lo23, 0x5410);  // bytes 0
+          pa[h][PLANES - 2][u] = __byte_perm(lo01, lo23, 0x7632);  // bytes 1
+          if constexpr (PLANES == 3) {
+            const uint32_t hi01 = __byte_perm(x[0], x[1], 0x0062), hi23 = __byte_perm(x[2], x[3], 0x0062);
+            pa[h][0][u] = __byte_perm(hi01, hi23, 0x5410);  // bits 16-22
           }
-          const int nt = BITS == 4 ? 2 * (i0 + i) + nib : i0 + i;
+        }
+      // ---- the weighted values
+      constexpr int STEP = NI % 4 == 0 ? 4 : NI % 2 == 0 ? 2 : 1;
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            // |first| <= 255 * 127 * 64, so 256 * first + second fits 32 bits
-            float f = (float)(acc[u] * 256 + acc[2 + u]);
-            if constexpr (PLANES == 3) f = __fmaf_rn(f, 256.0f, (float)acc3[u]);
-            o[nt][u] = __fmaf_rn(f, unit, o[nt][u]);
+      for (int i0 = 0; i0 < NI; i0 += STEP) {
+        uint32_t v[HALVES][2][STEP];
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            load_words<STEP>(v[h][u], reinterpret_cast<const uint32_t*>(vcodes + (8 * h + 2 * cc + u) * 4 * CB) + r * NI + i0);
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) {
+#pragma unroll
+          for (int nib = 0; nib < (BITS == 4 ? 2 : 1); ++nib) {
+            int acc[4] = {}, acc3[4] = {};
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+              uint32_t b0 = v[h][0][i], b1 = v[h][1][i];
+              if constexpr (BITS == 4) {
+                b0 = nib ? high_codes(b0) : low_codes(b0);
+                b1 = nib ? high_codes(b1) : low_codes(b1);
+              }
+              mma_u8s8(acc, pa[h][0][0], pa[h][1][0], pa[h][0][1], pa[h][1][1], b0, b1);
+              if constexpr (PLANES == 3) mma_u8s8(acc3, pa[h][2][0], 0u, pa[h][2][1], 0u, b0, b1);
+            }
+            const int nt = BITS == 4 ? 2 * (i0 + i) + nib : i0 + i;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              // |first| <= 255 * 127 * 64, so 256 * first + second fits 32 bits
+              float f = (float)(acc[u] * 256 + acc[2 + u]);
+              if constexpr (PLANES == 3) f = __fmaf_rn(f, 256.0f, (float)acc3[u]);
+              o[nt][u] = __fmaf_rn(f, unit, o[nt][u]);
+            }
           }
         }
       }
+      ++done;
+      __syncwarp();  // every lane has read the stage: it takes the next tile
+      issue();
+    }
+    if (!ok) break;
+    // ---- the row's sums over its quad; the centers' share goes to every dimension
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+      total = __fadd_rn(total, __shfl_xor_sync(~0u, total, x));
+      csum = __fadd_rn(csum, __shfl_xor_sync(~0u, csum, x));
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[i][0] = __fadd_rn(o[i][0], csum), o[i][1] = __fadd_rn(o[i][1], csum);
+    // thread (r, cc) has dimensions 8i + 2cc and 8i + 2cc + 1 of row r
+    if constexpr (WPI == 1) {
+      if (r < rows) {
+        const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
+        const long long base = b * a.out.row + (h0 + r) * a.out.head;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          store_pair(a.out.p, base + 8 * i + 2 * cc, a.dtype, a.vec, __fmul_rn(o[i][0], inv), __fmul_rn(o[i][1], inv));
+      }
     }
   }
-  // ---- the row's sums over its quad; the centers' share goes to every dimension
-#pragma unroll
-  for (int x = 1; x <= 2; x <<= 1) {
-    total = __fadd_rn(total, __shfl_xor_sync(~0u, total, x));
-    csum = __fadd_rn(csum, __shfl_xor_sync(~0u, csum, x));
-  }
-#pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = __fadd_rn(o[i][0], csum), o[i][1] = __fadd_rn(o[i][1], csum);
-  // thread (r, cc) has dimensions 8i + 2cc and 8i + 2cc + 1 of row r
+  // a wait that gave up: never leave with copies in flight into this warp's buffers
+  if (!ok && lane == 0)
+    for (; done < issued; ++done) mbar_wait(bars + done % STAGES, (done / STAGES) & 1, kErrWaitFull);
 
-  if constexpr (WPI == 1) {
-    if (r < rows) {
-      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
-      const long long base = b * a.out.row + (h0 + r) * a.out.head;
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) store_element(a.out.p, base + 8 * i + 2 * cc + u, a.dtype, __fmul_rn(o[i][u], inv));
-    }
-  } else {
-    __shared__ float part_o[WPI][kAttendRows][DIM];
-    __shared__ float part_m[WPI][kAttendRows], part_l[WPI][kAttendRows];
+  if constexpr (WPI != 1) {
+    constexpr int W = 2 + DIM;  // maximum, sum, weighted values of a row
+    float* results = reinterpret_cast<float*>(smem);  // [warp][row][W], over the ring of tiles
+    __shared__ float keeps[kMaxPieces * kAttendRows];
     __shared__ int last;
-    if (cc == 0) part_m[warp][r] = top, part_l[warp][r] = total;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(&part_o[warp][r][8 * i + 2 * cc]) = make_float2(o[i][0], o[i][1]);
+    const long long item = blockIdx.x;
     __syncthreads();
-    constexpr int W = 2 + DIM;
-    float* mine = a.partial + (item * a.pieces + piece) * kAttendRows * W;
+    {
+      float* mine = results + (warp * kAttendRows + r) * W;
+      if (cc == 0) mine[0] = top, mine[1] = total;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) mine[2 + 8 * i + 2 * cc] = o[i][0], mine[3 + 8 * i + 2 * cc] = o[i][1];
+    }
+    __syncthreads();
+    float* out = a.partial + (item * a.pieces + piece) * kAttendRows * W;
     for (int e = threadIdx.x; e < rows * DIM; e += kAttendWarps * 32) {
       const int row = e / DIM, d = e % DIM;
       float m = -INFINITY, l = 0.f, x = 0.f;
 #pragma unroll
-      for (int w = 0; w < WPI; ++w) m = fmaxf(m, part_m[w][row]);
+      for (int w = 0; w < WPI; ++w) m = fmaxf(m, results[(w * kAttendRows + row) * W]);
 #pragma unroll
       for (int w = 0; w < WPI; ++w) {
+        const float* q = results + (w * kAttendRows + row) * W;
         // a part without visible slots has maximum -inf and sums of zero
-        const float keep = part_m[w][row] == -INFINITY ? 0.f : exp2_fast(__fsub_rn(part_m[w][row], m));
-        l = __fmaf_rn(part_l[w][row], keep, l);
-        x = __fmaf_rn(part_o[w][row][d], keep, x);
+        const float keep = q[0] == -INFINITY ? 0.f : exp2_fast(__fsub_rn(q[0], m));
+        l = __fmaf_rn(q[1], keep, l);
+        x = __fmaf_rn(q[2 + d], keep, x);
       }
       if (a.pieces == 1) {
         store_element(a.out.p, b * a.out.row + (h0 + row) * a.out.head + d, a.dtype, l == 0.f ? 0.f : __fdiv_rn(x, l));
       } else {
-        if (d == 0) mine[row * W] = m, mine[row * W + 1] = l;
-        mine[row * W + 2 + d] = x;
+        if (d == 0) out[row * W] = m, out[row * W + 1] = l;
+        out[row * W + 2 + d] = x;
       }
     }
     if (a.pieces == 1) return;
@@ -420,31 +546,58 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 4) attend_kernel(const __gr
     if (!last) return;
     __threadfence();
     const float* all = a.partial + item * a.pieces * kAttendRows * W;
-    for (int e = threadIdx.x; e < rows * DIM; e += kAttendWarps * 32) {
-      const int row = e / DIM, d = e % DIM;
-      float m = -INFINITY, l = 0.f, x = 0.f;
-      for (int p = 0; p < a.pieces; ++p) m = fmaxf(m, __ldcg(all + (p * kAttendRows + row) * W));
-#pragma unroll 4
-      for (int p = 0; p < a.pieces; ++p) {
-        const float* q = all + (p * kAttendRows + row) * W;
-        const float pm = __ldcg(q), keep = pm == -INFINITY ? 0.f : exp2_fast(__fsub_rn(pm, m));
-        l = __fmaf_rn(__ldcg(q + 1), keep, l);
-        x = __fmaf_rn(__ldcg(q + 2 + d), keep, x);
+    // the pieces' factors: a quarter-warp's worth of threads per row
+    {
+      const int row = threadIdx.x / 16, l16 = threadIdx.x % 16;  // 128 threads: eight rows
+      float m = -INFINITY, l = 0.f;
+      if (row < rows) {
+        for (int p = l16; p < a.pieces; p += 16) m = fmaxf(m, __ldcg(all + (p * kAttendRows + row) * W));
       }
-      store_element(a.out.p, b * a.out.row + (h0 + row) * a.out.head + d, a.dtype, l == 0.f ? 0.f : __fdiv_rn(x, l));
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
+      if (row < rows) {
+        for (int p = l16; p < a.pieces; p += 16) {
+          const float pm = __ldcg(all + (p * kAttendRows + row) * W), keep = pm == -INFINITY ? 0.f : exp2_fast(__fsub_rn(pm, m));
+          keeps[row * kMaxPieces + p] = keep;
+          l = __fmaf_rn(__ldcg(all + (p * kAttendRows + row) * W + 1), keep, l);
+        }
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) l = __fadd_rn(l, __shfl_xor_sync(~0u, l, x));
+      if (l16 == 0) results[row] = l;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (DIM / 2); e += kAttendWarps * 32) {
+      const int row = e / (DIM / 2), d = 2 * (e % (DIM / 2));
+      float x0 = 0.f, x1 = 0.f;
+#pragma unroll 16
+      for (int p = 0; p < a.pieces; ++p) {
+        const float2 q = __ldcg(reinterpret_cast<const float2*>(all + (p * kAttendRows + row) * W + 2 + d));
+        const float keep = keeps[row * kMaxPieces + p];
+        x0 = __fmaf_rn(q.x, keep, x0);
+        x1 = __fmaf_rn(q.y, keep, x1);
+      }
+      const float l = results[row], inv = l == 0.f ? 0.f : __fdiv_rn(1.0f, l);
+      store_pair(a.out.p, b * a.out.row + (h0 + row) * a.out.head + d, a.dtype, a.vec, __fmul_rn(x0, inv), __fmul_rn(x1, inv));
     }
     if (threadIdx.x == 0) a.arrived[item] = 0;
   }
 }
 
+struct AttendVariant {
+  void (*f)(AttendArgs);
+  int smem;
+};
+
 template <int BITS, int DIM>
-inline void (*attend_variant(int planes, bool split))(AttendArgs) {
-  if (planes == 3) return split ? attend_kernel<BITS, DIM, 3, kAttendWarps> : attend_kernel<BITS, DIM, 3, 1>;
-  return split ? attend_kernel<BITS, DIM, 2, kAttendWarps> : attend_kernel<BITS, DIM, 2, 1>;
+inline AttendVariant attend_variant(int planes, bool split) {
+  if (planes == 3)
+    return {split ? attend_kernel<BITS, DIM, 3, kAttendWarps> : attend_kernel<BITS, DIM, 3, 1>, attend_smem(BITS, DIM, 3)};
+  return {split ? attend_kernel<BITS, DIM, 2, kAttendWarps> : attend_kernel<BITS, DIM, 2, 1>, attend_smem(BITS, DIM, 2)};
 }
 
 template <int BITS>
-inline void (*attend_variant_of(int dim, int planes, bool split))(AttendArgs) {
+inline AttendVariant attend_variant_of(int dim, int planes, bool split) {
   switch (dim) {
     case 16: return attend_variant<BITS, 16>(planes, split);
     case 32: return attend_variant<BITS, 32>(planes, split);

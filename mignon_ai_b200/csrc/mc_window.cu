@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(kWindowRowThreads) row_kernel(const __grid_con
   const long long item = (long long)blockIdx.x * (kWindowRowThreads / 32) + warp;
   const int row = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
   if (row >= a.n_q) return;
-  const int b = a.q_start ? kv::segment_of(a.q_start, a.n_seg, row) : 0;
+  const int b = a.q_start ? segment_of(a.q_start, a.n_seg, row) : 0;
   if (b < 0) return;
   const Segment s = segment(a, b);
   if (s.nq == 0) return;

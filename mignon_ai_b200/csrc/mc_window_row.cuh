@@ -78,6 +78,19 @@ __device__ void row_attention(const Args& a, int row, int h, int k0, int pos, fl
   }
 }
 
+// The segment of row r: the last b with start[b] <= r (null starts: one row per segment), or -1.
+__device__ __forceinline__ int segment_of(const int* start, int n, int r) {
+  if (!start) return r < n ? r : -1;
+  if (r < start[0] || r >= start[n]) return -1;
+  int lo = 0, hi = n;  // start[lo] <= r < start[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= r) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
 // The segment's queries and keys, with its bounds checked against the rows there are.
 struct Segment {
   int q0, nq, k0, nk;

@@ -17,7 +17,8 @@ device, allocate at most their output and never synchronize. There is no CPU pat
 from __future__ import annotations
 
 import ctypes
-import math
+import struct
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -36,47 +37,65 @@ class _Spec(ctypes.Structure):
     _fields_ = [(n, _i) for n in ("sessions", "heads", "head_dim", "bits", "slots", "sinks")]
 
 
-_rows_p = ctypes.POINTER(_Rows)
 _lib.register({
     "mc_kv_open": [_i, ctypes.POINTER(_Spec), ctypes.POINTER(c_vp)],
     "mc_kv_close": [c_vp],
     "mc_kv_error": [c_vp],
-    "mc_kv_write_dev": [c_vp, _rows_p, _rows_p, _i, _i, c_vp, c_vp, c_vp, _i, c_vp],
-    "mc_kv_read_dev": [c_vp, _rows_p, _rows_p, _i, _i, c_vp, c_vp, c_vp, c_vp, _i, c_vp],
-    "mc_kv_attend_dev": [c_vp, _rows_p, _rows_p, _i, _i, c_vp, c_vp, _i, _i, ctypes.c_float, c_vp],
-    "mc_window_attn_dev": [_rows_p, _rows_p, _rows_p, _rows_p] + [_i] * 6 + [c_vp, c_vp, _i, _i, _i, ctypes.c_float, c_vp],
+    "mc_kv_write_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, c_vp, _i, c_vp],
+    "mc_kv_read_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, c_vp, c_vp, _i, c_vp],
+    "mc_kv_attend_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, _i, _i, ctypes.c_float, c_vp],
+    "mc_window_attn_dev": [c_vp, c_vp, c_vp, c_vp] + [_i] * 6 + [c_vp, c_vp, _i, _i, _i, ctypes.c_float, c_vp],
 })
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _check(name: str, x: torch.Tensor, device: torch.device, heads: Optional[int], dim: int,
-           dtype: Optional[torch.dtype] = None):
-    if x.dim() != 3 or x.shape[2] != dim or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{name}: expected [rows, {heads or 'heads'}, {dim}], got {tuple(x.shape)}")
-    if x.dtype not in _DTYPES or (dtype is not None and x.dtype != dtype):
-        raise TypeError(f"{name}: {x.dtype} (float32, float16 or bfloat16, the same in all tensors of a call)")
-    if x.device != device:
-        raise ValueError(f"{name}: on {x.device}, expected {device}")
-    if dim > 1 and x.stride(2) != 1:
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_pack = struct.Struct("12q").pack_into  # up to four mc_rows
+
+
+class _Scratch(threading.local):
+    """The mc_rows of a call (a thread's own: the library reads them while the GIL is released)."""
+
+    def __init__(self):
+        self.buf = ctypes.create_string_buffer(4 * ctypes.sizeof(_Rows))
+        at = ctypes.addressof(self.buf)
+        self.rows = tuple(at + i * ctypes.sizeof(_Rows) for i in range(4))
+
+
+_scratch = _Scratch()
+
+
+def _rows(name: str, x: torch.Tensor, index: int, heads: Optional[int], dim: int, dtype: torch.dtype,
+          count: Optional[int] = None) -> Tuple[int, int, int]:
+    """Address, row stride and head stride of rows [count, heads, dim] on device `index`."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads) or (
+            count is not None and shape[0] != count):
+        raise ValueError(f"{name}: expected [{'rows' if count is None else count}, {heads or 'heads'}, {dim}], got {tuple(shape)}")
+    if x.dtype is not dtype:
+        raise TypeError(f"{name}: {x.dtype}, expected {dtype}")
+    if x.get_device() != index:
+        raise ValueError(f"{name}: on {x.device}, expected cuda:{index}")
+    if stride[2] != 1 and dim > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-
-
-def _rows(x: torch.Tensor) -> _Rows:
     # an empty tensor has no address, and the library takes no null rows
-    return _Rows(x.data_ptr() or 16, x.stride(0), x.stride(1))
+    return x.data_ptr() or 16, stride[0], stride[1]
 
 
-def _ints(name: str, x: Optional[torch.Tensor], count: int, device: torch.device) -> Optional[int]:
+def _dtype(x: torch.Tensor) -> int:
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise TypeError(f"{x.dtype}: float32, float16 or bfloat16 rows are supported")
+    return code
+
+
+def _ints(name: str, x: Optional[torch.Tensor], count: int, index: int) -> Optional[int]:
     if x is None:
         return None
-    if x.dtype != torch.int32 or x.device != device or x.dim() != 1 or x.shape[0] != count or not x.is_contiguous():
-        raise ValueError(f"{name}: expected {count} contiguous int32 on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if x.dtype is not torch.int32 or x.get_device() != index or x.shape != (count,) or not x.is_contiguous():
+        raise ValueError(f"{name}: expected {count} contiguous int32 on cuda:{index}, got {x.dtype} {tuple(x.shape)} on {x.device}")
     return x.data_ptr()
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
 
 
 class KvCache:
@@ -92,6 +111,7 @@ class KvCache:
         _lib.check(_lib.lib().mc_kv_open(device, ctypes.byref(spec), ctypes.byref(self._h)))
         self.sessions, self.heads, self.head_dim, self.slots = sessions, heads, head_dim, slots
         self.bits, self.sinks, self.device = bits, sinks, torch.device("cuda", device)
+        self._lib, self._index, self._scale = _lib.lib(), device, head_dim ** -0.5
 
     def close(self):
         if self._h:
@@ -114,21 +134,22 @@ class KvCache:
         n = pos0.shape[0]
         if row_start is None and n != n_rows:
             raise ValueError(f"without row_start every row is a segment: {n_rows} rows, {n} positions")
-        return (_ints("row_start", row_start, n + 1, self.device), _ints("sessions", sessions, n, self.device),
-                _ints("pos0", pos0, n, self.device), n)
+        i = self._index
+        return _ints("row_start", row_start, n + 1, i), _ints("sessions", sessions, n, i), _ints("pos0", pos0, n, i), n
 
     def write(self, k: torch.Tensor, v: torch.Tensor, pos0: torch.Tensor, row_start: Optional[torch.Tensor] = None,
               sessions: Optional[torch.Tensor] = None):
         """Quantises rows into the cache: rows [row_start[b], row_start[b+1]) of k and v are
         positions pos0[b], pos0[b]+1, ... of session sessions[b] (default b). Without row_start
         every row is a segment of its own, as in a decode step."""
-        _check("k", k, self.device, self.heads, self.head_dim)
-        _check("v", v, self.device, self.heads, self.head_dim, k.dtype)
-        if v.shape[0] != k.shape[0]:
-            raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
-        start, sess, pos, n = self._segments(k.shape[0], pos0, row_start, sessions)
-        _lib.check(_lib.lib().mc_kv_write_dev(self._h, _rows(k), _rows(v), _DTYPES[k.dtype], k.shape[0], start, sess, pos,
-                                              n, _stream(self.device)))
+        code, n_rows, index, s = _dtype(k), k.shape[0], self._index, _scratch
+        _pack(s.buf, 0, *_rows("k", k, index, self.heads, self.head_dim, k.dtype),
+              *_rows("v", v, index, self.heads, self.head_dim, k.dtype, n_rows), 0, 0, 0, 0, 0, 0)
+        start, sess, pos, n = self._segments(n_rows, pos0, row_start, sessions)
+        status = self._lib.mc_kv_write_dev(self._h, s.rows[0], s.rows[1], code, n_rows, start, sess, pos, n,
+                                           _raw_stream(index))
+        if status:
+            _lib.check(status)
 
     def read(self, pos0: torch.Tensor, lens: torch.Tensor, row_start: Optional[torch.Tensor] = None,
              n_rows: Optional[int] = None, sessions: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float32,
@@ -141,15 +162,19 @@ class KvCache:
                 if row_start is not None:
                     raise ValueError("read: give n_rows (the last entry of row_start) or out")
                 n_rows = pos0.shape[0]
-            out = tuple(torch.empty((n_rows, self.heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-        k, v = out
-        _check("out[0]", k, self.device, self.heads, self.head_dim)
-        _check("out[1]", v, self.device, self.heads, self.head_dim, k.dtype)
-        if v.shape[0] != k.shape[0]:
-            raise ValueError(f"out: {k.shape[0]} and {v.shape[0]} rows")
-        start, sess, pos, n = self._segments(k.shape[0], pos0, row_start, sessions)
-        _lib.check(_lib.lib().mc_kv_read_dev(self._h, _rows(k), _rows(v), _DTYPES[k.dtype], k.shape[0], start, sess, pos,
-                                             _ints("lens", lens, n, self.device), n, _stream(self.device)))
+            k = torch.empty((n_rows, self.heads, self.head_dim), dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
+        else:
+            k, v = out
+            n_rows = k.shape[0]
+        code, index, s = _dtype(k), self._index, _scratch
+        _pack(s.buf, 0, *_rows("out[0]", k, index, self.heads, self.head_dim, k.dtype),
+              *_rows("out[1]", v, index, self.heads, self.head_dim, k.dtype, n_rows), 0, 0, 0, 0, 0, 0)
+        start, sess, pos, n = self._segments(n_rows, pos0, row_start, sessions)
+        status = self._lib.mc_kv_read_dev(self._h, s.rows[0], s.rows[1], code, n_rows, start, sess, pos,
+                                          _ints("lens", lens, n, index), n, _raw_stream(index))
+        if status:
+            _lib.check(status)
         return k, v
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, sessions: Optional[torch.Tensor] = None, window: int = 0,
@@ -157,18 +182,17 @@ class KvCache:
         """Attention of one query token per session: row i of q [n, q_heads, head_dim] belongs to
         session sessions[i] (default i), which has lens[i] positions, the query's own the last.
         scale defaults to 1 / sqrt(head_dim)."""
-        _check("q", q, self.device, None, self.head_dim)
+        code, index, s = _dtype(q), self._index, _scratch
+        rows = _rows("q", q, index, None, self.head_dim, q.dtype)
+        n, q_heads, _ = q.shape
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        else:
-            _check("out", out, self.device, q.shape[1], self.head_dim, q.dtype)
-            if out.shape[0] != q.shape[0]:
-                raise ValueError(f"out has {out.shape[0]} rows, q {q.shape[0]}")
-        n = q.shape[0]
-        _lib.check(_lib.lib().mc_kv_attend_dev(
-            self._h, _rows(q), _rows(out), _DTYPES[q.dtype], q.shape[1], _ints("sessions", sessions, n, self.device),
-            _ints("lens", lens, n, self.device), n, window, 1 / math.sqrt(self.head_dim) if scale is None else scale,
-            _stream(self.device)))
+            out = torch.empty_like(q)
+        _pack(s.buf, 0, *rows, *_rows("out", out, index, q_heads, self.head_dim, q.dtype, n), 0, 0, 0, 0, 0, 0)
+        status = self._lib.mc_kv_attend_dev(
+            self._h, s.rows[0], s.rows[1], code, q_heads, _ints("sessions", sessions, n, index),
+            _ints("lens", lens, n, index), n, window, self._scale if scale is None else scale, _raw_stream(index))
+        if status:
+            _lib.check(status)
         return out
 
 
@@ -179,28 +203,29 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     head_dim] over keys [k_start[b], k_start[b+1]) of k and v [rows, heads, head_dim]. A segment's
     queries are its last positions (k_start defaults to q_start; both None: one segment). A row
     that sees nothing is zero; rows of no segment are not written."""
-    device, dim = q.device, q.shape[-1]
-    if device.type != "cuda":
+    index, dim, dtype, s = q.get_device(), q.shape[-1], q.dtype, _scratch
+    if index < 0:
         raise ValueError("q: expected a CUDA tensor")
-    _check("q", q, device, None, dim)
-    _check("k", k, device, None, dim, q.dtype)
-    _check("v", v, device, k.shape[1], dim, q.dtype)
-    if v.shape[0] != k.shape[0]:
-        raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
-    if q_start is None and k_start is not None:
-        raise ValueError("k_start without q_start")
+    code = _dtype(q)
+    if out is None:
+        out = torch.empty_like(q)
+    q_rows, k_rows = _rows("q", q, index, None, dim, dtype), _rows("k", k, index, None, dim, dtype)
+    n_q, q_heads, _ = q.shape
+    n_k, heads, _ = k.shape
+    _pack(s.buf, 0, *q_rows, *k_rows, *_rows("v", v, index, heads, dim, dtype, n_k),
+          *_rows("out", out, index, q_heads, dim, dtype, n_q))
     if k_start is None:
         k_start = q_start
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    else:
-        _check("out", out, device, q.shape[1], dim, q.dtype)
-        if out.shape[0] != q.shape[0]:
-            raise ValueError(f"out has {out.shape[0]} rows, q {q.shape[0]}")
+    elif q_start is None:
+        raise ValueError("k_start without q_start")
     n = 1 if q_start is None else q_start.shape[0] - 1
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().mc_window_attn_dev(
-            _rows(q), _rows(k), _rows(v), _rows(out), _DTYPES[q.dtype], q.shape[1], k.shape[1], dim, q.shape[0], k.shape[0],
-            _ints("q_start", q_start, n + 1, device), _ints("k_start", k_start, n + 1, device), n, window, sinks,
-            1 / math.sqrt(dim) if scale is None else scale, _stream(device)))
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return window_attention(q, k, v, q_start, k_start, window, sinks, scale, out)
+    status = _lib.lib().mc_window_attn_dev(
+        *s.rows, code, q_heads, heads, dim, n_q, n_k, _ints("q_start", q_start, n + 1, index),
+        _ints("k_start", k_start, n + 1, index), n, window, sinks, dim ** -0.5 if scale is None else scale,
+        _raw_stream(index))
+    if status:
+        _lib.check(status)
     return out

@@ -29,7 +29,7 @@ def test_null_arguments():
     assert L.mc_kv_open(0, None, None) == INVALID
     assert L.mc_kv_error(None) == INVALID
     assert L.mc_kv_close(None) == 0
-    r = kv._Rows(16, 64, 64)
+    r = ctypes.byref(kv._Rows(16, 64, 64))
     assert L.mc_kv_write_dev(None, r, r, 0, 1, None, None, 16, 1, None) == INVALID
     assert L.mc_kv_read_dev(None, r, r, 0, 1, None, None, 16, 16, 1, None) == INVALID
     assert L.mc_kv_attend_dev(None, r, r, 0, 2, None, 16, 1, 0, 1.0, None) == INVALID
@@ -44,13 +44,13 @@ WINDOW = dict(dtype=0, q_heads=4, kv_heads=2, head_dim=64, n_q=5, n_k=5, q_start
                                  dict(q_start=16), dict(window=-1), dict(sinks=-1), dict(scale=0.0),
                                  dict(scale=float("inf")), dict(scale=float("nan"))])
 def test_window_refuses(bad):
-    r = kv._Rows(16, 64, 64)
+    r = ctypes.byref(kv._Rows(16, 64, 64))
     args = list({**WINDOW, **bad}.values())
     assert _lib.lib().mc_window_attn_dev(r, r, r, r, *args, None) == INVALID
     assert _lib.lib().mc_last_error()
 
 
 def test_window_takes_no_null_rows_and_nothing_to_do():
-    r, null = kv._Rows(16, 64, 64), kv._Rows(None, 64, 64)
+    r, null = ctypes.byref(kv._Rows(16, 64, 64)), ctypes.byref(kv._Rows(None, 64, 64))
     assert _lib.lib().mc_window_attn_dev(null, r, r, r, *WINDOW.values(), None) == INVALID
     assert _lib.lib().mc_window_attn_dev(r, r, r, r, *{**WINDOW, "n_q": 0}.values(), None) == 0
