@@ -105,26 +105,25 @@ __device__ void write_row(const RowArgs& a, int row, int head, RowPlace w, int8_
       if (d < dim) cs[d] = (int8_t)code_bits(q, v[u], bits);
     }
     __syncwarp();
-    const int g = w.slot >> 2, s = w.slot & 3;
+    const int s = w.slot & 3;
+    uint32_t* group = codes_of(a.c, region, w.slot, which);
     if (which == 0) {
-      uint32_t* out = reinterpret_cast<uint32_t*>(region + (long long)g * 4 * cb);
       for (int i = lane; i < cb / 4; i += 32) {
         uint32_t word = 0;
         for (int b = 0; b < 4; ++b)
           word |= (uint32_t)(bits == 4 ? (cs[8 * i + b] & 15) | ((cs[8 * i + 4 + b] & 15) << 4) : (uint8_t)cs[4 * i + b])
                   << (8 * b);
-        out[4 * i + s] = word;
+        group[4 * i + s] = word;
       }
     } else {
-      uint8_t* out = region + values_offset(a.c) + (long long)g * 4 * cb;
+      uint8_t* out = reinterpret_cast<uint8_t*>(group);
       const int ni = cb / 8;
       for (int j = lane; j < cb; j += 32) {
         const int n = j / ni, i = j % ni;
         out[4 * j + s] = (uint8_t)(bits == 4 ? (cs[16 * i + n] & 15) | ((cs[16 * i + 8 + n] & 15) << 4) : cs[8 * i + n]);
       }
     }
-    if (lane == 0)
-      reinterpret_cast<uint32_t*>(region + params_offset(a.c))[(which ? a.c.cap : 0) + w.slot] = param_word(q);
+    if (lane == 0) *params_of(a.c, region, w.slot, which) = param_word(q);
     __syncwarp();
   }
 }
@@ -133,15 +132,14 @@ template <class T>
 __device__ void read_row(const RowArgs& a, int row, int head, RowPlace w) {
   const int lane = threadIdx.x & 31, dim = a.c.dim, bits = a.c.bits, cb = a.c.cb;
   const bool held = w.slot >= 0;
-  const int slot = held ? w.slot : 0, g = slot >> 2, s = slot & 3;
-  const uint8_t* region = region_of(a.c, w.session, head);
+  const int slot = held ? w.slot : 0, s = slot & 3;
+  uint8_t* region = region_of(a.c, w.session, head);
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const Rows& r = which ? a.v : a.k;
     T* y = static_cast<T*>(r.p) + row * r.row + head * r.head;
-    const uint8_t* codes = region + (which ? values_offset(a.c) : 0) + (long long)g * 4 * cb;
-    uint32_t param = 0;
-    if (held) param = reinterpret_cast<const uint32_t*>(region + params_offset(a.c))[(which ? a.c.cap : 0) + slot];
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(codes_of(a.c, region, slot, which));
+    const uint32_t param = held ? *params_of(a.c, region, slot, which) : 0;
     const float scale = param_scale(param), center = param_center(param);
     for (int d = lane; d < dim; d += 32) {
       float m = 0.f;
@@ -187,7 +185,6 @@ template <class T, int BITS>
 __device__ void write_group(const RowArgs& a, int row0, int head, int session, int slot0) {
   const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
   uint8_t* region = region_of(a.c, session, head);
-  uint32_t* params = reinterpret_cast<uint32_t*>(region + params_offset(a.c));
   float x[2][2][8];
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
@@ -212,7 +209,7 @@ __device__ void write_group(const RowArgs& a, int row0, int head, int session, i
       lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
     }
     const Quant q = quant_of(hi, lo, BITS);
-    uint32_t* out = reinterpret_cast<uint32_t*>(region + (which ? values_offset(a.c) : 0) + (long long)(slot0 >> 2) * 4 * cb);
+    uint32_t* out = codes_of(a.c, region, slot0, which);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (8 * u >= chunks) break;  // uniform
@@ -245,7 +242,7 @@ __device__ void write_group(const RowArgs& a, int row0, int head, int session, i
         }
       }
     }
-    if (c0 == 0) params[(which ? a.c.cap : 0) + slot0 + s] = param_word(q);
+    if (c0 == 0) params_of(a.c, region, slot0, which)[s] = param_word(q);
   }
 }
 
@@ -261,12 +258,11 @@ __device__ __forceinline__ void decode4(float* x, uint32_t biased, float scale, 
 template <class T, int BITS>
 __device__ void read_group(const RowArgs& a, int row0, int head, int session, int slot0) {
   const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
-  const uint8_t* region = region_of(a.c, session, head);
-  const uint32_t* params = reinterpret_cast<const uint32_t*>(region + params_offset(a.c)) + slot0 + s;
+  uint8_t* region = region_of(a.c, session, head);
   uint32_t w[2][2][2] = {};
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const uint32_t* in = reinterpret_cast<const uint32_t*>(region + (which ? values_offset(a.c) : 0) + (long long)(slot0 >> 2) * 4 * cb);
+    const uint32_t* in = codes_of(a.c, region, slot0, which);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int chunk = c0 + 8 * u;
@@ -279,7 +275,7 @@ __device__ void read_group(const RowArgs& a, int row0, int head, int session, in
       }
     }
   }
-  const uint32_t param[2] = {__ldg(params), __ldg(params + a.c.cap)};
+  const uint32_t param[2] = {params_of(a.c, region, slot0, false)[s], params_of(a.c, region, slot0, true)[s]};
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const Rows& r = which ? a.v : a.k;
@@ -472,7 +468,7 @@ extern "C" int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out) {
   c.ring = s.slots - s.sinks;
   c.cap = (s.slots + 63) / 64 * 64;
   c.cb = s.head_dim * s.bits / 8;
-  c.region = 2ll * c.cap * (c.cb + 4);
+  c.region = (long long)(c.cap / kv::kBlockSlots) * kv::block_bytes(c.cb);
   // the workspace of mc_kv_attend_dev is part of the cache, so that no call allocates
   const size_t head = 256 + kv::kMaxPartials * (sizeof(int) + kv::kAttendRows * (2 + s.head_dim) * sizeof(float));
   const double need = (double)c.region * s.sessions * s.heads + (double)head;
@@ -567,14 +563,13 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   const Cache& c = kv->c;
   const int group = q_heads / c.heads, row_groups = (group + kAttendRows - 1) / kAttendRows;
   const long long items = (long long)n * c.heads * row_groups;
-  // Warps an item's slots are split over: as many as fill the 12 warps of every SM, while each keeps
-  // two tiles of 64 slots.
+  // CTAs (of four warps) that an item's slots are split over. SLOTS_RULE
   const int seen = window > 0 ? (int)std::min<long long>(c.slots, (long long)window + c.sinks) : c.slots;
-  const long long warps = 12ll * kv->n_sm, wanted = std::min<long long>(warps / items, (seen + 127) / 128);
-  const bool split = wanted > 1;
-  int pieces = 1;
-  if (split)
-    pieces = (int)std::max<long long>(1, std::min<long long>({wanted / kAttendWarps, kMaxPartials / items, kMaxPieces}));
+  const AttendVariant f = attend_variant(c.bits, c.dim, dtype == kF32 ? 3 : 2, group);
+  const long long ctas = (long long)f.ctas * kv->n_sm, most = std::min<long long>({(seen + 511) / 512, kMaxPieces, kMaxPartials / std::max(1ll, items)});
+  int pieces = 0;  // 0: an item to a warp
+  if (items < kAttendWarps * ctas && seen > 64)
+    pieces = (int)std::max(1ll, std::min(most, 2 * items <= ctas ? ctas / items : (4 * ctas + items - 1) / items));
   const int size = dtype == kF32 ? 4 : 2;
   auto aligned = [&](const mc_rows* r) {
     return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
@@ -582,11 +577,9 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   const AttendArgs a{c, rows_of(q), rows_of(out), n, q_heads, group, row_groups, window, dtype, aligned(q) && aligned(out),
                      pieces, sessions, lens, scale * 1.4426950408889634f, kv->partial, kv->arrived};
   if (items > INT_MAX) return set_error(kInvalidArgument, "mc_kv_attend_dev: too many rows");
-  const long long blocks = split ? items : std::min<long long>((items + kAttendWarps - 1) / kAttendWarps, warps / kAttendWarps);
-  const int planes = dtype == kF32 ? 3 : 2;
-  const AttendVariant f = c.bits == 4 ? attend_variant_of<4>(c.dim, planes, split) : attend_variant_of<8>(c.dim, planes, split);
+  const long long blocks = pieces ? items : std::min<long long>((items + kAttendWarps - 1) / kAttendWarps, ctas);
   MC_CUDA(cudaFuncSetAttribute(f.f, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
-  f.f<<<dim3((unsigned)blocks, pieces), kAttendWarps * 32, f.smem, static_cast<cudaStream_t>(stream)>>>(a);
+  f.f<<<dim3((unsigned)blocks, std::max(1, pieces)), kAttendWarps * 32, f.smem, static_cast<cudaStream_t>(stream)>>>(a);
   MC_CUDA(cudaGetLastError());
   return kOk;
 }

@@ -2,20 +2,21 @@
 //
 // A cache has `slots` places per session. Position p of a session lies at slot p while p < sinks
 // (the first positions are never overwritten) and at sinks + (p - sinks) % (slots - sinks) after
-// that: a ring behind pinned places. Every (session, head) owns one region
+// that: a ring behind pinned places. Every (session, head) owns one region of cap / 32 blocks (cap =
+// slots rounded up to 64), a block being all there is of 32 slots, so that one copy fetches it:
 //
 //   keys' codes | values' codes | keys' scales and centers | values' scales and centers
 //
-// with `cap` = slots rounded up to 64 places. Codes of four consecutive slots are interleaved, so
-// that a 16-byte load gives a lane one 32-bit word of each of the four, in the order in which the
-// operands of an 8-bit m16n8k32 MMA want them:
+// Codes of four consecutive slots are interleaved, so that a 16-byte load gives a lane one 32-bit
+// word of each of the four, in the order in which the operands of an 8-bit m16n8k32 MMA want them
+// (slot s, group s / 4 of its block; cb code bytes per slot):
 //
-//   keys    word w of slot s is word (s / 4) * 4 * words + 4 * w + s % 4. 8 bits: word w holds
+//   keys    word w of slot s is word 4 * w + s % 4 of its group's cb. 8 bits: word w holds
 //           dimensions 4w..4w+3. 4 bits: byte b of word w holds dimensions 8w + b (low) and
 //           8w + 4 + b (high). The contraction runs along the dimensions: a word is an operand.
-//   values  word (s / 4) * cb + n * ni + i (cb code bytes per slot) holds dimension 8i + n
-//           (8 bits, ni = dim / 8), or 16i + n (low) and 16i + 8 + n (high) (4 bits, ni = dim / 16),
-//           of four slots, slot s in byte s % 4. The contraction runs along the slots.
+//   values  word n * ni + i of the group's cb holds dimension 8i + n (8 bits, ni = dim / 8), or
+//           16i + n (low) and 16i + 8 + n (high) (4 bits, ni = dim / 16), of four slots, slot s
+//           in byte s % 4. The contraction runs along the slots.
 //
 // A slot's scale and center are one word: scale in the low half, center in the high (bfloat16).
 #pragma once
@@ -48,8 +49,18 @@ struct Cache {
 __device__ __forceinline__ uint8_t* region_of(const Cache& c, int session, int head) {
   return c.base + ((long long)session * c.heads + head) * c.region;
 }
-__device__ __forceinline__ long long values_offset(const Cache& c) { return (long long)c.cap * c.cb; }
-__device__ __forceinline__ long long params_offset(const Cache& c) { return 2ll * c.cap * c.cb; }
+constexpr int kBlockSlots = 32;
+__host__ __device__ constexpr int block_bytes(int cb) { return kBlockSlots * (2 * cb + 8); }
+
+// The codes of slot s's group of four, and the words of scale and center from slot s on, in a region.
+__device__ __forceinline__ uint32_t* codes_of(const Cache& c, uint8_t* region, int s, bool values) {
+  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb) + (values ? kBlockSlots * c.cb : 0)) +
+         ((s & 31) >> 2) * c.cb;
+}
+__device__ __forceinline__ uint32_t* params_of(const Cache& c, uint8_t* region, int s, bool values) {
+  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb) + 2 * kBlockSlots * c.cb) + (s & 31) +
+         (values ? kBlockSlots : 0);
+}
 
 __device__ __forceinline__ int slot_of(const Cache& c, int pos) {
   return pos < c.sinks ? pos : c.sinks + (pos - c.sinks) % c.ring;

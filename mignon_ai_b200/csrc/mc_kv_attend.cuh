@@ -37,23 +37,49 @@ struct AttendArgs {
   Rows q, out;
   int n, q_heads, group, row_groups, window, dtype;
   int vec;               // rows of q and out take 16-byte (eight elements) and pair accesses
-  int pieces;            // CTAs an item's slots are split over
+  int pieces;            // CTAs an item's slots are split over; 0: every warp has items of its own
   const int *sess, *lens;
   float scale;           // of the scores, times log2(e)
   float* partial;        // [item][piece][8][2 + dim]: maximum, sum, weighted values
   int* arrived;          // [item] pieces done (zero between calls)
 };
 
-// d += a x b, a and b 8-bit (A unsigned for the weights, signed for the queries), 32-bit sums
-__device__ __forceinline__ void mma_s8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d (+)= a x b on 8-bit operands with 32-bit sums: B signed, A signed (the queries) or unsigned (the
+// weights). FIRST: d starts from zero.
+template <bool UNSIGNED, bool FIRST>
+__device__ __forceinline__ void mma_8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+#define MC_MMA_8(TYPE)                                                                                                    \
+  if constexpr (FIRST)                                                                                                    \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};" \
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                         \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));                                         \
+  else                                                                                                                    \
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." TYPE ".s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                         \
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1))
+  if constexpr (UNSIGNED) {
+    MC_MMA_8("u8");
+  } else {
+    MC_MMA_8("s8");
+  }
+#undef MC_MMA_8
 }
-__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b));
+  return d;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -158,13 +184,19 @@ __device__ __forceinline__ SlotSpan slot_span(const Cache& c, int len, int windo
   return s;
 }
 
-constexpr int attend_slots(int bits, int planes) { return bits == 4 && planes == 2 ? 64 : 32; }
-constexpr int attend_stage_bytes(int bits, int dim, int planes) {
-  return attend_slots(bits, planes) * (2 * dim * bits / 8 + 8);
+// CTAs that share an SM: four where 128 registers a thread hold the work.
+constexpr int attend_ctas(int dim) { return dim <= 64 ? 4 : 3; }
+// Slots of a tile: 64 (two blocks) where two tiles a warp then fit shared memory, and where the third
+// plane leaves the registers for it.
+constexpr int attend_slots(int bits, int dim, int planes) {
+  return bits == 4 ? (planes == 3 && dim > 64 ? 32 : 64) : dim <= 32 ? 64 : 32;
 }
-// Tiles in flight per warp: what fits three CTAs of four warps on an SM.
+constexpr int attend_stage_bytes(int bits, int dim, int planes) {
+  return attend_slots(bits, dim, planes) / kBlockSlots * block_bytes(dim * bits / 8);
+}
+// Tiles in flight per warp.
 constexpr int attend_stages(int bits, int dim, int planes) {
-  const int n = 71680 / (kAttendWarps * attend_stage_bytes(bits, dim, planes));
+  const int n = (221184 / attend_ctas(dim) - 1024) / (kAttendWarps * attend_stage_bytes(bits, dim, planes));
   return n > 4 ? 4 : n < 2 ? 2 : n;
 }
 constexpr int attend_smem(int bits, int dim, int planes) {
@@ -176,17 +208,23 @@ constexpr int attend_smem(int bits, int dim, int planes) {
 // Where a warp is in its work: an item (a session's up to eight query heads of one key/value head)
 // and a tile of its visible slots.
 struct AttendCursor {
-  long long item;
+  unsigned item;  // items fit 31 bits, and a stride beyond them 32
   int t, end;
   int tiles0, first1;
   const uint8_t* region;
 };
 
-// WPI warps of a CTA share an item: 1 gives every warp items of its own, one after the other with
-// the next one's tiles already in flight; kAttendWarps gives the CTA one piece of one item.
-template <int BITS, int DIM, int PLANES, int WPI>
-__global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int TS = attend_slots(BITS, PLANES), HALVES = TS / 32;
+// With few heads to an item the MMA's eight rows repeat them: HEADS rows of heads (8, 4 or 1), and the
+// rows of one head take different slots of the tile (row r: HEADS 4, the groups 2cc + r / 4; HEADS 1,
+// the slot r % 4 of those), so that no thread does another's exponentials. They share the
+// running maximum, and their sums meet at the end of the item.
+//
+// With a.pieces a CTA has one piece of one item; without, every warp goes through items of its own,
+// the next one's tiles already in flight.
+template <int BITS, int DIM, int PLANES, int HEADS>
+__global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int TS = attend_slots(BITS, DIM, PLANES), HALVES = TS / 32;
+  constexpr int NJ = HEADS == 1 ? 1 : 4, NU = HEADS == 8 ? 2 : 1;  // slots of a half that a thread weighs: NJ x NU
   constexpr int CB = DIM * BITS / 8;             // code bytes per slot
   constexpr int KS = (DIM + 31) / 32;            // MMA steps along the dimensions
   constexpr int NI = BITS == 4 ? DIM / 16 : DIM / 8;  // value words of a group of slots per thread
@@ -205,13 +243,15 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
   }
   __syncwarp();
 
-  const int per = c.heads * a.row_groups;
-  const long long items = (long long)a.n * per, stride = WPI == 1 ? (long long)gridDim.x * kAttendWarps : items;
-  const int piece = WPI == 1 ? 0 : blockIdx.y;
-  const int part = WPI == 1 ? 0 : piece * WPI + warp, parts = WPI == 1 ? 1 : a.pieces * WPI;
+  const unsigned per = c.heads * a.row_groups, items = a.n * per;
+  const unsigned stride = a.pieces ? items : gridDim.x * kAttendWarps;
+  const int piece = blockIdx.y;
+  const unsigned part = piece * kAttendWarps + warp, parts = a.pieces * kAttendWarps;
+  const int row_head = HEADS == 8 ? r : HEADS == 4 ? r & 3 : 0;  // the thread's query head in the item
+  const int my_u = r >> 2, my_j = r & 3;                         // and its slots: see above
 
   auto open = [&](AttendCursor& u, SlotSpan& span) {
-    const int b = (int)(u.item / per), head = (int)(u.item % per) / a.row_groups;
+    const unsigned b = u.item / per, hr = u.item - b * per, head = a.row_groups == 1 ? hr : hr / a.row_groups;
     int session = a.sess ? a.sess[b] : b, len = 0;
     if ((unsigned)session < (unsigned)c.sessions) {
       len = a.lens[b];
@@ -220,8 +260,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       session = 0;
     }
     span = slot_span<TS>(c, len, a.window);
-    u.t = (int)((long long)span.tiles * part / parts);
-    u.end = (int)((long long)span.tiles * (part + 1) / parts);
+    u.t = 0;
+    u.end = span.tiles;
+    if (a.pieces) {  // an even share of the tiles, the first parts one more
+      const unsigned share = (unsigned)span.tiles / parts, more = (unsigned)span.tiles - share * parts;
+      u.t = part * share + min(part, more);
+      u.end = u.t + share + (part < more ? 1 : 0);
+    }
     u.tiles0 = span.tiles0;
     u.first1 = span.first1;
     u.region = region_of(c, session, head);
@@ -229,7 +274,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
   auto slot_at = [](const AttendCursor& u, int t) { return (t < u.tiles0 ? t : u.first1 + t - u.tiles0) * TS; };
 
   // ---- the producer's side: lane 0 copies the tiles of this warp's items in their order
-  AttendCursor next{WPI == 1 ? (long long)blockIdx.x * kAttendWarps + warp : (long long)blockIdx.x, 0, 0, 0, 0, nullptr};
+  AttendCursor next{a.pieces ? blockIdx.x : blockIdx.x * kAttendWarps + warp, 0, 0, 0, 0, nullptr};
   AttendCursor cur = next;
   int issued = 0;
   SlotSpan scratch;
@@ -243,14 +288,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
     }
     if (lane == 0) {
       const int slot0 = slot_at(next, next.t), stage = issued % STAGES;
-      uint8_t* dst = ring + stage * STAGE;
-      const uint8_t* codes = next.region + (long long)slot0 * CB;
-      const uint8_t* params = next.region + params_offset(c) + (long long)slot0 * 4;
       mbar_arrive_expect_tx(bars + stage, STAGE);
-      bulk_load(dst, codes, TS * CB, bars + stage);
-      bulk_load(dst + TS * CB, codes + values_offset(c), TS * CB, bars + stage);
-      bulk_load(dst + 2 * TS * CB, params, TS * 4, bars + stage);
-      bulk_load(dst + 2 * TS * CB + TS * 4, params + (long long)c.cap * 4, TS * 4, bars + stage);
+      bulk_load(ring + stage * STAGE, next.region + (long long)(slot0 >> 5) * block_bytes(CB), STAGE, bars + stage);
     }
     ++issued;
     ++next.t;
@@ -259,15 +298,15 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
 
   int done = 0;
   bool ok = true;  // false after a wait gave up
-  float o[NT][2];
+  float2 o[NT];
   float top, total, csum;
   int b, rows, h0;
   for (; cur.item < items; cur.item += stride) {
     SlotSpan span;
     open(cur, span);
-    b = (int)(cur.item / per);
-    const int hr = (int)(cur.item % per), head = hr / a.row_groups, rg = hr % a.row_groups;
-    rows = min(kAttendRows, a.group - rg * kAttendRows);  // query heads of this item
+    b = cur.item / per;
+    const unsigned hr = cur.item - b * per, head = a.row_groups == 1 ? hr : hr / a.row_groups, rg = hr - head * a.row_groups;
+    rows = min(kAttendRows, a.group - (int)rg * kAttendRows);  // query heads of this item
     h0 = head * a.group + rg * kAttendRows;
 
     // ---- the queries as digit planes: thread (r, cc) holds row r's dimensions 8w..8w+7, w = cc + 4i
@@ -275,11 +314,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
     float qstep, qsum = 0.f;
     {
       float x[KS][8], big = 0.f;
-      const long long base = b * a.q.row + (h0 + r) * a.q.head;
+      const long long base = b * a.q.row + (h0 + row_head) * a.q.head;
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         const int w = cc + 4 * i;
-        const bool in = r < rows && 8 * w < DIM;
+        const bool in = row_head < rows && 8 * w < DIM;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
         if (in) load_query(x[i], a.q.p, base + 8 * w, a.dtype, a.vec);
@@ -311,25 +350,22 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       qsum = __fmul_rn(qsum, a.scale);
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = 0.f;
+    for (int i = 0; i < NT; ++i) o[i] = make_float2(0.f, 0.f);
     top = -INFINITY, total = 0.f, csum = 0.f;
 
     for (int t = cur.t; t < cur.end; ++t) {
       const int slot0 = slot_at(cur, t), stage = done % STAGES;
       ok = __all_sync(~0u, ok && mbar_wait_or_abort(bars + stage, (done / STAGES) & 1, kErrWaitFull));
       if (!ok) break;
-      const uint8_t* kcodes = ring + stage * STAGE;
-      const uint8_t* vcodes = kcodes + TS * CB;
-      const uint32_t* kparam = reinterpret_cast<const uint32_t*>(vcodes + TS * CB);
-      const uint32_t* vparam = kparam + TS;
-      // ---- scores: s[h][i][u] of slot 32h + 8cc + 4u + i
-      float s[HALVES][4][2];
+      const uint8_t* tile = ring + stage * STAGE;
+      // ---- scores: s[h][j * NU + u] of slot 32h + slot_in(j, u), this thread's share of the tile
+      auto slot_in = [&](int j, int u) { return 8 * cc + 4 * (HEADS == 8 ? u : my_u) + (HEADS == 1 ? my_j : j); };
+      float s[HALVES][NJ * NU];
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        const uint4* kp4 = reinterpret_cast<const uint4*>(kparam + 32 * h + 8 * cc);
-        const uint4 kp[2] = {kp4[0], kp4[1]};
-        const uint8_t* kc = kcodes + (8 * h + r) * 4 * CB;
-        int acc[4][4] = {}, acc3[4][4] = {};
+        const uint8_t* kc = tile + h * block_bytes(CB) + r * 4 * CB;
+        const uint32_t* kparam = reinterpret_cast<const uint32_t*>(tile + h * block_bytes(CB) + 2 * kBlockSlots * CB);
+        int acc[4][4], acc3[4][4];
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           const int w = cc + 4 * i;
@@ -350,19 +386,48 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            mma_s8s8(acc[j], qa[i][0][0], qa[i][1][0], qa[i][0][1], qa[i][1][1], b0[j], b1[j]);
-            if constexpr (PLANES == 3) mma_s8s8(acc3[j], qa[i][2][0], 0u, qa[i][2][1], 0u, b0[j], b1[j]);
+            if (i == 0) {
+              mma_8<false, true>(acc[j], qa[i][0][0], qa[i][1][0], qa[i][0][1], qa[i][1][1], b0[j], b1[j]);
+              if constexpr (PLANES == 3) mma_8<false, true>(acc3[j], qa[i][2][0], 0u, qa[i][2][1], 0u, b0[j], b1[j]);
+            } else {
+              mma_8<false, false>(acc[j], qa[i][0][0], qa[i][1][0], qa[i][0][1], qa[i][1][1], b0[j], b1[j]);
+              if constexpr (PLANES == 3) mma_8<false, false>(acc3[j], qa[i][2][0], 0u, qa[i][2][1], 0u, b0[j], b1[j]);
+            }
           }
         }
+        auto score = [&](int first, int second, int third, uint32_t w) {
+          // |first| <= 128 * 127 * 127, so 254 * first + second fits 32 bits
+          float f = (float)(first * 254 + second);
+          if constexpr (PLANES == 3) f = __fmaf_rn((float)third, 1.0f / 254.0f, f);
+          return __fmaf_rn(__fmul_rn(f, qstep), param_scale(w), __fmul_rn(param_center(w), qsum));
+        };
+        if constexpr (HEADS == 8) {
+          const uint4* kp4 = reinterpret_cast<const uint4*>(kparam + 8 * cc);
+          const uint4 kp[2] = {kp4[0], kp4[1]};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            // |first| <= 128 * 127 * 127, so 254 * first + second fits 32 bits
-            float f = (float)(acc[j][u] * 254 + acc[j][2 + u]);
-            if constexpr (PLANES == 3) f = __fmaf_rn((float)acc3[j][u], 1.0f / 254.0f, f);
-            const uint32_t w = word_of(kp[u], j);
-            s[h][j][u] = __fmaf_rn(__fmul_rn(f, qstep), param_scale(w), __fmul_rn(param_center(w), qsum));
+            for (int u = 0; u < 2; ++u) s[h][2 * j + u] = score(acc[j][u], acc[j][2 + u], PLANES == 3 ? acc3[j][u] : 0, word_of(kp[u], j));
+        } else {
+          int x[4][3];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j][0] = my_u ? acc[j][1] : acc[j][0];
+            x[j][1] = my_u ? acc[j][3] : acc[j][2];
+            x[j][2] = PLANES == 3 ? (my_u ? acc3[j][1] : acc3[j][0]) : 0;
+          }
+          if constexpr (HEADS == 4) {
+            const uint4 kp = *reinterpret_cast<const uint4*>(kparam + 8 * cc + 4 * my_u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[h][j] = score(x[j][0], x[j][1], x[j][2], word_of(kp, j));
+          } else {
+            int y[3];
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+              const int lo = my_j & 1 ? x[1][p] : x[0][p], hi = my_j & 1 ? x[3][p] : x[2][p];
+              y[p] = my_j & 2 ? hi : lo;
+            }
+            s[h][0] = score(y[0], y[1], PLANES == 3 ? y[2] : 0, kparam[slot_in(0, 0)]);
           }
         }
       }
@@ -371,27 +436,32 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int slot = slot0 + 32 * h + 8 * cc + 4 * u + j;
-              if (!(slot < span.e0 || (slot >= span.s1 && slot < span.e1))) s[h][j][u] = -INFINITY;
+            for (int u = 0; u < NU; ++u) {
+              const int slot = slot0 + 32 * h + slot_in(j, u);
+              if (!(slot < span.e0 || (slot >= span.s1 && slot < span.e1))) s[h][j * NU + u] = -INFINITY;
             }
       }
-      // ---- running maximum and sum (a row's slots are on the four threads of its quad)
+      // ---- running maximum of the head (its slots are on the row's quad and on the rows that repeat it)
       float m = top;
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(s[h][j][0], s[h][j][1]));
+        for (int e = 0; e < NJ * NU; ++e) m = fmaxf(m, s[h][e]);
       m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
       m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+      if constexpr (HEADS <= 4) m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+      if constexpr (HEADS == 1) {
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+      }
       if (__any_sync(~0u, m > top)) {
         const float keep = top == -INFINITY ? 0.f : exp2_fast(__fsub_rn(top, m));
         total = __fmul_rn(total, keep);
         csum = __fmul_rn(csum, keep);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) o[i][0] = __fmul_rn(o[i][0], keep), o[i][1] = __fmul_rn(o[i][1], keep);
+        for (int i = 0; i < NT; ++i) o[i] = mul2(o[i], keep);
         top = m;
       }
       // ---- weights p, their sum, and p * vscale in place of the scores
@@ -399,20 +469,29 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       const float shift = top == -INFINITY ? 0.f : top;  // nothing but scores of minus infinity so far
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        const uint4* vp4 = reinterpret_cast<const uint4*>(vparam + 32 * h + 8 * cc);
-        const uint4 vp[2] = {vp4[0], vp4[1]};
+        const uint32_t* vparam =
+            reinterpret_cast<const uint32_t*>(tile + h * block_bytes(CB) + 2 * kBlockSlots * CB) + kBlockSlots;
+        uint32_t vp[NJ * NU];
+        if constexpr (HEADS == 1) {
+          vp[0] = vparam[slot_in(0, 0)];
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int u = 0; u < NU; ++u) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vparam + slot_in(0, u));
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float p = exp2_fast(__fsub_rn(s[h][j][u], shift));
-            uint32_t w = word_of(vp[u], j);
-            if (!whole && s[h][j][u] == -INFINITY) w = 0;  // a hidden slot may hold a scale of NaN
-            total = __fadd_rn(total, p);
-            csum = __fmaf_rn(p, param_center(w), csum);
-            s[h][j][u] = __fmul_rn(p, param_scale(w));
-            pmax = fmaxf(pmax, s[h][j][u]);
+            for (int j = 0; j < 4; ++j) vp[j * NU + u] = word_of(w, j);
           }
+        }
+#pragma unroll
+        for (int e = 0; e < NJ * NU; ++e) {
+          const float p = exp2_fast(__fsub_rn(s[h][e], shift));
+          uint32_t w = vp[e];
+          if (!whole && s[h][e] == -INFINITY) w = 0;  // a hidden slot may hold a scale of NaN
+          total = __fadd_rn(total, p);
+          csum = __fmaf_rn(p, param_center(w), csum);
+          s[h][e] = __fmul_rn(p, param_scale(w));
+          pmax = fmaxf(pmax, s[h][e]);
+        }
       }
       pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 1));
       pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 2));
@@ -420,25 +499,47 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       constexpr float kFull = PLANES == 3 ? 8388607.0f : 65535.0f;
       const float inv = pmax > 1e-30f ? __fdividef(kFull, pmax) : 0.f;
       const float unit = __fmul_rn(pmax > 1e-30f ? pmax : 0.f, kOne / kFull);
-      // ---- the weights' bytes as A operands: plane 0 (highest) in rows 0-7, plane 1 in rows 8-15
+      // ---- the weights' bytes as A operands: plane 0 (highest) in rows 0-7, plane 1 in rows 8-15;
+      // a word holds the four slots of group 2cc + u, of which a row's are its own
       uint32_t pa[HALVES][PLANES][2];
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h)
+      for (int h = 0; h < HALVES; ++h) {
+        uint32_t x[NJ * NU];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t x[4];
+        for (int e = 0; e < NJ * NU; ++e)
+          x[e] = __float_as_uint(fminf(__fmaf_rn(s[h][e], inv, 8388608.0f), 8388608.0f + kFull));
+        if constexpr (HEADS == 1) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[j] = __float_as_uint(fminf(__fmaf_rn(s[h][j][u], inv, 8388608.0f), 8388608.0f + kFull));
-          const uint32_t lo01 = __byte_perm(x[0], x[1], 0x5140), lo23 = __byte_perm(x[2], x[3], 0x5140);
-          pa[h][PLANES - 1][u] = __byte_perm(lo01, lo23, 0x5410);  // bytes 0
-          pa[h][PLANES - 2][u] = __byte_perm(lo01, lo23, 0x7632);  // bytes 1
-          if constexpr (PLANES == 3) {
-            const uint32_t hi01 = __byte_perm(x[0], x[1], 0x0062), hi23 = __byte_perm(x[2], x[3], 0x0062);
-            pa[h][0][u] = __byte_perm(hi01, hi23, 0x5410);  // bits 16-22
+          for (int p = 0; p < PLANES; ++p) {
+            const uint32_t word = ((x[0] >> (8 * (PLANES - 1 - p))) & (p == 0 && PLANES == 3 ? 0x7Fu : 0xFFu)) << (8 * my_j);
+            pa[h][p][0] = my_u ? 0u : word;
+            pa[h][p][1] = my_u ? word : 0u;
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < NU; ++u) {
+            const uint32_t lo01 = __byte_perm(x[u], x[NU + u], 0x5140), lo23 = __byte_perm(x[2 * NU + u], x[3 * NU + u], 0x5140);
+            uint32_t word[3];
+            word[PLANES - 1] = __byte_perm(lo01, lo23, 0x5410);  // bytes 0
+            word[PLANES - 2] = __byte_perm(lo01, lo23, 0x7632);  // bytes 1
+            if constexpr (PLANES == 3) {
+              const uint32_t hi01 = __byte_perm(x[u], x[NU + u], 0x0062), hi23 = __byte_perm(x[2 * NU + u], x[3 * NU + u], 0x0062);
+              word[0] = __byte_perm(hi01, hi23, 0x5410);  // bits 16-22
+            }
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+              if constexpr (HEADS == 8) {
+                pa[h][p][u] = word[p];
+              } else {
+                pa[h][p][0] = my_u ? 0u : word[p];
+                pa[h][p][1] = my_u ? word[p] : 0u;
+              }
+            }
           }
         }
+      }
       // ---- the weighted values
+      const float2 unit2 = make_float2(unit, unit);
       constexpr int STEP = NI % 4 == 0 ? 4 : NI % 2 == 0 ? 2 : 1;
 #pragma unroll
       for (int i0 = 0; i0 < NI; i0 += STEP) {
@@ -447,12 +548,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
         for (int h = 0; h < HALVES; ++h)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
-            load_words<STEP>(v[h][u], reinterpret_cast<const uint32_t*>(vcodes + (8 * h + 2 * cc + u) * 4 * CB) + r * NI + i0);
+            load_words<STEP>(v[h][u], reinterpret_cast<const uint32_t*>(tile + h * block_bytes(CB) + kBlockSlots * CB) +
+                                          (2 * cc + u) * CB + r * NI + i0);
 #pragma unroll
         for (int i = 0; i < STEP; ++i) {
 #pragma unroll
           for (int nib = 0; nib < (BITS == 4 ? 2 : 1); ++nib) {
-            int acc[4] = {}, acc3[4] = {};
+            int acc[4], acc3[4];
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
               uint32_t b0 = v[h][0][i], b1 = v[h][1][i];
@@ -460,17 +562,19 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
                 b0 = nib ? high_codes(b0) : low_codes(b0);
                 b1 = nib ? high_codes(b1) : low_codes(b1);
               }
-              mma_u8s8(acc, pa[h][0][0], pa[h][1][0], pa[h][0][1], pa[h][1][1], b0, b1);
-              if constexpr (PLANES == 3) mma_u8s8(acc3, pa[h][2][0], 0u, pa[h][2][1], 0u, b0, b1);
+              if (h == 0) {
+                mma_8<true, true>(acc, pa[h][0][0], pa[h][1][0], pa[h][0][1], pa[h][1][1], b0, b1);
+                if constexpr (PLANES == 3) mma_8<true, true>(acc3, pa[h][2][0], 0u, pa[h][2][1], 0u, b0, b1);
+              } else {
+                mma_8<true, false>(acc, pa[h][0][0], pa[h][1][0], pa[h][0][1], pa[h][1][1], b0, b1);
+                if constexpr (PLANES == 3) mma_8<true, false>(acc3, pa[h][2][0], 0u, pa[h][2][1], 0u, b0, b1);
+              }
             }
             const int nt = BITS == 4 ? 2 * (i0 + i) + nib : i0 + i;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              // |first| <= 255 * 127 * 64, so 256 * first + second fits 32 bits
-              float f = (float)(acc[u] * 256 + acc[2 + u]);
-              if constexpr (PLANES == 3) f = __fmaf_rn(f, 256.0f, (float)acc3[u]);
-              o[nt][u] = __fmaf_rn(f, unit, o[nt][u]);
-            }
+            // |first| <= 255 * 127 * 64, so 256 * first + second fits 32 bits
+            float2 f = make_float2((float)(acc[0] * 256 + acc[2]), (float)(acc[1] * 256 + acc[3]));
+            if constexpr (PLANES == 3) f = fma2(f, make_float2(256.0f, 256.0f), make_float2((float)acc3[0], (float)acc3[1]));
+            o[nt] = fma2(f, unit2, o[nt]);
           }
         }
       }
@@ -479,30 +583,41 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       issue();
     }
     if (!ok) break;
-    // ---- the row's sums over its quad; the centers' share goes to every dimension
-#pragma unroll
-    for (int x = 1; x <= 2; x <<= 1) {
+    // ---- the sums over the row's quad and over the rows of its head; the centers' share goes to
+    // every dimension
+    auto join = [&](int x) {
       total = __fadd_rn(total, __shfl_xor_sync(~0u, total, x));
       csum = __fadd_rn(csum, __shfl_xor_sync(~0u, csum, x));
+      if (x < 4) return;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        o[i].x = __fadd_rn(o[i].x, __shfl_xor_sync(~0u, o[i].x, x));
+        o[i].y = __fadd_rn(o[i].y, __shfl_xor_sync(~0u, o[i].y, x));
+      }
+    };
+    join(1);
+    join(2);
+    if constexpr (HEADS <= 4) join(16);
+    if constexpr (HEADS == 1) {
+      join(4);
+      join(8);
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = __fadd_rn(o[i][0], csum), o[i][1] = __fadd_rn(o[i][1], csum);
+    for (int i = 0; i < NT; ++i) o[i] = make_float2(__fadd_rn(o[i].x, csum), __fadd_rn(o[i].y, csum));
     // thread (r, cc) has dimensions 8i + 2cc and 8i + 2cc + 1 of row r
-    if constexpr (WPI == 1) {
-      if (r < rows) {
-        const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
-        const long long base = b * a.out.row + (h0 + r) * a.out.head;
+    if (!a.pieces && r < min(rows, HEADS)) {
+      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
+      const long long base = b * a.out.row + (h0 + r) * a.out.head;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-          store_pair(a.out.p, base + 8 * i + 2 * cc, a.dtype, a.vec, __fmul_rn(o[i][0], inv), __fmul_rn(o[i][1], inv));
-      }
+      for (int i = 0; i < NT; ++i)
+        store_pair(a.out.p, base + 8 * i + 2 * cc, a.dtype, a.vec, __fmul_rn(o[i].x, inv), __fmul_rn(o[i].y, inv));
     }
   }
   // a wait that gave up: never leave with copies in flight into this warp's buffers
   if (!ok && lane == 0)
     for (; done < issued; ++done) mbar_wait(bars + done % STAGES, (done / STAGES) & 1, kErrWaitFull);
 
-  if constexpr (WPI != 1) {
+  if (a.pieces) {
     constexpr int W = 2 + DIM;  // maximum, sum, weighted values of a row
     float* results = reinterpret_cast<float*>(smem);  // [warp][row][W], over the ring of tiles
     __shared__ float keeps[kMaxPieces * kAttendRows];
@@ -513,7 +628,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       float* mine = results + (warp * kAttendRows + r) * W;
       if (cc == 0) mine[0] = top, mine[1] = total;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) mine[2 + 8 * i + 2 * cc] = o[i][0], mine[3 + 8 * i + 2 * cc] = o[i][1];
+      for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(mine + 2 + 8 * i + 2 * cc) = o[i];
     }
     __syncthreads();
     float* out = a.partial + (item * a.pieces + piece) * kAttendRows * W;
@@ -521,9 +636,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
       const int row = e / DIM, d = e % DIM;
       float m = -INFINITY, l = 0.f, x = 0.f;
 #pragma unroll
-      for (int w = 0; w < WPI; ++w) m = fmaxf(m, results[(w * kAttendRows + row) * W]);
+      for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, results[(w * kAttendRows + row) * W]);
 #pragma unroll
-      for (int w = 0; w < WPI; ++w) {
+      for (int w = 0; w < kAttendWarps; ++w) {
         const float* q = results + (w * kAttendRows + row) * W;
         // a part without visible slots has maximum -inf and sums of zero
         const float keep = q[0] == -INFINITY ? 0.f : exp2_fast(__fsub_rn(q[0], m));
@@ -586,28 +701,34 @@ __global__ void __launch_bounds__(kAttendWarps * 32, 3) attend_kernel(const __gr
 
 struct AttendVariant {
   void (*f)(AttendArgs);
-  int smem;
+  int smem, ctas;
 };
 
-template <int BITS, int DIM>
-inline AttendVariant attend_variant(int planes, bool split) {
-  if (planes == 3)
-    return {split ? attend_kernel<BITS, DIM, 3, kAttendWarps> : attend_kernel<BITS, DIM, 3, 1>, attend_smem(BITS, DIM, 3)};
-  return {split ? attend_kernel<BITS, DIM, 2, kAttendWarps> : attend_kernel<BITS, DIM, 2, 1>, attend_smem(BITS, DIM, 2)};
+template <int BITS, int DIM, int PLANES>
+inline AttendVariant attend_variant_of(int heads) {
+  return {heads > 4 ? attend_kernel<BITS, DIM, PLANES, 8> : heads > 1 ? attend_kernel<BITS, DIM, PLANES, 4> : attend_kernel<BITS, DIM, PLANES, 1>,
+          attend_smem(BITS, DIM, PLANES), attend_ctas(DIM)};
 }
-
+template <int BITS, int DIM>
+inline AttendVariant attend_variant_of(int planes, int heads) {
+  return planes == 3 ? attend_variant_of<BITS, DIM, 3>(heads) : attend_variant_of<BITS, DIM, 2>(heads);
+}
 template <int BITS>
-inline AttendVariant attend_variant_of(int dim, int planes, bool split) {
+inline AttendVariant attend_variant_of(int dim, int planes, int heads) {
   switch (dim) {
-    case 16: return attend_variant<BITS, 16>(planes, split);
-    case 32: return attend_variant<BITS, 32>(planes, split);
-    case 48: return attend_variant<BITS, 48>(planes, split);
-    case 64: return attend_variant<BITS, 64>(planes, split);
-    case 80: return attend_variant<BITS, 80>(planes, split);
-    case 96: return attend_variant<BITS, 96>(planes, split);
-    case 112: return attend_variant<BITS, 112>(planes, split);
-    default: return attend_variant<BITS, 128>(planes, split);
+    case 16: return attend_variant_of<BITS, 16>(planes, heads);
+    case 32: return attend_variant_of<BITS, 32>(planes, heads);
+    case 48: return attend_variant_of<BITS, 48>(planes, heads);
+    case 64: return attend_variant_of<BITS, 64>(planes, heads);
+    case 80: return attend_variant_of<BITS, 80>(planes, heads);
+    case 96: return attend_variant_of<BITS, 96>(planes, heads);
+    case 112: return attend_variant_of<BITS, 112>(planes, heads);
+    default: return attend_variant_of<BITS, 128>(planes, heads);
   }
+}
+// heads: query heads that share a key/value head (more than 8: in several items)
+inline AttendVariant attend_variant(int bits, int dim, int planes, int heads) {
+  return bits == 4 ? attend_variant_of<4>(dim, planes, heads) : attend_variant_of<8>(dim, planes, heads);
 }
 
 }  // namespace kv
