@@ -106,21 +106,22 @@ __device__ void write_row(const RowArgs& a, int row, int head, RowPlace w, int8_
     }
     __syncwarp();
     const int s = w.slot & 3;
-    uint32_t* group = codes_of(a.c, region, w.slot, which);
+    const int g = w.slot >> 2;
     if (which == 0) {
+      uint32_t* out = keys_of(a.c, region, w.slot);
       for (int i = lane; i < cb / 4; i += 32) {
         uint32_t word = 0;
         for (int b = 0; b < 4; ++b)
           word |= (uint32_t)(bits == 4 ? (cs[8 * i + b] & 15) | ((cs[8 * i + 4 + b] & 15) << 4) : (uint8_t)cs[4 * i + b])
                   << (8 * b);
-        group[4 * i + s] = word;
+        out[4 * key_unit(i, g, cb, bits) + s] = word;
       }
     } else {
-      uint8_t* out = reinterpret_cast<uint8_t*>(group);
+      uint8_t* out = reinterpret_cast<uint8_t*>(values_of(a.c, region, w.slot));
       const int ni = cb / 8;
       for (int j = lane; j < cb; j += 32) {
         const int n = j / ni, i = j % ni;
-        out[4 * j + s] = (uint8_t)(bits == 4 ? (cs[16 * i + n] & 15) | ((cs[16 * i + 8 + n] & 15) << 4) : cs[8 * i + n]);
+        out[4 * value_word(n, i, g, ni) + s] = (uint8_t)(bits == 4 ? (cs[16 * i + n] & 15) | ((cs[16 * i + 8 + n] & 15) << 4) : cs[8 * i + n]);
       }
     }
     if (lane == 0) *params_of(a.c, region, w.slot, which) = param_word(q);
@@ -138,7 +139,7 @@ __device__ void read_row(const RowArgs& a, int row, int head, RowPlace w) {
   for (int which = 0; which < 2; ++which) {
     const Rows& r = which ? a.v : a.k;
     T* y = static_cast<T*>(r.p) + row * r.row + head * r.head;
-    const uint8_t* codes = reinterpret_cast<const uint8_t*>(codes_of(a.c, region, slot, which));
+    const uint8_t* codes = reinterpret_cast<const uint8_t*>(which ? values_of(a.c, region, slot) : keys_of(a.c, region, slot));
     const uint32_t param = held ? *params_of(a.c, region, slot, which) : 0;
     const float scale = param_scale(param), center = param_center(param);
     for (int d = lane; d < dim; d += 32) {
@@ -146,9 +147,9 @@ __device__ void read_row(const RowArgs& a, int row, int head, RowPlace w) {
       if (held) {
         uint32_t byte;
         if (which == 0) {
-          byte = codes[16 * (bits == 4 ? d / 8 : d / 4) + 4 * s + d % 4];
+          byte = codes[16 * key_unit(bits == 4 ? d / 8 : d / 4, slot >> 2, cb, bits) + 4 * s + d % 4];
         } else {
-          byte = codes[4 * ((d % 8) * (cb / 8) + (bits == 4 ? d / 16 : d / 8)) + s];
+          byte = codes[4 * value_word(d % 8, bits == 4 ? d / 16 : d / 8, slot >> 2, cb / 8) + s];
         }
         m = bits == 4 ? (float)(2 * signed_nibble(byte, (d >> (which ? 3 : 2)) & 1) + 1) : (float)(int8_t)byte;
       }
@@ -183,7 +184,7 @@ __device__ __forceinline__ uint32_t transpose_bytes(uint32_t x, int s) {
 // The four rows of one group of slots, lane (s, c): row s, dimensions 8c.. and 64 + 8c..
 template <class T, int BITS>
 __device__ void write_group(const RowArgs& a, int row0, int head, int session, int slot0) {
-  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
+  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb, g = slot0 >> 2;
   uint8_t* region = region_of(a.c, session, head);
   float x[2][2][8];
 #pragma unroll
@@ -209,7 +210,7 @@ __device__ void write_group(const RowArgs& a, int row0, int head, int session, i
       lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
     }
     const Quant q = quant_of(hi, lo, BITS);
-    uint32_t* out = codes_of(a.c, region, slot0, which);
+    uint32_t* out = which ? values_of(a.c, region, slot0) : keys_of(a.c, region, slot0);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (8 * u >= chunks) break;  // uniform
@@ -222,10 +223,10 @@ __device__ void write_group(const RowArgs& a, int row0, int head, int session, i
       const uint32_t b1 = pack_low_bytes(code[4], code[5], code[6], code[7]);
       if (which == 0) {
         if constexpr (BITS == 4) {
-          if (in) out[4 * chunk + s] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
+          if (in) out[4 * key_unit(chunk, g, cb, 4) + s] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
         } else if (in) {
-          out[8 * chunk + s] = b0;
-          out[8 * chunk + 4 + s] = b1;
+          out[4 * key_unit(2 * chunk, g, cb, 8) + s] = b0;
+          out[4 * key_unit(2 * chunk + 1, g, cb, 8) + s] = b1;
         }
       } else if constexpr (BITS == 4) {
         // even chunks (low nibbles) keep dimensions n = 0..3 of the pair, odd ones (high) n = 4..7
@@ -233,12 +234,12 @@ __device__ void write_group(const RowArgs& a, int row0, int head, int session, i
         const uint32_t got = __shfl_xor_sync(~0u, odd ? b0 : b1, 1);
         const uint32_t low = odd ? got : b0, high = odd ? b1 : got;
         const uint32_t word = transpose_bytes((low & 0x0F0F0F0Fu) | ((high << 4) & 0xF0F0F0F0u), s);
-        if (in) out[(4 * (chunk & 1) + s) * (cb / 8) + (chunk >> 1)] = word;
+        if (in) out[value_word(4 * (chunk & 1) + s, chunk >> 1, g, cb / 8)] = word;
       } else {
         const uint32_t w0 = transpose_bytes(b0, s), w1 = transpose_bytes(b1, s);
         if (in) {
-          out[s * (cb / 8) + chunk] = w0;
-          out[(4 + s) * (cb / 8) + chunk] = w1;
+          out[value_word(s, chunk, g, cb / 8)] = w0;
+          out[value_word(4 + s, chunk, g, cb / 8)] = w1;
         }
       }
     }
@@ -257,21 +258,21 @@ __device__ __forceinline__ void decode4(float* x, uint32_t biased, float scale, 
 
 template <class T, int BITS>
 __device__ void read_group(const RowArgs& a, int row0, int head, int session, int slot0) {
-  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
+  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb, g = slot0 >> 2;
   uint8_t* region = region_of(a.c, session, head);
   uint32_t w[2][2][2] = {};
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const uint32_t* in = codes_of(a.c, region, slot0, which);
+    const uint32_t* in = which ? values_of(a.c, region, slot0) : keys_of(a.c, region, slot0);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int chunk = c0 + 8 * u;
       if (chunk >= chunks) break;
       if constexpr (BITS == 4) {
-        w[which][u][0] = __ldg(in + (which ? (4 * (chunk & 1) + s) * (cb / 8) + (chunk >> 1) : 4 * chunk + s));
+        w[which][u][0] = in[which ? value_word(4 * (chunk & 1) + s, chunk >> 1, g, cb / 8) : 4 * key_unit(chunk, g, cb, 4) + s];
       } else {
-        w[which][u][0] = __ldg(in + (which ? s * (cb / 8) + chunk : 8 * chunk + s));
-        w[which][u][1] = __ldg(in + (which ? (4 + s) * (cb / 8) + chunk : 8 * chunk + 4 + s));
+        w[which][u][0] = in[which ? value_word(s, chunk, g, cb / 8) : 4 * key_unit(2 * chunk, g, cb, 8) + s];
+        w[which][u][1] = in[which ? value_word(4 + s, chunk, g, cb / 8) : 4 * key_unit(2 * chunk + 1, g, cb, 8) + s];
       }
     }
   }
@@ -566,7 +567,7 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   // CTAs (of four warps) that an item's slots are split over. SLOTS_RULE
   const int seen = window > 0 ? (int)std::min<long long>(c.slots, (long long)window + c.sinks) : c.slots;
   const AttendVariant f = attend_variant(c.bits, c.dim, dtype == kF32 ? 3 : 2, group);
-  const long long ctas = (long long)f.ctas * kv->n_sm, most = std::min<long long>({(seen + 511) / 512, kMaxPieces, kMaxPartials / std::max(1ll, items)});
+  const long long ctas = (long long)f.ctas * kv->n_sm, most = std::min<long long>({(seen + 128 * kAttendWarps - 1) / (128 * kAttendWarps), kMaxPieces, kMaxPartials / std::max(1ll, items)});
   int pieces = 0;  // 0: an item to a warp
   if (items < kAttendWarps * ctas && seen > 64)
     pieces = (int)std::max(1ll, std::min(most, 2 * items <= ctas ? ctas / items : (4 * ctas + items - 1) / items));

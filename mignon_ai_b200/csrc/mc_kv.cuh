@@ -3,20 +3,24 @@
 // A cache has `slots` places per session. Position p of a session lies at slot p while p < sinks
 // (the first positions are never overwritten) and at sinks + (p - sinks) % (slots - sinks) after
 // that: a ring behind pinned places. Every (session, head) owns one region of cap / 32 blocks (cap =
-// slots rounded up to 64), a block being all there is of 32 slots, so that one copy fetches it:
+// slots rounded up to 64), a block being all there is of 32 slots, so that one copy fetches its keys or its values:
 //
-//   keys' codes | values' codes | keys' scales and centers | values' scales and centers
+//   keys' codes | keys' scales and centers | values' codes | values' scales and centers
 //
-// Codes of four consecutive slots are interleaved, so that a 16-byte load gives a lane one 32-bit
-// word of each of the four, in the order in which the operands of an 8-bit m16n8k32 MMA want them
-// (slot s, group s / 4 of its block; cb code bytes per slot):
+// Codes of consecutive slots are interleaved, so that a 16-byte load gives a lane words of several of
+// them, in the order in which the operands of an 8-bit m16n8k32 MMA want them (cb code bytes per slot):
 //
-//   keys    word w of slot s is word 4 * w + s % 4 of its group's cb. 8 bits: word w holds
-//           dimensions 4w..4w+3. 4 bits: byte b of word w holds dimensions 8w + b (low) and
-//           8w + 4 + b (high). The contraction runs along the dimensions: a word is an operand.
-//   values  word n * ni + i of the group's cb holds dimension 8i + n (8 bits, ni = dim / 8), or
-//           16i + n (low) and 16i + 8 + n (high) (4 bits, ni = dim / 16), of four slots, slot s
-//           in byte s % 4. The contraction runs along the slots.
+//   keys    four slots at a time: the group's 16-byte unit of word w holds that word of its slots,
+//           one after the other. 8 bits: word w is dimensions 4w..4w+3. 4 bits: byte b of word w is
+//           dimensions 8w + b (low) and 8w + 4 + b (high). The contraction runs along the dimensions:
+//           a word is an operand.
+//   values  eight slots at a time (two groups u): word n * 2ni + u * ni + i is dimension 8i + n
+//           (8 bits, ni = dim / 8), or 16i + n (low) and 16i + 8 + n (high) (4 bits, ni = dim / 16), of
+//           the group's four slots, slot s in byte s % 4. The contraction runs along the slots.
+//
+// Within a group or pair the 16-byte units are permuted (key_unit, value_word) such that the eight
+// lanes that load together, two groups by four units of keys, or two n by the four pairs of
+// a block of values, meet eight different shared-memory banks of 16 bytes.
 //
 // A slot's scale and center are one word: scale in the low half, center in the high (bfloat16).
 #pragma once
@@ -52,14 +56,36 @@ __device__ __forceinline__ uint8_t* region_of(const Cache& c, int session, int h
 constexpr int kBlockSlots = 32;
 __host__ __device__ constexpr int block_bytes(int cb) { return kBlockSlots * (2 * cb + 8); }
 
-// The codes of slot s's group of four, and the words of scale and center from slot s on, in a region.
-__device__ __forceinline__ uint32_t* codes_of(const Cache& c, uint8_t* region, int s, bool values) {
-  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb) + (values ? kBlockSlots * c.cb : 0)) +
-         ((s & 31) >> 2) * c.cb;
+// The 16-byte unit of a group of four slots that holds word w of their keys (g: the group's number).
+__host__ __device__ __forceinline__ constexpr int key_unit(int w, int g, int cb, int bits) {
+  return bits == 8 ? w ^ (g & 1) : cb % 32 == 0 ? w ^ ((g & 1) << 2) : w;
+}
+// The word of a pair of groups that holds value word (n, i) of group g; ni words per n and group.
+__host__ __device__ __forceinline__ constexpr int value_swizzle(int n, int pair, int ni) {
+  return ni == 2   ? 2 * (pair & 3)
+         : ni == 4 ? (pair & 1) | ((pair & 2) << 1)
+         : ni == 8 ? pair & 3
+         : ni == 16 ? (pair & 3) | ((n & 1) << 2)
+                    : 0;
+}
+__host__ __device__ __forceinline__ constexpr int value_word(int n, int i, int g, int ni) {
+  const int at = (2 * n + (g & 1)) * ni + i;
+  return at ^ (value_swizzle(n, g >> 1, ni) << 2);
+}
+
+// The words of slot s's group of four keys, those of its pair of groups of values, and the words of
+// scale and center from slot s on, in a region.
+__device__ __forceinline__ uint32_t* keys_of(const Cache& c, uint8_t* region, int s) {
+  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb)) + ((s & 31) >> 2) * c.cb;
+}
+__device__ __forceinline__ uint32_t* values_of(const Cache& c, uint8_t* region, int s) {
+  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb) + kBlockSlots * (c.cb + 4)) +
+         ((s & 31) >> 3) * 2 * c.cb;
 }
 __device__ __forceinline__ uint32_t* params_of(const Cache& c, uint8_t* region, int s, bool values) {
-  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb) + 2 * kBlockSlots * c.cb) + (s & 31) +
-         (values ? kBlockSlots : 0);
+  return reinterpret_cast<uint32_t*>(region + (long long)(s >> 5) * block_bytes(c.cb) + kBlockSlots * c.cb +
+                                     (values ? kBlockSlots * (c.cb + 4) : 0)) +
+         (s & 31);
 }
 
 __device__ __forceinline__ int slot_of(const Cache& c, int pos) {

@@ -6,8 +6,8 @@
 //   o_d = sum_j (p_j vscale_j) m_jd + sum_j p_j vcenter_j,   p_j = exp(s_j - max)
 // and both run as 8-bit matrix products with exact 32-bit sums: the codes are the MMA's B operand
 // as they lie in memory (an and-or per word for 4 bits, nothing for 8), and the other side is cut
-// into 8-bit planes. A query row becomes PLANES signed digits of base 254 relative to its largest
-// element, a row of weights p_j vscale_j becomes a fixed-point integer of 16 bits (PLANES 2) or 23
+// into 8-bit planes. A query row becomes integers of 16 (PLANES 2) or 23 bits (3) relative to its
+// largest element, cut into signed bytes, a row of weights p_j vscale_j becomes a fixed-point integer of 16 bits (PLANES 2) or 23
 // bits (3) relative to the tile's largest, whose bytes are the planes: adding 2^23 to
 // the scaled weight leaves them in the mantissa, so cutting costs one fused multiply-add a weight.
 // PLANES is 3 for float32 queries (errors of 2^-23 and below, as float32 itself) and 2 for 16-bit
@@ -82,6 +82,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float b) {
   return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -110,10 +116,15 @@ __device__ __forceinline__ void load8(float (&x)[8], const T* p, bool vec) {
   for (int i = 0; i < 8; ++i) x[i] = to_float<T>(p[i]);
 }
 
-__device__ __forceinline__ void load_query(float (&x)[8], const void* p, long long i, int dtype, bool vec) {
-  if (dtype == kF32) load8<float>(x, static_cast<const float*>(p) + i, vec);
-  else if (dtype == kF16) load8<__half>(x, static_cast<const __half*>(p) + i, vec);
-  else load8<__nv_bfloat16>(x, static_cast<const __nv_bfloat16*>(p) + i, vec);
+// Elements 8 (cc + 4i) .. + 7 of a row, all loads at once; zeros past dim and for a row that is not there.
+template <class T, int KS>
+__device__ __forceinline__ void load_row(float (&x)[KS][8], const T* p, int cc, int dim, bool in, bool vec) {
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+    if (in && 8 * (cc + 4 * i) < dim) load8<T>(x[i], p + 8 * (cc + 4 * i), vec);
+  }
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 __device__ __forceinline__ void store_element(void* p, long long i, int dtype, float x) {
@@ -184,35 +195,37 @@ __device__ __forceinline__ SlotSpan slot_span(const Cache& c, int len, int windo
   return s;
 }
 
-// CTAs that share an SM: four where 128 registers a thread hold the work.
-constexpr int attend_ctas(int dim) { return dim <= 64 ? 4 : 3; }
-// Slots of a tile: 64 (two blocks) where two tiles a warp then fit shared memory, and where the third
-// plane leaves the registers for it.
+// CTAs that share an SM: 16 warps where 128 registers a thread hold the work.
+constexpr int attend_ctas(int dim, int planes) { return (planes == 3 && dim > 64 ? 8 : 16) / kAttendWarps; }
+// Slots of a tile: 64 (two blocks) where a tile's keys and values then fit, and where the third plane
+// leaves the registers for it.
 constexpr int attend_slots(int bits, int dim, int planes) {
-  return bits == 4 ? (planes == 3 && dim > 64 ? 32 : 64) : dim <= 32 ? 64 : 32;
+  return bits == 4 ? (planes == 3 && dim > 64 ? 32 : 64) : dim <= 48 ? 64 : 32;
 }
-constexpr int attend_stage_bytes(int bits, int dim, int planes) {
-  return attend_slots(bits, dim, planes) / kBlockSlots * block_bytes(dim * bits / 8);
+// A tile's keys (or values) with their scales and centers; each has buffers of its own, so that the next
+// keys are on their way during a tile's weights and value product, and the next values during its scores.
+constexpr int attend_part_bytes(int bits, int dim, int planes) {
+  return attend_slots(bits, dim, planes) * (dim * bits / 8 + 4);
 }
-// Tiles in flight per warp.
-constexpr int attend_stages(int bits, int dim, int planes) {
-  const int n = (221184 / attend_ctas(dim) - 1024) / (kAttendWarps * attend_stage_bytes(bits, dim, planes));
-  return n > 4 ? 4 : n < 2 ? 2 : n;
+constexpr int attend_parts(int bits, int dim, int planes) {
+  const int n = (221184 / attend_ctas(dim, planes) - 8192) / (kAttendWarps * attend_part_bytes(bits, dim, planes));
+  return n > 8 ? 8 : n < 2 ? 2 : n;
 }
 constexpr int attend_smem(int bits, int dim, int planes) {
-  const int ring = kAttendWarps * attend_stages(bits, dim, planes) * attend_stage_bytes(bits, dim, planes);
+  const int ring = kAttendWarps * attend_parts(bits, dim, planes) * attend_part_bytes(bits, dim, planes);
   const int join = kAttendWarps * kAttendRows * (dim + 2) * 4;  // the warps' results, in the same place
   return ring > join ? ring : join;
 }
 
-// Where a warp is in its work: an item (a session's up to eight query heads of one key/value head)
-// and a tile of its visible slots.
-struct AttendCursor {
-  unsigned item;  // items fit 31 bits, and a stride beyond them 32
+// What a warp does of an item (a session's up to eight query heads of one key/value head): tiles
+// [t, end) of its visible slots.
+struct AttendItem {
+  SlotSpan span;
   int t, end;
-  int tiles0, first1;
   const uint8_t* region;
 };
+// Items a warp may have opened (to copy their tiles) ahead of the one it works on, a power of two.
+constexpr int kAttendAhead = 8;
 
 // With few heads to an item the MMA's eight rows repeat them: HEADS rows of heads (8, 4 or 1), and the
 // rows of one head take different slots of the tile (row r: HEADS 4, the groups 2cc + r / 4; HEADS 1,
@@ -222,7 +235,7 @@ struct AttendCursor {
 // With a.pieces a CTA has one piece of one item; without, every warp goes through items of its own,
 // the next one's tiles already in flight.
 template <int BITS, int DIM, int PLANES, int HEADS>
-__global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM, PLANES)) attend_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int TS = attend_slots(BITS, DIM, PLANES), HALVES = TS / 32;
   constexpr int NJ = HEADS == 1 ? 1 : 4, NU = HEADS == 8 ? 2 : 1;  // slots of a half that a thread weighs: NJ x NU
   constexpr int CB = DIM * BITS / 8;             // code bytes per slot
@@ -230,15 +243,19 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
   constexpr int NI = BITS == 4 ? DIM / 16 : DIM / 8;  // value words of a group of slots per thread
   constexpr int NT = DIM / 8;                    // 8-column tiles of the output
   constexpr float kOne = BITS == 4 ? 0.125f : 1.0f;   // the MMA's codes are 8m (4 bits) or m
-  constexpr int STAGES = attend_stages(BITS, DIM, PLANES), STAGE = attend_stage_bytes(BITS, DIM, PLANES);
+  constexpr int PART = attend_part_bytes(BITS, DIM, PLANES), PARTS = attend_parts(BITS, DIM, PLANES);
+  constexpr int NK = (PARTS + 1) / 2, NV = PARTS / 2;  // buffers of keys and of values
+  constexpr int BLOCK_PART = kBlockSlots * (CB + 4);   // a block's keys or values
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kAttendWarps][STAGES];
+  __shared__ uint64_t full[kAttendWarps][NK + NV];
+  __shared__ AttendItem queue[kAttendWarps][kAttendAhead];
+  __shared__ const uint8_t* sources[kAttendWarps][4];  // of the tiles whose keys have been asked for
   const Cache& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, cc = lane & 3;
-  uint8_t* ring = smem + warp * STAGES * STAGE;
-  uint64_t* bars = full[warp];
+  uint8_t *kring = smem + warp * PARTS * PART, *vring = kring + NK * PART;
+  uint64_t *kfull = full[warp], *vfull = kfull + NK;
   if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(bars + i, 1);
+    for (int i = 0; i < NK + NV; ++i) mbar_init(kfull + i, 1);
     fence_barrier_init();
   }
   __syncwarp();
@@ -250,8 +267,14 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
   const int row_head = HEADS == 8 ? r : HEADS == 4 ? r & 3 : 0;  // the thread's query head in the item
   const int my_u = r >> 2, my_j = r & 3;                         // and its slots: see above
 
-  auto open = [&](AttendCursor& u, SlotSpan& span) {
-    const unsigned b = u.item / per, hr = u.item - b * per, head = a.row_groups == 1 ? hr : hr / a.row_groups;
+  // ---- the producer's side: lane 0 copies the tiles of this warp's items in their order. `next` is the
+  // item being copied, the opened-th of the warp's; the warp works on the taken-th.
+  AttendItem next;
+  const unsigned item0 = a.pieces ? blockIdx.x : blockIdx.x * kAttendWarps + warp;
+  unsigned next_id = item0;
+  int opened = 0, taken = 0, kissued = 0, vissued = 0, done = 0;
+  auto open = [&]() {  // next_id's, into the queue
+    const unsigned b = next_id / per, hr = next_id - b * per, head = a.row_groups == 1 ? hr : hr / a.row_groups;
     int session = a.sess ? a.sess[b] : b, len = 0;
     if ((unsigned)session < (unsigned)c.sessions) {
       len = a.lens[b];
@@ -259,53 +282,60 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
       if (lane == 0) atomicExch(c.error, 1);
       session = 0;
     }
-    span = slot_span<TS>(c, len, a.window);
-    u.t = 0;
-    u.end = span.tiles;
+    next.span = slot_span<TS>(c, len, a.window);
+    next.t = 0;
+    next.end = next.span.tiles;
     if (a.pieces) {  // an even share of the tiles, the first parts one more
-      const unsigned share = (unsigned)span.tiles / parts, more = (unsigned)span.tiles - share * parts;
-      u.t = part * share + min(part, more);
-      u.end = u.t + share + (part < more ? 1 : 0);
+      const unsigned share = (unsigned)next.span.tiles / parts, more = (unsigned)next.span.tiles - share * parts;
+      next.t = part * share + min(part, more);
+      next.end = next.t + share + (part < more ? 1 : 0);
     }
-    u.tiles0 = span.tiles0;
-    u.first1 = span.first1;
-    u.region = region_of(c, session, head);
+    next.region = region_of(c, session, head);
+    if (lane == 0) queue[warp][opened & (kAttendAhead - 1)] = next;
+    ++opened;
   };
-  auto slot_at = [](const AttendCursor& u, int t) { return (t < u.tiles0 ? t : u.first1 + t - u.tiles0) * TS; };
-
-  // ---- the producer's side: lane 0 copies the tiles of this warp's items in their order
-  AttendCursor next{a.pieces ? blockIdx.x : blockIdx.x * kAttendWarps + warp, 0, 0, 0, 0, nullptr};
-  AttendCursor cur = next;
-  int issued = 0;
-  SlotSpan scratch;
-  if (next.item < items) open(next, scratch);
-  auto issue = [&]() {
-    while (next.t >= next.end) {
-      if (next.item >= items) return;
-      next.item += stride;
-      if (next.item >= items) return;
-      open(next, scratch);
+  auto slot_at = [](const SlotSpan& s, int t) { return (t < s.tiles0 ? t : s.first1 + t - s.tiles0) * TS; };
+  auto copy = [&](uint8_t* dst, const uint8_t* src, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, PART);
+#pragma unroll
+    for (int h = 0; h < HALVES; ++h) bulk_load(dst + h * BLOCK_PART, src + h * 2 * BLOCK_PART, BLOCK_PART, bar);
+  };
+  auto issue_keys = [&]() {
+    while (next.t >= next.end) {  // on to the next item, if there is one and room for it in the queue
+      if (next_id + stride < next_id || next_id + stride >= items || opened - taken >= kAttendAhead) return false;
+      next_id += stride;
+      open();
     }
     if (lane == 0) {
-      const int slot0 = slot_at(next, next.t), stage = issued % STAGES;
-      mbar_arrive_expect_tx(bars + stage, STAGE);
-      bulk_load(ring + stage * STAGE, next.region + (long long)(slot0 >> 5) * block_bytes(CB), STAGE, bars + stage);
+      const uint8_t* src = next.region + (long long)(slot_at(next.span, next.t) >> 5) * block_bytes(CB);
+      sources[warp][kissued & 3] = src;
+      copy(kring + kissued % NK * PART, src, kfull + kissued % NK);
     }
-    ++issued;
+    ++kissued;
     ++next.t;
+    return true;
   };
-  for (int i = 0; i < STAGES; ++i) issue();
+  auto issue_values = [&]() {  // NV <= NK <= 4: the source is still there
+    if (vissued >= kissued) return;
+    if (lane == 0) copy(vring + vissued % NV * PART, sources[warp][vissued & 3] + BLOCK_PART, vfull + vissued % NV);
+    ++vissued;
+  };
 
-  int done = 0;
   bool ok = true;  // false after a wait gave up
   float2 o[NT];
   float top, total, csum;
-  int b, rows, h0;
-  for (; cur.item < items; cur.item += stride) {
-    SlotSpan span;
-    open(cur, span);
-    b = cur.item / per;
-    const unsigned hr = cur.item - b * per, head = a.row_groups == 1 ? hr : hr / a.row_groups, rg = hr - head * a.row_groups;
+  int b = 0, rows = 0, h0 = 0;
+  if (item0 < items) open();
+  for (unsigned id = item0; id < items; id += stride, ++taken) {
+    // the buffers that are free ask for tiles: at the start, and after items without any
+    while (kissued - done < NK && issue_keys()) {
+    }
+    while (vissued - done < NV && vissued < kissued) issue_values();
+    __syncwarp();
+    const AttendItem cur = queue[warp][taken & (kAttendAhead - 1)];
+    const SlotSpan& span = cur.span;
+    b = id / per;
+    const unsigned hr = id - b * per, head = a.row_groups == 1 ? hr : hr / a.row_groups, rg = hr - head * a.row_groups;
     rows = min(kAttendRows, a.group - (int)rg * kAttendRows);  // query heads of this item
     h0 = head * a.group + rg * kAttendRows;
 
@@ -315,38 +345,46 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
     {
       float x[KS][8], big = 0.f;
       const long long base = b * a.q.row + (h0 + row_head) * a.q.head;
+      const bool in = row_head < rows;
+      if (a.dtype == kF32) load_row<float, KS>(x, static_cast<const float*>(a.q.p) + base, cc, DIM, in, a.vec);
+      else if (a.dtype == kF16) load_row<__half, KS>(x, static_cast<const __half*>(a.q.p) + base, cc, DIM, in, a.vec);
+      else load_row<__nv_bfloat16, KS>(x, static_cast<const __nv_bfloat16*>(a.q.p) + base, cc, DIM, in, a.vec);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        const int w = cc + 4 * i;
-        const bool in = row_head < rows && 8 * w < DIM;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-        if (in) load_query(x[i], a.q.p, base + 8 * w, a.dtype, a.vec);
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           qsum = __fadd_rn(qsum, x[i][e]);
           big = fmaxf(big, fabsf(x[i][e]));
         }
-      }
 #pragma unroll
       for (int x = 1; x <= 2; x <<= 1) {
         qsum = __fadd_rn(qsum, __shfl_xor_sync(~0u, qsum, x));
         big = fmaxf(big, __shfl_xor_sync(~0u, big, x));
       }
-      const float inv = row_inv_step(big);
-      // a non-finite query has no digits: its scores become NaN by qsum
-      qstep = __fmul_rn(__fmul_rn(row_step(big), a.scale), kOne / 254.0f);
+      // n = q / step in 16 or 23 bits, cut into signed bytes: adding 0x80 to the lower ones carries into
+      // the next what a byte above 127 stands for. 1.5 * 2^23 leaves n in the mantissa's low bits.
+      constexpr float kMost = PLANES == 3 ? 4161000.0f : 32600.0f, kBias = PLANES == 3 ? 32896.0f : 128.0f;
+      // below 1e-30 the inverse leaves float32's range: such a row counts as zeros; a non-finite query has
+      // no digits: its scores become NaN by qsum
+      const float inv = big >= 1e-30f ? __fdividef(kMost, big) : 0.f;
+      qstep = __fmul_rn(big >= 1e-30f ? __fmul_rn(big, 1.0f / kMost) : 0.f, __fmul_rn(a.scale, kOne));
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        uint32_t u[8][3];
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) slice3_bits(x[i][e], inv, u[e][0], u[e][1], u[e][2]);
+        for (int e = 0; e < 2; ++e) {
+          uint32_t u[4];
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-          qa[i][p][0] = pack_low_bytes(u[0][p], u[1][p], u[2][p], u[3][p]);
-          qa[i][p][1] = pack_low_bytes(u[4][p], u[5][p], u[6][p], u[7][p]);
+          for (int d = 0; d < 4; ++d) u[d] = __float_as_uint(__fadd_rn(__fmaf_rn(x[i][4 * e + d], inv, 12582912.0f), kBias));
+          const uint32_t lo01 = __byte_perm(u[0], u[1], 0x5140), lo23 = __byte_perm(u[2], u[3], 0x5140);
+          qa[i][PLANES - 1][e] = __byte_perm(lo01, lo23, 0x5410) ^ 0x80808080u;
+          qa[i][PLANES - 2][e] = __byte_perm(lo01, lo23, 0x7632);
+          if constexpr (PLANES == 3) {
+            qa[i][1][e] ^= 0x80808080u;
+            // bits 16-22 above the mantissa's 0x40: v - 64 as a signed byte
+            const uint32_t hi = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410);
+            qa[i][0][e] = ((hi | 0x80808080u) - 0x40404040u) ^ 0x80808080u;
+          }
         }
-      }
       qsum = __fmul_rn(qsum, a.scale);
     }
 #pragma unroll
@@ -354,17 +392,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
     top = -INFINITY, total = 0.f, csum = 0.f;
 
     for (int t = cur.t; t < cur.end; ++t) {
-      const int slot0 = slot_at(cur, t), stage = done % STAGES;
-      ok = __all_sync(~0u, ok && mbar_wait_or_abort(bars + stage, (done / STAGES) & 1, kErrWaitFull));
+      const int slot0 = slot_at(span, t);
+      ok = __all_sync(~0u, mbar_wait_or_abort(kfull + done % NK, (done / NK) & 1, kErrWaitFull));
       if (!ok) break;
-      const uint8_t* tile = ring + stage * STAGE;
+      const uint8_t* ktile = kring + done % NK * PART;
       // ---- scores: s[h][j * NU + u] of slot 32h + slot_in(j, u), this thread's share of the tile
       auto slot_in = [&](int j, int u) { return 8 * cc + 4 * (HEADS == 8 ? u : my_u) + (HEADS == 1 ? my_j : j); };
       float s[HALVES][NJ * NU];
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        const uint8_t* kc = tile + h * block_bytes(CB) + r * 4 * CB;
-        const uint32_t* kparam = reinterpret_cast<const uint32_t*>(tile + h * block_bytes(CB) + 2 * kBlockSlots * CB);
+        const uint8_t* kc = ktile + h * BLOCK_PART + r * 4 * CB;
+        const uint32_t* kparam = reinterpret_cast<const uint32_t*>(ktile + h * BLOCK_PART + kBlockSlots * CB);
         int acc[4][4], acc3[4][4];
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
@@ -373,12 +411,12 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
           if (DIM % 32 == 0 || 8 * w < DIM) {
             if constexpr (BITS == 4) {
               uint32_t x[4];
-              load_words<4>(x, reinterpret_cast<const uint32_t*>(kc + 16 * w));
+              load_words<4>(x, reinterpret_cast<const uint32_t*>(kc + 16 * key_unit(w, r, CB, 4)));
 #pragma unroll
               for (int j = 0; j < 4; ++j) b0[j] = low_codes(x[j]), b1[j] = high_codes(x[j]);
             } else {
-              load_words<4>(b0, reinterpret_cast<const uint32_t*>(kc + 32 * w));
-              load_words<4>(b1, reinterpret_cast<const uint32_t*>(kc + 32 * w + 16));
+              load_words<4>(b0, reinterpret_cast<const uint32_t*>(kc + 16 * key_unit(2 * w, r, CB, 8)));
+              load_words<4>(b1, reinterpret_cast<const uint32_t*>(kc + 16 * key_unit(2 * w + 1, r, CB, 8)));
             }
           } else {
 #pragma unroll
@@ -396,9 +434,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
           }
         }
         auto score = [&](int first, int second, int third, uint32_t w) {
-          // |first| <= 128 * 127 * 127, so 254 * first + second fits 32 bits
-          float f = (float)(first * 254 + second);
-          if constexpr (PLANES == 3) f = __fmaf_rn((float)third, 1.0f / 254.0f, f);
+          // |first| <= 128 * 128 * 127, so 256 * first + second fits 32 bits
+          float f = (float)(first * 256 + second);
+          if constexpr (PLANES == 3) f = __fmaf_rn(f, 256.0f, (float)third);
           return __fmaf_rn(__fmul_rn(f, qstep), param_scale(w), __fmul_rn(param_center(w), qsum));
         };
         if constexpr (HEADS == 8) {
@@ -431,6 +469,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
           }
         }
       }
+      __syncwarp();  // every lane has read the keys: their buffer takes the next tile's
+      issue_keys();
       const bool whole = slot0 + TS <= span.e0 || (slot0 >= span.s1 && slot0 + TS <= span.e1);
       if (!whole) {
 #pragma unroll
@@ -448,7 +488,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int e = 0; e < NJ * NU; ++e) m = fmaxf(m, s[h][e]);
+        for (int e = 0; e + 1 < NJ * NU; e += 2) m = max3(m, s[h][e], s[h][e + 1]);
+      if constexpr (HEADS == 1) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) m = fmaxf(m, s[h][0]);
+      }
       m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
       m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
       if constexpr (HEADS <= 4) m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
@@ -465,12 +509,14 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
         top = m;
       }
       // ---- weights p, their sum, and p * vscale in place of the scores
+      ok = __all_sync(~0u, mbar_wait_or_abort(vfull + done % NV, (done / NV) & 1, kErrWaitFull));
+      if (!ok) break;
+      const uint8_t* vtile = vring + done % NV * PART;
       float pmax = 0.f;
       const float shift = top == -INFINITY ? 0.f : top;  // nothing but scores of minus infinity so far
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        const uint32_t* vparam =
-            reinterpret_cast<const uint32_t*>(tile + h * block_bytes(CB) + 2 * kBlockSlots * CB) + kBlockSlots;
+        const uint32_t* vparam = reinterpret_cast<const uint32_t*>(vtile + h * BLOCK_PART + kBlockSlots * CB);
         uint32_t vp[NJ * NU];
         if constexpr (HEADS == 1) {
           vp[0] = vparam[slot_in(0, 0)];
@@ -490,13 +536,15 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
           total = __fadd_rn(total, p);
           csum = __fmaf_rn(p, param_center(w), csum);
           s[h][e] = __fmul_rn(p, param_scale(w));
-          pmax = fmaxf(pmax, s[h][e]);
+          if (e & 1) pmax = max3(pmax, s[h][e - 1], s[h][e]);
         }
+        if constexpr (HEADS == 1) pmax = fmaxf(pmax, s[h][0]);
       }
       pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 1));
       pmax = fmaxf(pmax, __shfl_xor_sync(~0u, pmax, 2));
-      // below 1e-30 the inverse leaves float32's range: such weights count as nothing
-      constexpr float kFull = PLANES == 3 ? 8388607.0f : 65535.0f;
+      // below 1e-30 the inverse leaves float32's range: such weights count as nothing. kFull leaves room
+      // below 2^23 and 2^16 for the quotient's and the product's rounding
+      constexpr float kFull = PLANES == 3 ? 8388600.0f : 65534.9f;
       const float inv = pmax > 1e-30f ? __fdividef(kFull, pmax) : 0.f;
       const float unit = __fmul_rn(pmax > 1e-30f ? pmax : 0.f, kOne / kFull);
       // ---- the weights' bytes as A operands: plane 0 (highest) in rows 0-7, plane 1 in rows 8-15;
@@ -507,7 +555,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
         uint32_t x[NJ * NU];
 #pragma unroll
         for (int e = 0; e < NJ * NU; ++e)
-          x[e] = __float_as_uint(fminf(__fmaf_rn(s[h][e], inv, 8388608.0f), 8388608.0f + kFull));
+          x[e] = __float_as_uint(__fmaf_rn(s[h][e], inv, 8388608.0f));
         if constexpr (HEADS == 1) {
 #pragma unroll
           for (int p = 0; p < PLANES; ++p) {
@@ -545,11 +593,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
       for (int i0 = 0; i0 < NI; i0 += STEP) {
         uint32_t v[HALVES][2][STEP];
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            load_words<STEP>(v[h][u], reinterpret_cast<const uint32_t*>(tile + h * block_bytes(CB) + kBlockSlots * CB) +
-                                          (2 * cc + u) * CB + r * NI + i0);
+        for (int h = 0; h < HALVES; ++h) {
+          const uint32_t* pair = reinterpret_cast<const uint32_t*>(vtile + h * BLOCK_PART) + cc * 2 * CB;
+          if constexpr (NI == 2) {
+            uint32_t both[4];
+            load_words<4>(both, pair + value_word(r, 0, 2 * cc, NI));
+            v[h][0][0] = both[0], v[h][0][1] = both[1], v[h][1][0] = both[2], v[h][1][1] = both[3];
+          } else {
+            load_words<STEP>(v[h][0], pair + value_word(r, i0, 2 * cc, NI));
+            load_words<STEP>(v[h][1], pair + value_word(r, i0, 2 * cc + 1, NI));
+          }
+        }
 #pragma unroll
         for (int i = 0; i < STEP; ++i) {
 #pragma unroll
@@ -579,8 +633,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
         }
       }
       ++done;
-      __syncwarp();  // every lane has read the stage: it takes the next tile
-      issue();
+      __syncwarp();  // and the values
+      issue_values();
     }
     if (!ok) break;
     // ---- the sums over the row's quad and over the rows of its head; the centers' share goes to
@@ -614,8 +668,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
     }
   }
   // a wait that gave up: never leave with copies in flight into this warp's buffers
-  if (!ok && lane == 0)
-    for (; done < issued; ++done) mbar_wait(bars + done % STAGES, (done / STAGES) & 1, kErrWaitFull);
+  if (!ok && lane == 0) {
+    for (int i = max(0, kissued - NK); i < kissued; ++i) mbar_wait(kfull + i % NK, (i / NK) & 1, kErrWaitFull);
+    for (int i = max(0, vissued - NV); i < vissued; ++i) mbar_wait(vfull + i % NV, (i / NV) & 1, kErrWaitFull);
+  }
 
   if (a.pieces) {
     constexpr int W = 2 + DIM;  // maximum, sum, weighted values of a row
@@ -661,39 +717,49 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM)) attend_ke
     if (!last) return;
     __threadfence();
     const float* all = a.partial + item * a.pieces * kAttendRows * W;
-    // the pieces' factors: a quarter-warp's worth of threads per row
-    {
-      const int row = threadIdx.x / 16, l16 = threadIdx.x % 16;  // 128 threads: eight rows
+    {  // the pieces' factors: a share of the threads to a row, all their loads at once
+      constexpr int SHARE = kAttendWarps * 32 / kAttendRows, PER = kMaxPieces / SHARE;
+      static_assert(SHARE == 16 || SHARE == 32, "a row's threads are in one warp");
+      const int row = threadIdx.x / SHARE, l16 = threadIdx.x % SHARE;
+      float2 ml[PER];
       float m = -INFINITY, l = 0.f;
-      if (row < rows) {
-        for (int p = l16; p < a.pieces; p += 16) m = fmaxf(m, __ldcg(all + (p * kAttendRows + row) * W));
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int p = l16 + SHARE * i;
+        ml[i] = make_float2(-INFINITY, 0.f);
+        if (row < rows && p < a.pieces) ml[i] = __ldcg(reinterpret_cast<const float2*>(all + (p * kAttendRows + row) * W));
       }
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
-      if (row < rows) {
-        for (int p = l16; p < a.pieces; p += 16) {
-          const float pm = __ldcg(all + (p * kAttendRows + row) * W), keep = pm == -INFINITY ? 0.f : exp2_fast(__fsub_rn(pm, m));
-          keeps[row * kMaxPieces + p] = keep;
-          l = __fmaf_rn(__ldcg(all + (p * kAttendRows + row) * W + 1), keep, l);
-        }
+      for (int i = 0; i < PER; ++i) m = fmaxf(m, ml[i].x);
+#pragma unroll
+      for (int x = 1; x < SHARE; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const float keep = ml[i].x == -INFINITY ? 0.f : exp2_fast(__fsub_rn(ml[i].x, m));
+        keeps[row * kMaxPieces + l16 + SHARE * i] = keep;
+        l = __fmaf_rn(ml[i].y, keep, l);
       }
 #pragma unroll
-      for (int x = 1; x < 16; x <<= 1) l = __fadd_rn(l, __shfl_xor_sync(~0u, l, x));
+      for (int x = 1; x < SHARE; x <<= 1) l = __fadd_rn(l, __shfl_xor_sync(~0u, l, x));
       if (l16 == 0) results[row] = l;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < rows * (DIM / 2); e += kAttendWarps * 32) {
       const int row = e / (DIM / 2), d = 2 * (e % (DIM / 2));
-      float x0 = 0.f, x1 = 0.f;
-#pragma unroll 16
-      for (int p = 0; p < a.pieces; ++p) {
-        const float2 q = __ldcg(reinterpret_cast<const float2*>(all + (p * kAttendRows + row) * W + 2 + d));
-        const float keep = keeps[row * kMaxPieces + p];
-        x0 = __fmaf_rn(q.x, keep, x0);
-        x1 = __fmaf_rn(q.y, keep, x1);
+      float2 x = make_float2(0.f, 0.f);
+      for (int p0 = 0; p0 < a.pieces; p0 += 32) {  // 32 loads in flight; past the last piece the factor is zero
+        float2 q[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          q[i] = __ldcg(reinterpret_cast<const float2*>(all + (min(p0 + i, a.pieces - 1) * kAttendRows + row) * W + 2 + d));
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float keep = p0 + i < a.pieces ? keeps[row * kMaxPieces + p0 + i] : 0.f;
+          x = fma2(q[i], make_float2(keep, keep), x);
+        }
       }
       const float l = results[row], inv = l == 0.f ? 0.f : __fdiv_rn(1.0f, l);
-      store_pair(a.out.p, b * a.out.row + (h0 + row) * a.out.head + d, a.dtype, a.vec, __fmul_rn(x0, inv), __fmul_rn(x1, inv));
+      store_pair(a.out.p, b * a.out.row + (h0 + row) * a.out.head + d, a.dtype, a.vec, __fmul_rn(x.x, inv), __fmul_rn(x.y, inv));
     }
     if (threadIdx.x == 0) a.arrived[item] = 0;
   }
@@ -707,7 +773,7 @@ struct AttendVariant {
 template <int BITS, int DIM, int PLANES>
 inline AttendVariant attend_variant_of(int heads) {
   return {heads > 4 ? attend_kernel<BITS, DIM, PLANES, 8> : heads > 1 ? attend_kernel<BITS, DIM, PLANES, 4> : attend_kernel<BITS, DIM, PLANES, 1>,
-          attend_smem(BITS, DIM, PLANES), attend_ctas(DIM)};
+          attend_smem(BITS, DIM, PLANES), attend_ctas(DIM, PLANES)};
 }
 template <int BITS, int DIM>
 inline AttendVariant attend_variant_of(int planes, int heads) {
