@@ -33,23 +33,9 @@ struct RowArgs {
   Rows k, v;
   int n_rows, n_seg;
   const int *start, *sess, *pos0, *lens;
-  int vec;  // rows are aligned for 16-byte accesses of eight elements
+  int vec;         // rows are aligned for 16-byte accesses of eight elements
+  int warp_heads;  // heads that a warp of segment_kernel takes one after the other
 };
-
-// The last i of [0, n) for which `at_most` holds, by a whole warp with 32 probes a round (0 if it
-// holds nowhere; it must not hold again after it failed).
-template <class F>
-__device__ __forceinline__ int last_at_most(int n, F at_most) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const bool below = at < hi && (lane == 0 || at_most(at));
-    lo += (31 - __clz(__ballot_sync(~0u, below))) * step;
-    hi = min(hi, lo + step);
-  }
-  return lo;
-}
 
 // Where a row goes or comes from: its session and slot, slot -1 for none.
 struct RowPlace {
@@ -181,143 +167,204 @@ __device__ __forceinline__ uint32_t transpose_bytes(uint32_t x, int s) {
   return s & 2 ? __byte_perm(y, x, 0x7632) : __byte_perm(x, y, 0x5410);
 }
 
-// The four rows of one group of slots, lane (s, c): row s, dimensions 8c.. and 64 + 8c..
-template <class T, int BITS>
-__device__ void write_group(const RowArgs& a, int row0, int head, int session, int slot0) {
-  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb, g = slot0 >> 2;
-  uint8_t* region = region_of(a.c, session, head);
-  float x[2][2][8];
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const Rows& r = which ? a.v : a.k;
-    const T* p = static_cast<const T*>(r.p) + (row0 + s) * r.row + head * r.head;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (c0 + 8 * u < chunks) load8<T>(x[which][u], p + 8 * (c0 + 8 * u), a.vec);
-  }
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    float hi = -INFINITY, lo = INFINITY;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (c0 + 8 * u < chunks) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) hi = max_nan(hi, x[which][u][e]), lo = min_nan(lo, x[which][u][e]);
-      }
-#pragma unroll
-    for (int o = 1; o <= 4; o <<= 1) {
-      hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
-      lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
-    }
-    const Quant q = quant_of(hi, lo, BITS);
-    uint32_t* out = which ? values_of(a.c, region, slot0) : keys_of(a.c, region, slot0);
+// Where a lane's words of a group of slots are, from the start of its block: the same for every head.
+// Lane (s, c): row s, chunks of eight dimensions c and c + 8 (u). Keys: 4 bits one word a chunk, 8 bits two;
+// values: likewise, after the transpose.
+template <int BITS>
+struct LaneWords {
+  static constexpr int W = BITS / 4;
+  int key[2][W], value[2][W];
+  __device__ __forceinline__ LaneWords(int slot0, int cb) {
+    const int lane = threadIdx.x & 31, s = lane >> 3, c = lane & 7, g = slot0 >> 2, ni = cb / 8;
+    const int kbase = ((slot0 & 31) >> 2) * cb, vbase = kBlockSlots * (cb + 4) / 4 + ((slot0 & 31) >> 3) * 2 * cb;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if (8 * u >= chunks) break;  // uniform
-      const int chunk = c0 + 8 * u;
-      const bool in = chunk < chunks;
-      uint32_t code[8];
+      const int chunk = c + 8 * u;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) code[e] = code_bits(q, in ? x[which][u][e] : 0.f, BITS);
-      const uint32_t b0 = pack_low_bytes(code[0], code[1], code[2], code[3]);
-      const uint32_t b1 = pack_low_bytes(code[4], code[5], code[6], code[7]);
-      if (which == 0) {
-        if constexpr (BITS == 4) {
-          if (in) out[4 * key_unit(chunk, g, cb, 4) + s] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
-        } else if (in) {
-          out[4 * key_unit(2 * chunk, g, cb, 8) + s] = b0;
-          out[4 * key_unit(2 * chunk + 1, g, cb, 8) + s] = b1;
-        }
-      } else if constexpr (BITS == 4) {
-        // even chunks (low nibbles) keep dimensions n = 0..3 of the pair, odd ones (high) n = 4..7
-        const bool odd = chunk & 1;
-        const uint32_t got = __shfl_xor_sync(~0u, odd ? b0 : b1, 1);
-        const uint32_t low = odd ? got : b0, high = odd ? b1 : got;
-        const uint32_t word = transpose_bytes((low & 0x0F0F0F0Fu) | ((high << 4) & 0xF0F0F0F0u), s);
-        if (in) out[value_word(4 * (chunk & 1) + s, chunk >> 1, g, cb / 8)] = word;
-      } else {
-        const uint32_t w0 = transpose_bytes(b0, s), w1 = transpose_bytes(b1, s);
-        if (in) {
-          out[value_word(s, chunk, g, cb / 8)] = w0;
-          out[value_word(4 + s, chunk, g, cb / 8)] = w1;
-        }
+      for (int w = 0; w < W; ++w) {
+        key[u][w] = kbase + 4 * key_unit(W * chunk + w, g, cb, BITS) + s;
+        value[u][w] = vbase + (BITS == 4 ? value_word(4 * (chunk & 1) + s, chunk >> 1, g, ni) : value_word(4 * w + s, chunk, g, ni));
       }
     }
-    if (c0 == 0) params_of(a.c, region, slot0, which)[s] = param_word(q);
+  }
+};
+
+// The words of scale and center of slot0's keys, from the start of its block (the values': kBlockSlots
+// (cb + 4) bytes on).
+__device__ __forceinline__ int param_word_at(int slot0, int cb) { return kBlockSlots * cb / 4 + (slot0 & 31); }
+
+// Eight consecutive elements as they are in memory.
+template <class T>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      alignas(16) T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float<T>(e[i]);
+  }
+};
+
+// The four rows of one group of slots, heads [h0, h1).
+template <class T, int BITS>
+__device__ void write_group(const RowArgs& a, int row0, int h0, int h1, int session, int slot0) {
+  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
+  const LaneWords<BITS> at(slot0, cb);
+  const int param_at = param_word_at(slot0, cb) + s;
+  uint32_t* block = reinterpret_cast<uint32_t*>(region_of(a.c, session, h0) + (long long)(slot0 >> 5) * block_bytes(cb));
+  const T* rows[2] = {static_cast<const T*>(a.k.p) + (row0 + s) * a.k.row + h0 * a.k.head + 8 * c0,
+                      static_cast<const T*>(a.v.p) + (row0 + s) * a.v.row + h0 * a.v.head + 8 * c0};
+  const bool in[2] = {c0 < chunks, c0 + 8 < chunks};
+  for (int h = h0; h < h1; ++h) {
+    Raw8<T> raw[2][2];
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (in[u]) raw[which][u].load(rows[which] + 64 * u, a.vec);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (in[u]) {
+          float x[8];
+          raw[which][u].get(x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) hi = max_nan(hi, x[e]), lo = min_nan(lo, x[e]);
+        }
+#pragma unroll
+      for (int o = 1; o <= 4; o <<= 1) {
+        hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
+        lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
+      }
+      const Quant q = quant_of(hi, lo, BITS);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (8 * u >= chunks) break;  // uniform
+        uint32_t code[8];
+        float x[8];
+        raw[which][u].get(x);
+        code_bits8<BITS>(q, x, code);
+        const uint32_t b0 = pack_low_bytes(code[0], code[1], code[2], code[3]);
+        const uint32_t b1 = pack_low_bytes(code[4], code[5], code[6], code[7]);
+        if (which == 0) {
+          if constexpr (BITS == 4) {
+            if (in[u]) block[at.key[u][0]] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
+          } else if (in[u]) {
+            block[at.key[u][0]] = b0;
+            block[at.key[u][BITS / 4 - 1]] = b1;
+          }
+        } else if constexpr (BITS == 4) {
+          // even chunks (low nibbles) keep dimensions n = 0..3 of the pair, odd ones (high) n = 4..7
+          const bool odd = c0 & 1;
+          const uint32_t got = __shfl_xor_sync(~0u, odd ? b0 : b1, 1);
+          const uint32_t low = odd ? got : b0, high = odd ? b1 : got;
+          const uint32_t word = transpose_bytes((low & 0x0F0F0F0Fu) | ((high << 4) & 0xF0F0F0F0u), s);
+          if (in[u]) block[at.value[u][0]] = word;
+        } else {
+          const uint32_t w0 = transpose_bytes(b0, s), w1 = transpose_bytes(b1, s);
+          if (in[u]) {
+            block[at.value[u][0]] = w0;
+            block[at.value[u][BITS / 4 - 1]] = w1;
+          }
+        }
+      }
+      if (c0 == 0) block[param_at + (which ? kBlockSlots * (cb + 4) / 4 : 0)] = param_word(q);
+      rows[which] += which ? a.v.head : a.k.head;
+    }
+    block += a.c.region / 4;
   }
 }
 
 // Four codes as they are in bytes biased by 128: 2^23 + byte is a float whose low byte it is.
-__device__ __forceinline__ void decode4(float* x, uint32_t biased, float scale, float center) {
+__device__ __forceinline__ void decode4(float* x, uint32_t biased, float2 scale, float2 center) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float m = __fsub_rn(__uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7440 + e)), 8388736.0f);
-    x[e] = __fmaf_rn(scale, m, center);
+  for (int e = 0; e < 4; e += 2) {
+    const float2 f = make_float2(__uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7440 + e)),
+                                 __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7441 + e)));
+    const float2 y = fma2(scale, add2(f, make_float2(-8388736.0f, -8388736.0f)), center);
+    x[e] = y.x, x[e + 1] = y.y;
   }
 }
 
 template <class T, int BITS>
-__device__ void read_group(const RowArgs& a, int row0, int head, int session, int slot0) {
-  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb, g = slot0 >> 2;
-  uint8_t* region = region_of(a.c, session, head);
-  uint32_t w[2][2][2] = {};
+__device__ void read_group(const RowArgs& a, int row0, int h0, int h1, int session, int slot0) {
+  constexpr int W = BITS / 4;
+  const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
+  const LaneWords<BITS> at(slot0, cb);
+  const int param_at = param_word_at(slot0, cb) + s;
+  const uint32_t* block = reinterpret_cast<const uint32_t*>(region_of(a.c, session, h0) + (long long)(slot0 >> 5) * block_bytes(cb));
+  T* rows[2] = {static_cast<T*>(a.k.p) + (row0 + s) * a.k.row + h0 * a.k.head + 8 * c0,
+                static_cast<T*>(a.v.p) + (row0 + s) * a.v.row + h0 * a.v.head + 8 * c0};
+  const bool in[2] = {c0 < chunks, c0 + 8 < chunks};
+  for (int h = h0; h < h1; ++h) {
+    uint32_t w[2][2][W] = {};
+    uint32_t param[2];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const uint32_t* in = which ? values_of(a.c, region, slot0) : keys_of(a.c, region, slot0);
+    for (int which = 0; which < 2; ++which) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int chunk = c0 + 8 * u;
-      if (chunk >= chunks) break;
-      if constexpr (BITS == 4) {
-        w[which][u][0] = in[which ? value_word(4 * (chunk & 1) + s, chunk >> 1, g, cb / 8) : 4 * key_unit(chunk, g, cb, 4) + s];
-      } else {
-        w[which][u][0] = in[which ? value_word(s, chunk, g, cb / 8) : 4 * key_unit(2 * chunk, g, cb, 8) + s];
-        w[which][u][1] = in[which ? value_word(4 + s, chunk, g, cb / 8) : 4 * key_unit(2 * chunk + 1, g, cb, 8) + s];
-      }
-    }
-  }
-  const uint32_t param[2] = {params_of(a.c, region, slot0, false)[s], params_of(a.c, region, slot0, true)[s]};
+      for (int u = 0; u < 2; ++u)
+        if (in[u]) {
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const Rows& r = which ? a.v : a.k;
-    T* p = static_cast<T*>(r.p) + (row0 + s) * r.row + head * r.head;
-    // nibbles come as bytes 16c + 8 = 8m, so their scale is an eighth
-    const float scale = __fmul_rn(param_scale(param[which]), BITS == 4 ? 0.125f : 1.0f), center = param_center(param[which]);
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (8 * u >= chunks) break;  // uniform
-      const int chunk = c0 + 8 * u;
-      uint32_t b0, b1;
-      if constexpr (BITS == 4) {
-        const uint32_t word = w[which][u][0];
-        if (which == 0) {
-          b0 = low_codes(word), b1 = high_codes(word);
-        } else {
-          const uint32_t mine = transpose_bytes(word, s), other = __shfl_xor_sync(~0u, mine, 1);
-          b0 = chunk & 1 ? high_codes(other) : low_codes(mine);
-          b1 = chunk & 1 ? high_codes(mine) : low_codes(other);
+          for (int i = 0; i < W; ++i) w[which][u][i] = block[which ? at.value[u][i] : at.key[u][i]];
         }
-      } else {
-        b0 = which ? transpose_bytes(w[which][u][0], s) : w[which][u][0];
-        b1 = which ? transpose_bytes(w[which][u][1], s) : w[which][u][1];
-      }
-      float y[8];
-      decode4(y, b0 ^ 0x80808080u, scale, center);
-      decode4(y + 4, b1 ^ 0x80808080u, scale, center);
-      if (chunk < chunks) store8<T>(p + 8 * chunk, y, a.vec);
+      param[which] = block[param_at + (which ? kBlockSlots * (cb + 4) / 4 : 0)];
     }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      // nibbles come as bytes 16c + 8 = 8m, so their scale is an eighth
+      const float scale = __fmul_rn(param_scale(param[which]), BITS == 4 ? 0.125f : 1.0f), center = param_center(param[which]);
+      const float2 scale2 = make_float2(scale, scale), center2 = make_float2(center, center);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (8 * u >= chunks) break;  // uniform
+        uint32_t b0, b1;
+        if constexpr (BITS == 4) {
+          const uint32_t word = w[which][u][0];
+          if (which == 0) {
+            b0 = low_codes(word), b1 = high_codes(word);
+          } else {
+            const uint32_t mine = transpose_bytes(word, s), other = __shfl_xor_sync(~0u, mine, 1);
+            b0 = c0 & 1 ? high_codes(other) : low_codes(mine);
+            b1 = c0 & 1 ? high_codes(mine) : low_codes(other);
+          }
+        } else {
+          b0 = which ? transpose_bytes(w[which][u][0], s) : w[which][u][0];
+          b1 = which ? transpose_bytes(w[which][u][W - 1], s) : w[which][u][W - 1];
+        }
+        float y[8];
+        decode4(y, b0 ^ 0x80808080u, scale2, center2);
+        decode4(y + 4, b1 ^ 0x80808080u, scale2, center2);
+        if (in[u]) store8<T>(rows[which] + 64 * u, y, a.vec);
+      }
+      rows[which] += which ? a.v.head : a.k.head;
+    }
+    block += a.c.region / 4;
   }
 }
 
-// One warp per (group of slots, head) of the segments. Segment b's groups have numbers from
-// start[b] / 4 + 2b on: room for its rows / 4 + 2, and it has no more whatever its first slot.
+// One warp per group of slots and a.warp_heads heads of the segments. Segment b's groups have numbers
+// from start[b] / 4 + 2b on: room for its rows / 4 + 2, and it has no more whatever its first slot.
 template <class T, bool WRITE>
-__global__ void __launch_bounds__(kCacheThreads) segment_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5) : 6) segment_kernel(const __grid_constant__ RowArgs a) {
   __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
-  const long long group = item / a.c.heads;
-  const int head = (int)(item % a.c.heads);
+  const int parts = (a.c.heads + a.warp_heads - 1) / a.warp_heads;
+  const long long group = item / parts;
+  const int h0 = (int)(item - group * parts) * a.warp_heads, h1 = min(h0 + a.warp_heads, a.c.heads);
   if constexpr (!WRITE) {  // rows before the first segment and after the last come back as zeros
     const int lo = max(0, min(a.start[0], a.n_rows)), hi = max(lo, min(a.start[a.n_seg], a.n_rows));
     for (long long e = item; e < (long long)(lo + a.n_rows - hi) * a.c.heads; e += (long long)gridDim.x * (kCacheThreads / 32)) {
@@ -339,20 +386,22 @@ __global__ void __launch_bounds__(kCacheThreads) segment_kernel(const __grid_con
   const int slot0 = __shfl_sync(~0u, p.slot, 0);
   if (__all_sync(~0u, count == 4 && slot0 >= 0 && (slot0 & 3) == 0 && p.slot == slot0 + s)) {
     if (a.c.bits == 4) {
-      if constexpr (WRITE) write_group<T, 4>(a, row0, head, p.session, slot0);
-      else read_group<T, 4>(a, row0, head, p.session, slot0);
+      if constexpr (WRITE) write_group<T, 4>(a, row0, h0, h1, p.session, slot0);
+      else read_group<T, 4>(a, row0, h0, h1, p.session, slot0);
     } else {
-      if constexpr (WRITE) write_group<T, 8>(a, row0, head, p.session, slot0);
-      else read_group<T, 8>(a, row0, head, p.session, slot0);
+      if constexpr (WRITE) write_group<T, 8>(a, row0, h0, h1, p.session, slot0);
+      else read_group<T, 8>(a, row0, h0, h1, p.session, slot0);
     }
     return;
   }
   for (int i = 0; i < count; ++i) {
     const RowPlace q{p.session, __shfl_sync(~0u, p.slot, 8 * i)};
-    if constexpr (WRITE) {
-      if (q.slot >= 0) write_row<T>(a, row0 + i, head, q, codes[warp]);
-    } else {
-      read_row<T>(a, row0 + i, head, q);
+    for (int h = h0; h < h1; ++h) {
+      if constexpr (WRITE) {
+        if (q.slot >= 0) write_row<T>(a, row0 + i, h, q, codes[warp]);
+      } else {
+        read_row<T>(a, row0 + i, h, q);
+      }
     }
   }
 }
@@ -429,10 +478,17 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
   auto aligned = [&](const mc_rows* r) {  // for the 16-byte accesses of eight elements
     return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
   };
-  const RowArgs a{kv->c, rows_of(k), rows_of(v), n_rows, n_seg, start, sess, pos0, lens, aligned(k) && aligned(v)};
   // Groups of slots pay once a segment has rows to fill them: GROUPS_RULE
   const bool groups = start && n_rows >= 4ll * n_seg;
-  const long long warps = (groups ? n_rows / 4 + 2ll * n_seg : (long long)n_rows) * kv->c.heads;
+  long long warps = (long long)n_rows * kv->c.heads;
+  int warp_heads = 1;
+  if (groups) {
+    // heads a warp goes through with one group's addresses: as many as leave every SM its 32 warps twice
+    const long long n = n_rows / 4 + 2ll * n_seg;
+    while (2 * warp_heads <= kv->c.heads && warp_heads < (write ? 2 : 4) && n * kv->c.heads / (2 * warp_heads) >= 128ll * kv->n_sm) warp_heads *= 2;
+    warps = n * ((kv->c.heads + warp_heads - 1) / warp_heads);
+  }
+  const RowArgs a{kv->c, rows_of(k), rows_of(v), n_rows, n_seg, start, sess, pos0, lens, aligned(k) && aligned(v), warp_heads};
   const long long blocks = (warps + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
   if (blocks > INT_MAX) return set_error(kInvalidArgument, std::string(name) + ": too many rows");
   auto f = groups ? row_variant<true>(dtype, write) : row_variant<false>(dtype, write);

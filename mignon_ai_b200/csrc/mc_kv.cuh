@@ -125,6 +125,37 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2_down(float2 a, float b) {  // rounded down
+  float2 d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tadd.rm.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b));
+  return d;
+}
+
 // The quantiser of one row x of one head, from its extremes:
 //   center = bf16(hi / 2 + lo / 2), half = max(hi - center, center - lo),
 //   scale  = half / (15 or 127), rounded up to bfloat16 so that the codes reach both extremes
@@ -183,6 +214,39 @@ __device__ __forceinline__ uint32_t code_bits(const Quant& q, float x, int bits)
 // A word of nibbles c (two's complement) as bytes 16c + 8 = 8m: the low and the high nibbles.
 __device__ __forceinline__ uint32_t low_codes(uint32_t w) { return ((w << 4) & 0xF0F0F0F0u) | 0x08080808u; }
 __device__ __forceinline__ uint32_t high_codes(uint32_t w) { return (w & 0xF0F0F0F0u) | 0x08080808u; }
+
+// Eight codes at once (as code_bits).
+template <int BITS>
+__device__ __forceinline__ void code_bits8(const Quant& q, const float (&x)[8], uint32_t (&code)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2 d = add2(make_float2(x[e], x[e + 1]), make_float2(-q.center, -q.center));
+    const float2 t = mul2(d, q.inv);
+    if constexpr (BITS == 4) {
+      const float2 y = add2_down(t, 25165824.0f);
+      code[e] = __float_as_uint(y.x);
+      code[e + 1] = __float_as_uint(y.y);
+    } else {  // one by one: a packed product and sum, both to nearest, came out fused, rounded once
+      code[e] = __float_as_uint(__fadd_rn(t.x, 12582912.0f));
+      code[e + 1] = __float_as_uint(__fadd_rn(t.y, 12582912.0f));
+    }
+  }
+}
+
+// The last i of [0, n) for which `at_most` holds, by a whole warp with 32 probes a round (0 if it
+// holds nowhere; it must not hold again after it failed).
+template <class F>
+__device__ __forceinline__ int last_at_most(int n, F at_most) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const bool below = at < hi && (lane == 0 || at_most(at));
+    lo += (31 - __clz(__ballot_sync(~0u, below))) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
 
 }  // namespace kv
 }  // namespace mc

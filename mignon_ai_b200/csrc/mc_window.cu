@@ -66,7 +66,9 @@ static int tile_launch(const Args& a, cudaStream_t stream) {
   const long long tiles = a.n_q / (kTileRows / a.group) + (long long)a.n_seg;
   if (tiles > INT_MAX || a.heads > 65535) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows or heads");
   auto aligned = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.row % 4 == 0 && r.head % 4 == 0; };
-  const TileArgs args{a, std::is_same<T, float>::value && a.dim % 4 == 0 && aligned(a.k) && aligned(a.v)};
+  auto paired = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.p) % (2 * sizeof(T)) == 0 && r.row % 2 == 0 && r.head % 2 == 0; };
+  const TileArgs args{a, std::is_same<T, float>::value && a.dim % 4 == 0 && aligned(a.k) && aligned(a.v),
+                      a.dim % 2 == 0 && paired(a.q) && paired(a.out)};
   f<<<dim3((unsigned)tiles, a.heads), kTileThreads, smem, stream>>>(args);
   MC_CUDA(cudaGetLastError());
   return kOk;

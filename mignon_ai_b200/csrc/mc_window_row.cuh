@@ -110,15 +110,9 @@ __device__ __forceinline__ Segment segment(const Args& a, int b) {
 }
 
 // The tiled kernels hand out tiles of tt tokens so that segment b's begin at start[b] / tt + b: each
-// segment has room for all of its own, and a tile finds its segment by bisection.
+// segment has room for all of its own, and a tile finds its segment by a search (by whole warps).
 __device__ __forceinline__ int tile_segment(const int* start, int n, int tt, int tile) {
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] / tt + mid <= tile) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+  return kv::last_at_most(n, [&](int i) { return start[i] / tt + i <= tile; });
 }
 
 }  // namespace win

@@ -27,7 +27,7 @@ constexpr int kTileKeys = 64;
 constexpr int kTileMaxDim = 128;
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -37,23 +37,46 @@ __device__ __forceinline__ void cut(float x, uint32_t& hi, uint32_t& lo) {
   lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
 }
 
-// d += a x b with a's and b's parts (PRODUCTS 1: the high parts alone)
+// d[j] += a x b[j] for four independent sums, product by product, so that no MMA waits for the one
+// before it; with a's and b's parts (PRODUCTS 1: the high parts alone)
 template <int PRODUCTS>
-__device__ __forceinline__ void mma_cut(float (&d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
-  uint32_t bh0, bl0, bh1, bl1;
-  cut(b0, bh0, bl0);
-  cut(b1, bh1, bl1);
+__device__ __forceinline__ void mma_cut(float (*d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const float (&b)[4][2]) {
+  uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) cut(b[j][e], bh[j][e], bl[j][e]);
   if constexpr (PRODUCTS == 3) {
-    mma_tf32(d, al, bh0, bh1);
-    mma_tf32(d, ah, bl0, bl1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mma_tf32(d[j], al, bh[j][0], bh[j][1]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mma_tf32(d[j], ah, bl[j][0], bl[j][1]);
   }
-  mma_tf32(d, ah, bh0, bh1);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) mma_tf32(d[j], ah, bh[j][0], bh[j][1]);
 }
 
 struct TileArgs {
   Args a;
-  int vec;  // float32 rows of keys and values, 16-byte aligned, of a multiple of 4 dimensions
+  int vec;    // float32 rows of keys and values, 16-byte aligned, of a multiple of 4 dimensions
+  int pairs;  // rows of queries and outputs take accesses of two elements
 };
+
+template <class T>
+__device__ __forceinline__ float2 load_pair(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float2*>(p);
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    const T* e = reinterpret_cast<const T*>(&w);
+    return make_float2(to_float<T>(e[0]), to_float<T>(e[1]));
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_pair(T* p, float x, float y) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
+  else *reinterpret_cast<uint32_t*>(p) = pack16<T>(x, y);
+}
 
 __device__ __forceinline__ void copy16_async(float* dst, const float* src, bool in) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
@@ -92,6 +115,7 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
   constexpr int PRODUCTS = std::is_same<T, float>::value ? 3 : 1;
   constexpr int KD = DIMP / 8;                   // MMA steps along the dimensions
   constexpr int NK = kTileKeys / 8;              // 8-key columns of a tile
+  constexpr int DV = (DIMP / 8 + 3) / 4 * 4;     // 8-dimension columns of the output, in fours
   constexpr int SK = DIMP + 8, SV = DIMP + 4;    // row strides of the staged keys and values
   extern __shared__ float sm[];
   float* sk = sm;
@@ -131,19 +155,26 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
   // ---- the queries' parts: step s, thread (r, c): dimensions 8s + 2c (a0, a1) and 8s + 2c + 1 (a2, a3)
   float q[KD][4];
 #pragma unroll
-  for (int s = 0; s < KD; ++s)
+  for (int e = 0; e < 2; ++e) {
+    const T* p = static_cast<const T*>(a.q.p) + row[e] * a.q.row + head[e] * a.q.head;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int d = 8 * s + 2 * c + u;
-        float x = 0.f;
-        if (real[e] && d < a.dim) x = to_float<T>(static_cast<const T*>(a.q.p)[row[e] * a.q.row + head[e] * a.q.head + d]);
-        q[s][2 * u + e] = PRODUCTS == 3 ? __fmul_rn(x, a.scale) : x;  // 16-bit values stay exact in tf32
+    for (int s = 0; s < KD; ++s) {
+      const int d = 8 * s + 2 * c;
+      float2 x = make_float2(0.f, 0.f);
+      if (real[e] && args.pairs) {
+        if (d < a.dim) x = load_pair<T>(p + d);
+      } else if (real[e]) {
+        if (d < a.dim) x.x = to_float<T>(p[d]);
+        if (d + 1 < a.dim) x.y = to_float<T>(p[d + 1]);
       }
-  float o[DIMP / 8][4];
+      // 16-bit values stay exact in tf32: their scores are scaled instead
+      q[s][e] = PRODUCTS == 3 ? __fmul_rn(x.x, a.scale) : x.x;
+      q[s][2 + e] = PRODUCTS == 3 ? __fmul_rn(x.y, a.scale) : x.y;
+    }
+  }
+  float o[DV][4];
 #pragma unroll
-  for (int i = 0; i < DIMP / 8; ++i)
+  for (int i = 0; i < DV; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f};
@@ -177,10 +208,13 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) cut(q[k][e], ah[e], al[e]);
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        if (n < n_begin || n >= n_end) continue;
-        const float2 x = *reinterpret_cast<const float2*>(&sk[(8 * n + r) * SK + 8 * k + 2 * c]);
-        mma_cut<PRODUCTS>(s[n], ah, al, x.x, x.y);
+      for (int n = 0; n < NK; n += 4) {
+        if (n + 4 <= n_begin || n >= n_end) continue;
+        float x[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float2*>(x[j]) = *reinterpret_cast<const float2*>(&sk[(8 * (n + j) + r) * SK + 8 * k + 2 * c]);
+        mma_cut<PRODUCTS>(s + n, ah, al, x);
       }
     }
     __syncthreads();
@@ -233,9 +267,15 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
       cut(s[n][1], ph[2], pl[2]);
       cut(s[n][3], ph[3], pl[3]);
 #pragma unroll
-      for (int d = 0; d < DIMP / 8; ++d) {
-        const float* x = &sv[(8 * n + 2 * c) * SV + 8 * d + r];
-        mma_cut<PRODUCTS>(o[d], ph, pl, x[0], x[SV]);
+      for (int d = 0; d < DV; d += 4) {
+        float x[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float* v = &sv[(8 * n + 2 * c) * SV + 8 * (d + j) + r];
+          x[j][0] = d + j < DIMP / 8 ? v[0] : 0.f;
+          x[j][1] = d + j < DIMP / 8 ? v[SV] : 0.f;
+        }
+        mma_cut<PRODUCTS>(o + d, ph, pl, x);
       }
     }
     __syncthreads();
@@ -252,13 +292,17 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
     float bad = __fmul_rn(sum, 0.f);
     T* out = static_cast<T*>(a.out.p) + row[e] * a.out.row + head[e] * a.out.head;
 #pragma unroll
-    for (int d = 0; d < DIMP / 8; ++d)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float x = __fmul_rn(o[d][2 * e + u], inv);
-        bad = __fmaf_rn(x, 0.f, bad);  // NaN once a value is not finite
-        if (real[e] && 8 * d + 2 * c + u < a.dim) out[8 * d + 2 * c + u] = from_float<T>(x);
+    for (int d = 0; d < DIMP / 8; ++d) {
+      const float x = __fmul_rn(o[d][2 * e], inv), y = __fmul_rn(o[d][2 * e + 1], inv);
+      const int at = 8 * d + 2 * c;
+      bad = __fmaf_rn(x, 0.f, __fmaf_rn(y, 0.f, bad));  // NaN once a value is not finite
+      if (real[e] && args.pairs) {
+        if (at < a.dim) store_pair<T>(out + at, x, y);
+      } else if (real[e]) {
+        if (at < a.dim) out[at] = from_float<T>(x);
+        if (at + 1 < a.dim) out[at + 1] = from_float<T>(y);
       }
+    }
     again[e] = __ballot_sync(~0u, real[e] && !(bad == 0.f));
   }
   // a non-finite row may have met a hidden key's infinity or NaN times its weight of zero: key by key
