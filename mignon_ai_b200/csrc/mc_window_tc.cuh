@@ -3,7 +3,7 @@
 // A CTA takes 128 rows: TT = floor(128 / group) tokens times the group's query heads, which share
 // their keys and values, and walks the 128-key tiles that any of the rows sees. Per tile
 //   S = Q K^T      tcgen05 128 x 128 x dim, operands by TMA in the 128-byte swizzle, S in TMEM
-//   P = exp2(S - m) a thread owns a row (a TMEM lane): no exchange between threads
+//   P = exp2(S - m) two threads own a row (a TMEM lane), 64 keys each; they exchange their maxima
 //   O += P V       P from TMEM (over S's columns, 16-bit pairs), V as it lies in memory (MN-major)
 // The running maximum m is only raised when a row's tile maximum exceeds it by more than 8 (in
 // log2): until then the weights are at most 2^8 and nothing has to be rescaled; a raise rescales
@@ -23,8 +23,9 @@
 namespace mc {
 namespace win {
 
-constexpr int kTcThreads = 192;          // 4 softmax warps, 1 TMA warp, 1 MMA warp
+constexpr int kTcThreads = 320;          // 8 softmax warps, 1 TMA warp, 1 MMA warp
 constexpr int kTcKeys = 128;             // keys per tile
+constexpr int kTcMaxDim = 128;
 constexpr int kTcBlock = 128 * 128;      // 128 rows x 64 16-bit values
 constexpr uint32_t kTcCols = 256;        // TMEM: S (P over it) | O
 
@@ -56,7 +57,8 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[8];
   __shared__ uint32_t tmem_slot;
-  __shared__ float redo[4][kMaxDim];
+  __shared__ float redo[4][kTcMaxDim];
+  __shared__ float exchange[2][2][128];  // [tile parity][half][row]
   const Args& a = args.a;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -86,21 +88,22 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     mbar_init(k_full, 1);
     mbar_init(v_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(p_full, 128);
+    mbar_init(p_full, 256);
     mbar_init(o_full, 1);
     mbar_init(v_free, 1);
     fence_barrier_init();
   }
-  if (warp == 5) tmem_alloc(&tmem_slot, kTcCols);
+  if (warp == 9) tmem_alloc(&tmem_slot, kTcCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const uint32_t t_s = tmem, t_o = tmem + 128;
   // rows [first, first + tokens) x group of the segment; the row of a thread
-  const int row_token = threadIdx.x / a.group, row_head = threadIdx.x % a.group;
+  const int my_row = threadIdx.x & 127, half = threadIdx.x >> 7;
+  const int row_token = my_row / a.group, row_head = my_row - row_token * a.group;
 
-  if (warp == 4) {
+  if (warp == 8) {
     if (lane == 0 && n_tiles > 0) {
       bool ok = true;
       mbar_arrive_expect_tx(q_full, (uint32_t)(blocks * tt * a.group * 128));
@@ -126,7 +129,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
         if (loads > 1) mbar_wait(v_full, (loads - 2) & 1, kErrWaitFull);
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     if (lane == 0 && n_tiles > 0) {
       constexpr bool kBf = sizeof(T) == 2 && !std::is_same<T, __half>::value;
       const uint32_t id_s = idesc_f16(128, kTcKeys, kBf, false), id_o = idesc_f16(128, dim, kBf, true);
@@ -161,44 +164,47 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     const int pos = pos0 + row_token;  // of this thread's row
     const bool real = row_token < tokens;
     const int lo = a.window > 0 ? pos - a.window + 1 : 0;
-    const uint32_t lane_off = (uint32_t)(32 * warp) << 16;
-    float top = -INFINITY, total = 0.f;
+    const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
+    const int c0 = 64 * half;  // this thread's keys of a tile
+    auto meet = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };  // the softmax warps
+    float top = -INFINITY;
+    float2 total = make_float2(0.f, 0.f);
+    const float2 scale2 = make_float2(a.scale, a.scale);
     bool ok = true;
     for (int i = 0; i < n_tiles; ++i) {
-      const int key = tile_key(i);
+      const int key = tile_key(i) + c0;
       ok = __all_sync(~0u, mbar_wait_or_abort(s_full, i & 1, kErrWaitAcc));
-      if (!ok) break;
-      tc_fence_after();
-      // visible: key + c in [lo, pos] or below the sinks (which never lie past pos)
-      const int c_lo = lo - key, c_hi = pos - key, c_sink = min(a.sinks, pos + 1) - key;
-      const bool whole = __all_sync(~0u, c_hi >= kTcKeys - 1 && (c_lo <= 0 || c_sink >= kTcKeys));
-      // S is read twice, 64 columns at a time: for the maximum, then for the weights
-      float s[64];
-      auto load = [&](int c0) {
+      float s[64], m = -INFINITY;
+      if (ok) {
+        tc_fence_after();
         tmem_ld32(t_s + lane_off + c0, *reinterpret_cast<uint32_t(*)[32]>(s));
         tmem_ld32(t_s + lane_off + c0 + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
         tmem_wait_ld();
-        if (!whole) {
+        // visible: key + c in [lo, pos] or below the sinks (which never lie past pos)
+        const int c_lo = lo - key, c_hi = pos - key, c_sink = min(a.sinks, pos + 1) - key;
+        if (!__all_sync(~0u, c_hi >= 63 && (c_lo <= 0 || c_sink >= 64))) {
 #pragma unroll
           for (int c = 0; c < 64; ++c)
-            if (!((c0 + c >= c_lo && c0 + c <= c_hi) || c0 + c < c_sink)) s[c] = -INFINITY;
+            if (!((c >= c_lo && c <= c_hi) || c < c_sink)) s[c] = -INFINITY;
         }
-      };
-      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c0 = 0; c0 < kTcKeys; c0 += 64) {
-        load(c0);
+        for (int c = 0; c < 64; c += 8)
 #pragma unroll
-        for (int c = 0; c < 64; ++c) m4[c & 3] = fmaxf(m4[c & 3], s[c]);
+          for (int e = 0; e < 4; ++e) m4[e] = kv::max3(m4[e], s[c + 2 * e], s[c + 2 * e + 1]);
+        m = __fmul_rn(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), a.scale);
+        exchange[i & 1][half][my_row] = m;
       }
-      const float m = __fmul_rn(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), a.scale);
-      if (__any_sync(~0u, m > top + 8.f || (top == -INFINITY && m > top))) {
+      meet();  // every softmax warp takes every tile's turn, also after a wait that gave up
+      // the two threads of a row, and so the warps that have the same rows, decide alike
+      m = fmaxf(m, exchange[i & 1][1 - half][my_row]);
+      if (ok && __any_sync(~0u, m > top + 8.f || (top == -INFINITY && m > top))) {
         const float raised = fmaxf(top, m);
         const float keep = top == -INFINITY ? 0.f : exp2f(__fsub_rn(top, raised));
-        total = __fmul_rn(total, keep);
+        total = kv::mul2(total, keep);
         top = raised;
         if (i > 0) {
-          for (int c = 0; c < dim; c += 16) {
+          for (int c = 16 * half; c < dim; c += 32) {
             uint32_t x[16];
             tmem_ld16(t_o + lane_off + c, x);
             tmem_wait_ld();
@@ -208,40 +214,40 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
           }
         }
       }
-      const float shift = top == -INFINITY ? 0.f : top;
-      float sum[2] = {0.f, 0.f};
-#pragma unroll
-      for (int c0 = 0; c0 < kTcKeys; c0 += 64) {
-        load(c0);
+      if (ok) {
+        const float shift = top == -INFINITY ? 0.f : top;
+        const float2 shift2 = make_float2(-shift, -shift);
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = kv::exp2_fast(__fmaf_rn(s[c + 2 * e], a.scale, -shift));
-            const float p1 = kv::exp2_fast(__fmaf_rn(s[c + 2 * e + 1], a.scale, -shift));
-            sum[0] = __fadd_rn(sum[0], p0);
-            sum[1] = __fadd_rn(sum[1], p1);
-            p[e] = pack16<T>(p0, p1);
+            const float2 x = kv::fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2);
+            const float2 y = make_float2(kv::exp2_fast(x.x), kv::exp2_fast(x.y));
+            total = kv::add2(total, y);
+            p[e] = pack16<T>(y.x, y.y);
           }
-          // columns (c0 + c) / 2.. of P lie over scores that have been read for the last time
+          // P's columns lie over scores that both threads of the row have read: they have met since
           tmem_st16(t_s + lane_off + (c0 + c) / 2, p);
         }
+        tmem_wait_st();
+        tc_fence_before();
       }
-      total = __fadd_rn(total, __fadd_rn(sum[0], sum[1]));
-      tmem_wait_st();
-      tc_fence_before();
       mbar_arrive(p_full);
     }
-    // ---- the output row
-    if (ok && n_tiles > 0) ok = __all_sync(~0u, mbar_wait_or_abort(o_full, 0, kErrWaitAcc));
+    // ---- the output row: each thread every other 16 dimensions of it
+    if (n_tiles > 0) ok = __all_sync(~0u, ok && mbar_wait_or_abort(o_full, 0, kErrWaitAcc));
+    meet();
+    exchange[0][half][my_row] = __fadd_rn(total.x, total.y);
+    meet();
+    const float sum = __fadd_rn(exchange[0][0][my_row], exchange[0][1][my_row]);
+    float bad = 0.f;
     if (ok) {
       tc_fence_after();
-      const float inv = total == 0.f ? 0.f : __fdiv_rn(1.0f, total);
+      const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum);
       const int row = seg.q0 + first + row_token, h = hk * a.group + row_head;
       T* out = static_cast<T*>(a.out.p) + row * a.out.row + h * a.out.head;
-      float bad = 0.f;
-      for (int c = 0; c < dim; c += 16) {
+      for (int c = 16 * half; c < dim; c += 32) {
         uint32_t x[16];
         if (n_tiles > 0) {
           tmem_ld16(t_o + lane_off + c, x);
@@ -267,8 +273,12 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
           }
         }
       }
-      bad = __fmaf_rn(total, 0.f, bad);
-      uint32_t again = __ballot_sync(~0u, real && !(bad == 0.f));
+      bad = __fmaf_rn(sum, 0.f, bad);
+    }
+    exchange[1][half][my_row] = bad;
+    meet();  // also orders the row's stores before those of a second computation
+    if (ok && half == 0) {
+      uint32_t again = __ballot_sync(~0u, real && !(exchange[1][0][my_row] == 0.f && exchange[1][1][my_row] == 0.f));
       while (again) {
         const int l = __ffs(again) - 1, r = 32 * warp + l;
         again &= again - 1;
@@ -280,7 +290,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, kTcCols);
+  if (warp == 9) tmem_dealloc(tmem, kTcCols);
 }
 
 }  // namespace win

@@ -6,9 +6,10 @@
 // than tf32's bits before a 16-bit output: one product.
 //
 // A CTA of four warps takes 64 rows (tokens x the query heads that share a key/value head), a warp
-// 16 of them; keys and values of 64 positions at a time are staged as float32 in shared memory,
-// the next keys in flight behind the softmax and the value product, the next values behind the
-// score product (cp.async where rows are 16-byte aligned float32). Scores stay in
+// 16 of them, for one or more key/value heads one after the other. Queries, and keys and values of 64
+// positions at a time, are staged as float32 in shared memory: the next keys (and the next head's
+// queries) in flight behind the softmax and the value product, the next values behind the score
+// product (cp.async where rows are 16-byte aligned float32). Scores stay in
 // registers: the layout in which an MMA leaves them is the one its A operand wants if the k order
 // of the value product is taken as (2c, 2c + 1) for a thread's (c, c + 4). Row strides of dim + 8 and
 // dim + 4 floats keep the operands' shared loads free of bank conflicts.
@@ -59,19 +60,11 @@ __device__ __forceinline__ void mma_cut(float (*d)[4], const uint32_t (&ah)[4], 
 struct TileArgs {
   Args a;
   int vec;    // float32 rows of keys and values, 16-byte aligned, of a multiple of 4 dimensions
-  int pairs;  // rows of queries and outputs take accesses of two elements
+  int qvec;   // and of queries
+  int pairs;  // rows of outputs take accesses of two elements
+  int heads;  // key/value heads that a CTA takes one after the other
 };
 
-template <class T>
-__device__ __forceinline__ float2 load_pair(const T* p) {
-  if constexpr (sizeof(T) == 4) {
-    return *reinterpret_cast<const float2*>(p);
-  } else {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-    const T* e = reinterpret_cast<const T*>(&w);
-    return make_float2(to_float<T>(e[0]), to_float<T>(e[1]));
-  }
-}
 template <class T>
 __device__ __forceinline__ void store_pair(T* p, float x, float y) {
   if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
@@ -85,16 +78,19 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Rows [0, count) of 64 staged with stride S, zeros past count and past the head's width.
+// Rows [0, count) of 64 staged with stride S, zeros past count and past the head's width. Row j is token
+// j / group, head j % group of it.
 template <class T, int DIMP, int S>
-__device__ __forceinline__ void stage(float* dst, const T* src, long long stride, int count, int dim, bool vec) {
+__device__ __forceinline__ void stage(float* dst, const T* src, long long row, long long head, unsigned group, int count, int dim,
+                                      bool vec) {
+  auto offset = [&](unsigned j) { return group == 1 ? j * row : (j / group) * row + (j % group) * head; };
   if constexpr (std::is_same<T, float>::value) {
     if (vec) {
 #pragma unroll 4
       for (int e = threadIdx.x; e < kTileKeys * DIMP / 4; e += kTileThreads) {
         const int j = e / (DIMP / 4), d = 4 * (e % (DIMP / 4));
         const bool in = j < count && d < dim;
-        copy16_async(dst + j * S + d, src + (in ? j * stride + d : 0), in);
+        copy16_async(dst + j * S + d, src + (in ? offset(j) + d : 0), in);
       }
       return;
     }
@@ -102,15 +98,16 @@ __device__ __forceinline__ void stage(float* dst, const T* src, long long stride
 #pragma unroll 4
   for (int e = threadIdx.x; e < kTileKeys * DIMP; e += kTileThreads) {
     const int j = e / DIMP, d = e % DIMP;
-    dst[j * S + d] = j < count && d < dim ? to_float<T>(src[j * stride + d]) : 0.f;
+    dst[j * S + d] = j < count && d < dim ? to_float<T>(src[offset(j) + d]) : 0.f;
   }
 }
 
-inline size_t tile_smem(int dimp) { return (size_t)kTileKeys * (2 * dimp + 12) * sizeof(float) + 4 * kMaxDim * sizeof(float); }
+// queries and keys (stride dimp + 8), values (dimp + 4)
+inline size_t tile_smem(int dimp) { return (size_t)kTileKeys * (3 * dimp + 20) * sizeof(float); }
 
 // DIMP: the head width rounded up to 16, 32, 64, 96 or 128 (dimensions past the width are zeros).
 template <class T, int DIMP>
-__global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(const __grid_constant__ TileArgs args) {
+__global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(const __grid_constant__ TileArgs args) {
   const Args& a = args.a;
   constexpr int PRODUCTS = std::is_same<T, float>::value ? 3 : 1;
   constexpr int KD = DIMP / 8;                   // MMA steps along the dimensions
@@ -118,12 +115,14 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
   constexpr int DV = (DIMP / 8 + 3) / 4 * 4;     // 8-dimension columns of the output, in fours
   constexpr int SK = DIMP + 8, SV = DIMP + 4;    // row strides of the staged keys and values
   extern __shared__ float sm[];
-  float* sk = sm;
+  __shared__ float redo[kTileThreads / 32][kTileMaxDim];
+  float* sq = sm;
+  float* sk = sq + kTileRows * SK;
   float* sv = sk + kTileKeys * SK;
-  float* redo = sv + kTileKeys * SV;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 
-  const int tt = kTileRows / a.group, tile_id = gridDim.x - 1 - blockIdx.x, hk = blockIdx.y;
+  const int tt = kTileRows / a.group, tile_id = gridDim.x - 1 - blockIdx.x;
+  const int h0 = blockIdx.y * args.heads, n_heads = min(args.heads, a.heads - h0);
   const int b = a.q_start ? tile_segment(a.q_start, a.n_seg, tt, tile_id) : 0;
   const Segment seg = segment(a, b);
   const int first = (tile_id - (a.q_start ? a.q_start[b] / tt + b : 0)) * tt;  // first token in the segment
@@ -141,7 +140,7 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
     pos[e] = real[e] ? base + token : -1;
     lo[e] = a.window > 0 ? max(0, pos[e] - a.window + 1) : 0;
     row[e] = seg.q0 + first + token;
-    head[e] = hk * a.group + i % a.group;
+    head[e] = i - token * a.group;  // among those that share a key/value head
   }
   // positions of the CTA's and of the warp's first and last real rows
   const int last_token = min(tokens - 1, (16 * warp + 15) / a.group), first_token = 16 * warp / a.group;
@@ -152,47 +151,37 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
   const int sink_tiles = cta_hi < 0 ? 0 : min(win_tile, (min(a.sinks, cta_lo) + kTileKeys - 1) / kTileKeys);
   const int n_tiles = cta_hi < 0 ? 0 : sink_tiles + cta_hi / kTileKeys - win_tile + 1;
 
-  // ---- the queries' parts: step s, thread (r, c): dimensions 8s + 2c (a0, a1) and 8s + 2c + 1 (a2, a3)
-  float q[KD][4];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const T* p = static_cast<const T*>(a.q.p) + row[e] * a.q.row + head[e] * a.q.head;
-#pragma unroll
-    for (int s = 0; s < KD; ++s) {
-      const int d = 8 * s + 2 * c;
-      float2 x = make_float2(0.f, 0.f);
-      if (real[e] && args.pairs) {
-        if (d < a.dim) x = load_pair<T>(p + d);
-      } else if (real[e]) {
-        if (d < a.dim) x.x = to_float<T>(p[d]);
-        if (d + 1 < a.dim) x.y = to_float<T>(p[d + 1]);
+  auto tile_key = [&](int i) { return (i < sink_tiles ? i : win_tile + i - sink_tiles) * kTileKeys; };
+  // steps: the tiles of head h0, then those of the next. Keys past cta_hi are seen by no row and stay zero.
+  const int steps = n_heads * n_tiles;
+  auto load = [&](int step, bool values) {
+    if (step < steps) {
+      const int hk = h0 + (n_heads == 1 ? 0 : step / n_tiles), i = step - (hk - h0) * n_tiles;
+      const int key = tile_key(i), count = min(kTileKeys, cta_hi + 1 - key);
+      if (values) {
+        stage<T, DIMP, SV>(sv, static_cast<const T*>(a.v.p) + (seg.k0 + key) * a.v.row + hk * a.v.head, a.v.row, 0, 1, count, a.dim,
+                           args.vec);
+      } else {
+        if (i == 0)
+          stage<T, DIMP, SK>(sq, static_cast<const T*>(a.q.p) + (seg.q0 + first) * a.q.row + (long long)hk * a.group * a.q.head,
+                             a.q.row, a.q.head, a.group, tokens * a.group, a.dim, args.qvec);
+        stage<T, DIMP, SK>(sk, static_cast<const T*>(a.k.p) + (seg.k0 + key) * a.k.row + hk * a.k.head, a.k.row, 0, 1, count, a.dim,
+                           args.vec);
       }
-      // 16-bit values stay exact in tf32: their scores are scaled instead
-      q[s][e] = PRODUCTS == 3 ? __fmul_rn(x.x, a.scale) : x.x;
-      q[s][2 + e] = PRODUCTS == 3 ? __fmul_rn(x.y, a.scale) : x.y;
     }
-  }
+    copies_commit();
+  };
+  load(0, false);
+  load(0, true);
+  int step = 0;
+  for (int hk = h0; hk < h0 + n_heads; ++hk) {
   float o[DV][4];
 #pragma unroll
   for (int i = 0; i < DV; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
   float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f};
-
-  const T* kbase = static_cast<const T*>(a.k.p) + seg.k0 * a.k.row + hk * a.k.head;
-  const T* vbase = static_cast<const T*>(a.v.p) + seg.k0 * a.v.row + hk * a.v.head;
-  auto tile_key = [&](int i) { return (i < sink_tiles ? i : win_tile + i - sink_tiles) * kTileKeys; };
-  auto load = [&](int i, bool values) {  // keys past cta_hi are seen by no row and stay zero
-    if (i < n_tiles) {
-      const int key = tile_key(i), count = min(kTileKeys, cta_hi + 1 - key);
-      if (values) stage<T, DIMP, SV>(sv, vbase + key * a.v.row, a.v.row, count, a.dim, args.vec);
-      else stage<T, DIMP, SK>(sk, kbase + key * a.k.row, a.k.row, count, a.dim, args.vec);
-    }
-    copies_commit();
-  };
-  load(0, false);
-  load(0, true);
-  for (int i = 0; i < n_tiles; ++i) {
+  for (int i = 0; i < n_tiles; ++i, ++step) {
     const int key = tile_key(i);
     // 8-key columns that some row of the warp sees
     const int n_end = w_hi < key ? 0 : min(NK, (w_hi - key) / 8 + 1);
@@ -204,9 +193,15 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
     for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < KD; ++k) {
+      // step k, thread (r, c): dimensions 8k + 2c (a0, a1) and 8k + 2c + 1 (a2, a3) of rows r and r + 8
       uint32_t ah[4], al[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) cut(q[k][e], ah[e], al[e]);
+      for (int e = 0; e < 2; ++e) {
+        const float2 q = *reinterpret_cast<const float2*>(&sq[(16 * warp + r + 8 * e) * SK + 8 * k + 2 * c]);
+        // 16-bit values stay exact in tf32: their scores are scaled instead
+        cut(PRODUCTS == 3 ? __fmul_rn(q.x, a.scale) : q.x, ah[e], al[e]);
+        cut(PRODUCTS == 3 ? __fmul_rn(q.y, a.scale) : q.y, ah[2 + e], al[2 + e]);
+      }
 #pragma unroll
       for (int n = 0; n < NK; n += 4) {
         if (n + 4 <= n_begin || n >= n_end) continue;
@@ -218,7 +213,7 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
       }
     }
     __syncthreads();
-    load(i + 1, false);
+    load(step + 1, false);
     // ---- what each row sees, its maximum, its weights. s[n][2e + u]: row e, key 8n + 2c + u
     float keep[2];
 #pragma unroll
@@ -279,7 +274,7 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
       }
     }
     __syncthreads();
-    load(i + 1, true);
+    load(step + 1, true);
   }
   // ---- the output rows: o[d][2e + u] is row e, dimension 8d + 2c + u
   uint32_t again[2];
@@ -290,7 +285,7 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
     sum = __fadd_rn(sum, __shfl_xor_sync(~0u, sum, 2));
     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum);
     float bad = __fmul_rn(sum, 0.f);
-    T* out = static_cast<T*>(a.out.p) + row[e] * a.out.row + head[e] * a.out.head;
+    T* out = static_cast<T*>(a.out.p) + row[e] * a.out.row + (long long)(hk * a.group + head[e]) * a.out.head;
 #pragma unroll
     for (int d = 0; d < DIMP / 8; ++d) {
       const float x = __fmul_rn(o[d][2 * e], inv), y = __fmul_rn(o[d][2 * e + 1], inv);
@@ -312,9 +307,9 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 3 : 2) tile_kernel(
       if (!(again[e] & (0xFu << (4 * i)))) continue;
       const int at = 16 * warp + 8 * e + i;
       __syncwarp();
-      row_attention<T>(a, seg.q0 + first + at / a.group, hk * a.group + at % a.group, seg.k0, base + at / a.group,
-                       redo + warp * kMaxDim);
+      row_attention<T>(a, seg.q0 + first + at / a.group, hk * a.group + at % a.group, seg.k0, base + at / a.group, redo[warp]);
     }
+  }
 }
 
 template <class T>
