@@ -295,8 +295,9 @@ typedef struct mc_kv mc_kv;
 int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out);
 /* Waits for the device's work and frees the cache. */
 int mc_kv_close(mc_kv* kv);
-/* Waits for the device's work; MC_INVALID_ARGUMENT if a call since the last check named a session
- * or a position out of range (such rows are skipped, attention rows written as zero). */
+/* Waits for the device's work; MC_DEVICE_TIMEOUT if a kernel of this section (window attention
+ * included) gave up a wait since the last check; MC_INVALID_ARGUMENT if a call on this cache named a
+ * session or a position out of range (such rows are skipped, attention rows written as zero). */
 int mc_kv_error(mc_kv* kv);
 
 /* Quantises rows into the cache. Segment b is rows [row_start[b], row_start[b+1]) and goes to

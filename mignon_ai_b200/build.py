@@ -4,14 +4,16 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmignoncuda.so")
+UNITS = ("libmignoncuda", "libmignoncuda_kv")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-         "-Xcompiler", "-fPIC", "-shared", "--expt-relaxed-constexpr", "-Xptxas", "-v",
+         "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas", "-v",
          "-ccbin", "/usr/bin/g++"]
 
 
@@ -30,14 +32,23 @@ def needs_build() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
-    cmd = [NVCC, *FLAGS, "-o", LIB, os.path.join(CSRC, "libmignoncuda.cu")]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-    if r.returncode != 0:
+    # the translation units side by side, then one link
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, u + ".o") for u in UNITS]
+        jobs = [subprocess.Popen([NVCC, *FLAGS, "-c", "-o", o, os.path.join(CSRC, u + ".cu")], stdout=subprocess.PIPE,
+                                 stderr=subprocess.STDOUT, text=True) for u, o in zip(UNITS, objs)]
+        outs = [j.communicate()[0] for j in jobs]
+        failed = any(j.returncode for j in jobs)
+        if not failed:
+            r = subprocess.run([NVCC, *FLAGS, "-shared", "-o", LIB, *objs], capture_output=True, text=True)
+            outs.append(r.stdout + r.stderr)
+            failed = r.returncode != 0
+    if verbose or failed:
+        sys.stderr.write("".join(outs))
+    if failed:
         raise RuntimeError("nvcc failed building libmignoncuda.so")
     with open(os.path.join(HERE, "ptxas_info.txt"), "w") as f:
-        f.write(r.stderr)
+        f.write("".join(outs))
     return LIB
 
 

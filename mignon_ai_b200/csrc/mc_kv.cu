@@ -579,9 +579,13 @@ extern "C" int mc_kv_error(mc_kv* kv) {
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
   MC_CUDA(cudaDeviceSynchronize());
-  const int st = check_device_error(0);
-  if (st != kOk) return st;
   int code = 0;
+  MC_CUDA(cudaMemcpyFromSymbol(&code, g_device_error, sizeof(int)));
+  if (code) {
+    const int zero = 0;
+    MC_CUDA(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)));
+    return set_error(kDeviceTimeout, "device wait gave up (code " + std::to_string(code) + "); the kernel returned without finishing its work");
+  }
   MC_CUDA(cudaMemcpy(&code, kv->c.error, sizeof(int), cudaMemcpyDeviceToHost));
   if (!code) return kOk;
   MC_CUDA(cudaMemset(kv->c.error, 0, sizeof(int)));

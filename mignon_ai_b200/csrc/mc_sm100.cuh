@@ -12,9 +12,10 @@
 
 namespace mc {
 
-// Error word written by device code (0 = ok). Read and cleared by the host after each call. The
-// library is one translation unit, so this is its only definition.
-__device__ int g_device_error = 0;
+// Error word written by device code (0 = ok). Read and cleared by the host after each call. Each of
+// the library's translation units has one of its own: the engine's, and that of the key/value cache
+// and window attention.
+static __device__ int g_device_error = 0;
 
 enum DeviceError : int {
   kErrNone = 0,

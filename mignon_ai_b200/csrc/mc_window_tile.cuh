@@ -2,7 +2,9 @@
 //
 // A float32 operand x is cut into hi = x with the low 13 bits cleared (tf32, 11 significant bits)
 // and lo = x - hi (exact); a product is hi*hi + hi*lo + lo*hi, whose error, about 2^-22 of
-// |a||b|, is float32's own size. 16-bit operands are exact in tf32 and their weights need no more
+// |a||b|, is float32's own size. The tensor unit does not round its sums to nearest: summed over a row of
+// 8192 keys that alone came to 1.3e-5 of the result. So the two small products have a sum of their own,
+// each tile's value sums start from zero, and what they are added up in is float32. 16-bit operands are exact in tf32 and their weights need no more
 // than tf32's bits before a 16-bit output: one product.
 //
 // A CTA of four warps takes 64 rows (tokens x the query heads that share a key/value head), a warp
@@ -37,11 +39,17 @@ __device__ __forceinline__ void cut(float x, uint32_t& hi, uint32_t& lo) {
   hi = __float_as_uint(x) & 0xFFFFE000u;
   lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
 }
+// The A operands, fewer than B's, are cut to nearest: their low parts then have either sign, and the
+// low-by-low products that are left out no longer add up.
+__device__ __forceinline__ void cut_nearest(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+  lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
+}
 
-// d[j] += a x b[j] for four independent sums, product by product, so that no MMA waits for the one
-// before it; with a's and b's parts (PRODUCTS 1: the high parts alone)
+// d[j] + small[j] += a x b[j] for four independent sums, product by product, so that no MMA waits for the
+// one before it; with a's and b's parts (PRODUCTS 1: the high parts alone)
 template <int PRODUCTS>
-__device__ __forceinline__ void mma_cut(float (*d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const float (&b)[4][2]) {
+__device__ __forceinline__ void mma_cut(float (*d)[4], float (*small)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const float (&b)[4][2]) {
   uint32_t bh[4][2], bl[4][2];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -49,9 +57,9 @@ __device__ __forceinline__ void mma_cut(float (*d)[4], const uint32_t (&ah)[4], 
     for (int e = 0; e < 2; ++e) cut(b[j][e], bh[j][e], bl[j][e]);
   if constexpr (PRODUCTS == 3) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mma_tf32(d[j], al, bh[j][0], bh[j][1]);
+    for (int j = 0; j < 4; ++j) mma_tf32(small[j], al, bh[j][0], bh[j][1]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mma_tf32(d[j], ah, bl[j][0], bl[j][1]);
+    for (int j = 0; j < 4; ++j) mma_tf32(small[j], ah, bl[j][0], bl[j][1]);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) mma_tf32(d[j], ah, bh[j][0], bh[j][1]);
@@ -192,24 +200,31 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
 #pragma unroll
     for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-    for (int k = 0; k < KD; ++k) {
-      // step k, thread (r, c): dimensions 8k + 2c (a0, a1) and 8k + 2c + 1 (a2, a3) of rows r and r + 8
-      uint32_t ah[4], al[4];
+    for (int n = 0; n < NK; n += 4) {
+      if (n + 4 <= n_begin || n >= n_end) continue;
+      float small[4][4] = {};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float2 q = *reinterpret_cast<const float2*>(&sq[(16 * warp + r + 8 * e) * SK + 8 * k + 2 * c]);
-        // 16-bit values stay exact in tf32: their scores are scaled instead
-        cut(PRODUCTS == 3 ? __fmul_rn(q.x, a.scale) : q.x, ah[e], al[e]);
-        cut(PRODUCTS == 3 ? __fmul_rn(q.y, a.scale) : q.y, ah[2 + e], al[2 + e]);
-      }
+      for (int k = 0; k < KD; ++k) {
+        // step k, thread (r, c): dimensions 8k + 2c (a0, a1) and 8k + 2c + 1 (a2, a3) of rows r and r + 8
+        uint32_t ah[4], al[4];
 #pragma unroll
-      for (int n = 0; n < NK; n += 4) {
-        if (n + 4 <= n_begin || n >= n_end) continue;
+        for (int e = 0; e < 2; ++e) {
+          const float2 q = *reinterpret_cast<const float2*>(&sq[(16 * warp + r + 8 * e) * SK + 8 * k + 2 * c]);
+          // 16-bit values stay exact in tf32: their scores are scaled instead
+          cut_nearest(PRODUCTS == 3 ? __fmul_rn(q.x, a.scale) : q.x, ah[e], al[e]);
+          cut_nearest(PRODUCTS == 3 ? __fmul_rn(q.y, a.scale) : q.y, ah[2 + e], al[2 + e]);
+        }
         float x[4][2];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           *reinterpret_cast<float2*>(x[j]) = *reinterpret_cast<const float2*>(&sk[(8 * (n + j) + r) * SK + 8 * k + 2 * c]);
-        mma_cut<PRODUCTS>(s + n, ah, al, x);
+        mma_cut<PRODUCTS>(s + n, small, ah, al, x);
+      }
+      if (PRODUCTS == 3) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n + j][e] = __fadd_rn(s[n + j][e], small[j][e]);
       }
     }
     __syncthreads();
@@ -246,23 +261,21 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
         }
       total[e] = __fmaf_rn(total[e], keep[e], sum);
     }
-#pragma unroll
-    for (int d = 0; d < DIMP / 8; ++d) {
-      o[d][0] = __fmul_rn(o[d][0], keep[0]), o[d][1] = __fmul_rn(o[d][1], keep[0]);
-      o[d][2] = __fmul_rn(o[d][2], keep[1]), o[d][3] = __fmul_rn(o[d][3], keep[1]);
-    }
     copies_wait<1>();
     __syncthreads();
+    // a tile's sums start from zero and are added to the row's in float32: the tensor unit does not round
+    // its sums to nearest, which would add up over a long row
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      if (n < n_begin || n >= n_end) continue;
-      uint32_t ph[4], pl[4];
-      cut(s[n][0], ph[0], pl[0]);
-      cut(s[n][2], ph[1], pl[1]);
-      cut(s[n][1], ph[2], pl[2]);
-      cut(s[n][3], ph[3], pl[3]);
+    for (int d = 0; d < DV; d += 4) {
+      float sum[4][4] = {}, small[4][4] = {};
 #pragma unroll
-      for (int d = 0; d < DV; d += 4) {
+      for (int n = 0; n < NK; ++n) {
+        if (n < n_begin || n >= n_end) continue;
+        uint32_t ph[4], pl[4];
+        cut_nearest(s[n][0], ph[0], pl[0]);
+        cut_nearest(s[n][2], ph[1], pl[1]);
+        cut_nearest(s[n][1], ph[2], pl[2]);
+        cut_nearest(s[n][3], ph[3], pl[3]);
         float x[4][2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -270,8 +283,12 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
           x[j][0] = d + j < DIMP / 8 ? v[0] : 0.f;
           x[j][1] = d + j < DIMP / 8 ? v[SV] : 0.f;
         }
-        mma_cut<PRODUCTS>(o + d, ph, pl, x);
+        mma_cut<PRODUCTS>(sum, small, ph, pl, x);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d + j][e] = __fmaf_rn(o[d + j][e], keep[e >> 1], PRODUCTS == 3 ? __fadd_rn(sum[j][e], small[j][e]) : sum[j][e]);
     }
     __syncthreads();
     load(step + 1, true);

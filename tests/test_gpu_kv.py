@@ -481,3 +481,17 @@ def test_refusals(kv, call):
             kv.window_attention(x, x, x, scale=float("nan"))
         else:
             cache.write(x.transpose(1, 2).contiguous().transpose(1, 2), x, ints([0, 0]))
+
+
+@pytest.mark.parametrize("dim", [32, 128])
+def test_window_float32_does_not_drift_over_long_rows(kv, dim):
+    """Rows of thousands of keys stay at float32's accuracy: within 2^-20 of the result in the 2-norm,
+    sixteen of its roundings, as sums that round to nearest stay; sums cut off at every step do not."""
+    g = gen(dim)
+    n, last = 8192, 64
+    q = torch.randn((last, 1, dim), generator=g)
+    k, v = torch.randn((n, 1, dim), generator=g), torch.randn((n, 1, dim), generator=g)
+    got = kv.window_attention(q.to(DEV), k.to(DEV), v.to(DEV), ints([0, last]), ints([0, n])).cpu().double()
+    i, j = torch.arange(last)[:, None] + n - last, torch.arange(n)[None]
+    want = ref.attention(q[:, 0], k[:, 0], v[:, 0], j <= i)
+    assert (got[:, 0] - want).norm() <= 2.0 ** -20 * want.norm()
