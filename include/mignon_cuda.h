@@ -284,16 +284,18 @@ typedef struct {
 
 typedef struct mc_kv mc_kv;
 
-/* A cache of keys and values for `sessions` sessions of one layer, in device memory that the
- * library owns. Position p of a session is held at place p while p < sinks, then in a ring of
+/* A cache of keys and values for `sessions` sessions of one layer, in `memory`: device memory of
+ * mc_kv_bytes(spec), 256-byte aligned, that the caller owns and leaves to the cache until it is
+ * closed and its work is done; NULL: the library allocates it. It is zeroed on `stream`. Position p of a session is held at place p while p < sinks, then in a ring of
  * slots - sinks places: the cache holds the first `sinks` positions and the last slots - sinks.
  * Each row of head_dim values is held as codes of `bits` bits with a scale and a center
  * (bfloat16): center + scale * m, m an odd integer in [-15, 15] (4 bits) or an integer in
  * [-127, 127] (8 bits). The center is the bfloat16 next to the middle of the row's extremes and
  * the scale is rounded up, so |x - read back| <= scale (4 bits) or scale / 2 (8 bits), plus float32
  * rounding. A row that is not all finite reads back as NaN; a masked one reaches no output. */
-int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out);
-/* Waits for the device's work and frees the cache. */
+int mc_kv_bytes(const mc_kv_spec* spec, size_t* bytes);
+int mc_kv_open(int device, const mc_kv_spec* spec, void* memory, void* stream, mc_kv** out);
+/* Closes the cache; memory of the library's is freed once the device's work is done. */
 int mc_kv_close(mc_kv* kv);
 /* Waits for the device's work; MC_DEVICE_TIMEOUT if a kernel of this section (window attention
  * included) gave up a wait since the last check; MC_INVALID_ARGUMENT if a call on this cache named a

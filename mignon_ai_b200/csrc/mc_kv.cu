@@ -35,6 +35,7 @@ struct RowArgs {
   const int *start, *sess, *pos0, *lens;
   int vec;         // rows are aligned for 16-byte accesses of eight elements
   int warp_heads;  // heads that a warp of segment_kernel takes one after the other
+  float spread;    // segments per row, on average
 };
 
 // Where a row goes or comes from: its session and slot, slot -1 for none.
@@ -361,9 +362,8 @@ template <class T, bool WRITE>
 __global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5) : 6) segment_kernel(const __grid_constant__ RowArgs a) {
   __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
-  const int parts = (a.c.heads + a.warp_heads - 1) / a.warp_heads;
-  const long long group = item / parts;
+  const unsigned item = blockIdx.x * (kCacheThreads / 32) + warp;  // fewer than 2^31
+  const unsigned parts = (unsigned)(a.c.heads + a.warp_heads - 1) / a.warp_heads, group = item / parts;
   const int h0 = (int)(item - group * parts) * a.warp_heads, h1 = min(h0 + a.warp_heads, a.c.heads);
   if constexpr (!WRITE) {  // rows before the first segment and after the last come back as zeros
     const int lo = max(0, min(a.start[0], a.n_rows)), hi = max(lo, min(a.start[a.n_seg], a.n_rows));
@@ -372,9 +372,9 @@ __global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5
       read_row<T>(a, i < lo ? i : hi + i - lo, (int)(e % a.c.heads), RowPlace{0, -1});
     }
   }
-  const int b = last_at_most(a.n_seg, [&](int i) { return (a.start[i] >> 2) + 2ll * i <= group; });
+  const int b = last_at_most(a.n_seg, [&](int i) { return (a.start[i] >> 2) + 2ll * i <= (long long)group; });
   const int first = a.start[b], rows = a.start[b + 1] - first;
-  const long long at = group - ((first >> 2) + 2ll * b);
+  const long long at = (long long)group - ((first >> 2) + 2ll * b);
   if (rows <= 0 || first < 0 || rows > a.n_rows - first || at < 0) return;
   const int offset = a.pos0[b] >= 0 ? slot_of(a.c, a.pos0[b]) & 3 : 0;  // of the segment's first row in its group
   const long long begin = max(0ll, 4 * at - offset), end = min((long long)rows, 4 * at - offset + 4);
@@ -411,14 +411,16 @@ template <class T, bool WRITE>
 __global__ void __launch_bounds__(kCacheThreads) single_kernel(const __grid_constant__ RowArgs a) {
   __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
   const int warp = threadIdx.x >> 5;
-  const long long item = (long long)blockIdx.x * (kCacheThreads / 32) + warp;
-  const int row = (int)(item / a.c.heads), head = (int)(item % a.c.heads);
+  const unsigned item = blockIdx.x * (kCacheThreads / 32) + warp;  // fewer than 2^31
+  const int row = (int)(item / a.c.heads), head = (int)(item - (unsigned)row * a.c.heads);
   if (row >= a.n_rows) return;
   RowPlace w{0, -1};
   if (!a.start) {
     w = place<WRITE>(a, row, row, 1, row);
   } else if (row >= a.start[0] && row < a.start[a.n_seg]) {
-    const int b = last_at_most(a.n_seg, [&](int i) { return a.start[i] <= row; });
+    // where an even spread has the row (decode steps), else by search
+    int b = min((int)((float)row * a.spread), a.n_seg - 1);
+    if (a.start[b] > row || a.start[b + 1] <= row) b = last_at_most(a.n_seg, [&](int i) { return a.start[i] <= row; });
     const int first = a.start[b], rows = a.start[b + 1] - first;
     if (first >= 0 && row - first < rows && rows <= a.n_rows - first) w = place<WRITE>(a, b, first, rows, row);
   }
@@ -439,6 +441,7 @@ struct mc_kv {
   int device = 0;
   mc::kv::Cache c{};
   void* mem = nullptr;       // error word, arrival counters, partial results, regions
+  bool own = false;          // whether the memory is the library's
   int* arrived = nullptr;
   float* partial = nullptr;
   int n_sm = 0;
@@ -488,9 +491,10 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
     while (2 * warp_heads <= kv->c.heads && warp_heads < (write ? 2 : 4) && n * kv->c.heads / (2 * warp_heads) >= 128ll * kv->n_sm) warp_heads *= 2;
     warps = n * ((kv->c.heads + warp_heads - 1) / warp_heads);
   }
-  const RowArgs a{kv->c, rows_of(k), rows_of(v), n_rows, n_seg, start, sess, pos0, lens, aligned(k) && aligned(v), warp_heads};
+  const RowArgs a{kv->c, rows_of(k), rows_of(v), n_rows, n_seg, start, sess, pos0, lens, aligned(k) && aligned(v), warp_heads,
+                  (float)n_seg / (float)n_rows};
   const long long blocks = (warps + kCacheThreads / 32 - 1) / (kCacheThreads / 32);
-  if (blocks > INT_MAX) return set_error(kInvalidArgument, std::string(name) + ": too many rows");
+  if (warps > INT_MAX) return set_error(kInvalidArgument, std::string(name) + ": too many rows");
   auto f = groups ? row_variant<true>(dtype, write) : row_variant<false>(dtype, write);
   f<<<(unsigned)blocks, kCacheThreads, 0, stream>>>(a);
   MC_CUDA(cudaGetLastError());
@@ -500,59 +504,86 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
 }  // namespace kv
 }  // namespace mc
 
-extern "C" int mc_kv_open(int device, const mc_kv_spec* spec, mc_kv** out) {
-  using namespace mc;
-  clear_error();
-  if (!spec || !out) return set_error(kInvalidArgument, "mc_kv_open: null argument");
-  *out = nullptr;
+namespace mc {
+namespace kv {
+
+// The cache of a spec, without its memory, and the bytes it needs: `head` of workspace, then the regions.
+static int layout(const char* name, const mc_kv_spec* spec, Cache* c, size_t* head, size_t* bytes) {
+  const std::string who = std::string(name) + ": ";
+  if (!spec) return set_error(kInvalidArgument, who + "null argument");
   const mc_kv_spec& s = *spec;
   if (s.sessions < 1 || s.heads < 1 || s.slots < 1)
-    return set_error(kInvalidArgument, "mc_kv_open: sessions, heads and slots must be positive");
-  if (s.head_dim < 16 || s.head_dim > kv::kMaxDim || s.head_dim % 16)
-    return set_error(kInvalidArgument, "mc_kv_open: head_dim must be a multiple of 16 from 16 to 128");
-  if (s.bits != 4 && s.bits != 8) return set_error(kInvalidArgument, "mc_kv_open: bits must be 4 or 8");
-  if (s.sinks < 0 || s.sinks >= s.slots) return set_error(kInvalidArgument, "mc_kv_open: sinks must be in [0, slots)");
-  if (s.slots > (1 << 30)) return set_error(kInvalidArgument, "mc_kv_open: slots above 2^30");
+    return set_error(kInvalidArgument, who + "sessions, heads and slots must be positive");
+  if (s.head_dim < 16 || s.head_dim > kMaxDim || s.head_dim % 16)
+    return set_error(kInvalidArgument, who + "head_dim must be a multiple of 16 from 16 to 128");
+  if (s.bits != 4 && s.bits != 8) return set_error(kInvalidArgument, who + "bits must be 4 or 8");
+  if (s.sinks < 0 || s.sinks >= s.slots) return set_error(kInvalidArgument, who + "sinks must be in [0, slots)");
+  if (s.slots > (1 << 30)) return set_error(kInvalidArgument, who + "slots above 2^30");
+  *c = Cache{};
+  c->sessions = s.sessions;
+  c->heads = s.heads;
+  c->dim = s.head_dim;
+  c->bits = s.bits;
+  c->slots = s.slots;
+  c->sinks = s.sinks;
+  c->ring = s.slots - s.sinks;
+  c->cap = (s.slots + 63) / 64 * 64;
+  c->cb = s.head_dim * s.bits / 8;
+  c->region = (long long)(c->cap / kBlockSlots) * block_bytes(c->cb);
+  // the workspace of mc_kv_attend_dev is part of the cache, so that no call allocates
+  *head = 256 + kMaxPartials * (sizeof(int) + kAttendRows * (2 + s.head_dim) * sizeof(float));
+  const double need = (double)c->region * s.sessions * s.heads + (double)*head;
+  if (need > 9e18) return set_error(kOutOfMemory, who + "a cache of " + std::to_string(need) + " bytes");
+  *bytes = (size_t)c->region * s.sessions * s.heads + *head;
+  return kOk;
+}
+
+}  // namespace kv
+}  // namespace mc
+
+extern "C" int mc_kv_bytes(const mc_kv_spec* spec, size_t* bytes) {
+  using namespace mc;
+  clear_error();
+  kv::Cache c;
+  size_t head = 0;
+  if (!bytes) return set_error(kInvalidArgument, "mc_kv_bytes: null argument");
+  return kv::layout("mc_kv_bytes", spec, &c, &head, bytes);
+}
+
+extern "C" int mc_kv_open(int device, const mc_kv_spec* spec, void* memory, void* stream, mc_kv** out) {
+  using namespace mc;
+  clear_error();
+  if (!out) return set_error(kInvalidArgument, "mc_kv_open: null argument");
+  *out = nullptr;
+  kv::Cache c;
+  size_t head = 0, bytes = 0;
+  const int st = kv::layout("mc_kv_open", spec, &c, &head, &bytes);
+  if (st != kOk) return st;
+  if (reinterpret_cast<uintptr_t>(memory) % 256) return set_error(kInvalidArgument, "mc_kv_open: memory must be 256-byte aligned");
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(device));
-  kv::Cache c{};
-  c.sessions = s.sessions;
-  c.heads = s.heads;
-  c.dim = s.head_dim;
-  c.bits = s.bits;
-  c.slots = s.slots;
-  c.sinks = s.sinks;
-  c.ring = s.slots - s.sinks;
-  c.cap = (s.slots + 63) / 64 * 64;
-  c.cb = s.head_dim * s.bits / 8;
-  c.region = (long long)(c.cap / kv::kBlockSlots) * kv::block_bytes(c.cb);
-  // the workspace of mc_kv_attend_dev is part of the cache, so that no call allocates
-  const size_t head = 256 + kv::kMaxPartials * (sizeof(int) + kv::kAttendRows * (2 + s.head_dim) * sizeof(float));
-  const double need = (double)c.region * s.sessions * s.heads + (double)head;
-  size_t bytes = 0;
-  void* mem = nullptr;
   int n_sm = 0;
   MC_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
-  if (need < 9e18) bytes = (size_t)c.region * s.sessions * s.heads + head;
-  if (!bytes || cudaMalloc(&mem, bytes) != cudaSuccess) {
+  mc_kv* kv = new (std::nothrow) mc_kv;
+  if (!kv) return set_error(kOutOfMemory, "mc_kv_open: out of host memory");
+  void* mem = memory;
+  if (!mem && cudaMalloc(&mem, bytes) != cudaSuccess) {
     (void)cudaGetLastError();
-    return set_error(kOutOfMemory, "mc_kv_open: no room for a cache of " + std::to_string(need) + " bytes");
+    delete kv;
+    return set_error(kOutOfMemory, "mc_kv_open: no room for a cache of " + std::to_string(bytes) + " bytes");
   }
-  const cudaError_t e = cudaMemset(mem, 0, bytes);
+  const cudaError_t e = cudaMemsetAsync(mem, 0, bytes, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) {
-    cudaFree(mem);
-    return set_error(kCudaError, std::string("mc_kv_open: cudaMemset: ") + cudaGetErrorString(e));
+    if (!memory) cudaFree(mem);
+    delete kv;
+    return set_error(kCudaError, std::string("mc_kv_open: cudaMemsetAsync: ") + cudaGetErrorString(e));
   }
   c.error = static_cast<int*>(mem);
   c.base = static_cast<uint8_t*>(mem) + head;  // a multiple of 256
-  mc_kv* kv = new (std::nothrow) mc_kv;
-  if (!kv) {
-    cudaFree(mem);
-    return set_error(kOutOfMemory, "mc_kv_open: out of host memory");
-  }
   kv->device = device;
   kv->c = c;
   kv->mem = mem;
+  kv->own = !memory;
   kv->arrived = reinterpret_cast<int*>(static_cast<uint8_t*>(mem) + 256);
   kv->partial = reinterpret_cast<float*>(kv->arrived + kv::kMaxPartials);
   kv->n_sm = n_sm;
@@ -564,9 +595,12 @@ extern "C" int mc_kv_close(mc_kv* kv) {
   using namespace mc;
   clear_error();
   if (!kv) return kOk;
-  DeviceRestore restore_device;
-  cudaSetDevice(kv->device);
-  const cudaError_t e = cudaFree(kv->mem);  // waits for the device's work
+  cudaError_t e = cudaSuccess;
+  if (kv->own) {
+    DeviceRestore restore_device;
+    cudaSetDevice(kv->device);
+    e = cudaFree(kv->mem);  // waits for the device's work
+  }
   delete kv;
   if (e != cudaSuccess) return set_error(kCudaError, std::string("mc_kv_close: ") + cudaGetErrorString(e));
   return kOk;

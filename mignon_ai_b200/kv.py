@@ -38,7 +38,8 @@ class _Spec(ctypes.Structure):
 
 
 _lib.register({
-    "mc_kv_open": [_i, ctypes.POINTER(_Spec), ctypes.POINTER(c_vp)],
+    "mc_kv_bytes": [ctypes.POINTER(_Spec), ctypes.POINTER(ctypes.c_size_t)],
+    "mc_kv_open": [_i, ctypes.POINTER(_Spec), c_vp, c_vp, ctypes.POINTER(c_vp)],
     "mc_kv_close": [c_vp],
     "mc_kv_error": [c_vp],
     "mc_kv_write_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, c_vp, _i, c_vp],
@@ -101,21 +102,25 @@ def _ints(name: str, x: Optional[torch.Tensor], count: int, index: int) -> Optio
 class KvCache:
     """Keys and values of ``sessions`` sessions of one attention layer, held in 4 or 8 bits.
 
-    A session keeps its first ``sinks`` positions and the last ``slots - sinks``. Close it (or let
-    it go) when its work is done: ``close`` waits for the device.
+    A session keeps its first ``sinks`` positions and the last ``slots - sinks``. The cache lies in
+    ``memory``, a uint8 tensor allocated on the current stream; as with any tensor, work on other
+    streams has to be done, or recorded on it, before the cache is closed or let go.
     """
 
     def __init__(self, sessions: int, heads: int, head_dim: int, slots: int, bits: int = 4, sinks: int = 0, device: int = 0):
         self._h = c_vp()
-        spec = _Spec(sessions, heads, head_dim, bits, slots, sinks)
-        _lib.check(_lib.lib().mc_kv_open(device, ctypes.byref(spec), ctypes.byref(self._h)))
+        spec, n = _Spec(sessions, heads, head_dim, bits, slots, sinks), ctypes.c_size_t()
+        lib = _lib.lib()
+        _lib.check(lib.mc_kv_bytes(ctypes.byref(spec), ctypes.byref(n)))
+        self.memory = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", device))
+        _lib.check(lib.mc_kv_open(device, ctypes.byref(spec), self.memory.data_ptr(), _raw_stream(device), ctypes.byref(self._h)))
         self.sessions, self.heads, self.head_dim, self.slots = sessions, heads, head_dim, slots
         self.bits, self.sinks, self.device = bits, sinks, torch.device("cuda", device)
         self._lib, self._index, self._scale = _lib.lib(), device, head_dim ** -0.5
 
     def close(self):
         if self._h:
-            h, self._h = self._h, c_vp()
+            h, self._h, self.memory = self._h, c_vp(), None
             _lib.check(_lib.lib().mc_kv_close(h))
 
     def __del__(self):

@@ -460,6 +460,23 @@ def test_the_same_inputs_give_the_same_bits(kv):
     assert torch.equal(first, kv.window_attention(k, k, v, ints([0, 6000, 12000]), window=100))
 
 
+def test_a_cache_in_the_librarys_own_memory(kv):
+    """mc_kv_open without memory: the library allocates and frees it."""
+    import ctypes
+    from mignon_ai_b200 import _lib
+    h, spec = ctypes.c_void_p(), kv._Spec(3, 2, 64, 4, 100, 4)
+    _lib.check(_lib.lib().mc_kv_open(0, ctypes.byref(spec), None, None, ctypes.byref(h)))
+    cache = kv.KvCache(3, 2, 64, 100, sinks=4)
+    theirs, cache._h = cache._h, h  # the wrapper around the other handle
+    x = torch.randn((3, 2, 64), device=DEV)
+    cache.write(x, x, ints([0, 5, 99]))
+    rk, _ = cache.read(ints([0, 5, 99]), ints([1, 6, 100]))
+    assert torch.equal(rk.cpu(), ref.value(x.cpu(), 4).float())
+    cache._h = theirs
+    _lib.check(_lib.lib().mc_kv_close(h))
+    cache.close()
+
+
 @pytest.mark.parametrize("call", ["dtype", "shape", "device", "ints", "groups", "window", "scale", "stride"])
 def test_refusals(kv, call):
     cache = kv.KvCache(2, 2, 32, 8)

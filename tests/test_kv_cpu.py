@@ -20,13 +20,28 @@ def spec(**c):
                                  dict(slots=(1 << 30) + 1)])
 def test_open_refuses(bad):
     h = ctypes.c_void_p()
-    assert _lib.lib().mc_kv_open(0, ctypes.byref(spec(**bad)), ctypes.byref(h)) == INVALID
+    assert _lib.lib().mc_kv_open(0, ctypes.byref(spec(**bad)), None, None, ctypes.byref(h)) == INVALID
     assert _lib.lib().mc_last_error() and not h
+    n = ctypes.c_size_t()
+    assert _lib.lib().mc_kv_bytes(ctypes.byref(spec(**bad)), ctypes.byref(n)) == INVALID
+
+
+def test_bytes():
+    """Codes of 4 or 8 bits and two 16-bit numbers a row, slots rounded up to 64, and the workspace."""
+    for bits, dim, slots in ((4, 64, 100), (8, 128, 64), (4, 16, 1)):
+        n = ctypes.c_size_t()
+        assert _lib.lib().mc_kv_bytes(ctypes.byref(spec(bits=bits, head_dim=dim, slots=slots, sinks=0)), ctypes.byref(n)) == 0
+        rows = 2 * 2 * 2 * ((slots + 63) // 64 * 64)
+        assert 0 <= n.value - rows * (dim * bits // 8 + 4) <= 12 << 20
+    assert _lib.lib().mc_kv_open(0, ctypes.byref(spec()), 100, None, ctypes.byref(ctypes.c_void_p())) == INVALID  # not aligned
 
 
 def test_null_arguments():
     L = _lib.lib()
-    assert L.mc_kv_open(0, None, None) == INVALID
+    h = ctypes.c_void_p()
+    assert L.mc_kv_open(0, None, None, None, ctypes.byref(h)) == INVALID
+    assert L.mc_kv_open(0, ctypes.byref(spec()), None, None, None) == INVALID
+    assert L.mc_kv_bytes(None, None) == INVALID
     assert L.mc_kv_error(None) == INVALID
     assert L.mc_kv_close(None) == 0
     r = ctypes.byref(kv._Rows(16, 64, 64))
