@@ -3,7 +3,11 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <mutex>
 #include <new>
+#include <set>
+#include <type_traits>
+#include <utility>
 
 #include "../../include/mignon_cuda.h"
 #include "mc_host.h"
@@ -217,6 +221,50 @@ struct Raw8 {
   }
 };
 
+// The extremes of a row held by eight lanes (NaN once an element is). 16-bit elements are compared in
+// pairs, as they are.
+template <class T>
+__device__ __forceinline__ void row_extremes(const Raw8<T> (&raw)[2], const bool (&in)[2], float& hi, float& lo) {
+  if constexpr (sizeof(T) == 4) {
+    hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (in[u]) {
+        float x[8];
+        raw[u].get(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hi = max_nan(hi, x[e]), lo = min_nan(lo, x[e]);
+      }
+#pragma unroll
+    for (int o = 1; o <= 4; o <<= 1) {
+      hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
+      lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
+    }
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 h, l;
+    h.x = h.y = from_float<T>(-INFINITY);
+    l.x = l.y = from_float<T>(INFINITY);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (in[u]) {
+        const T2* e = reinterpret_cast<const T2*>(raw[u].w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h = __hmax2_nan(h, e[i]), l = __hmin2_nan(l, e[i]);
+      }
+    T2 both;  // the maximum of the elements and that of their negatives
+    both.x = __hmax_nan(h.x, h.y);
+    both.y = __hneg(__hmin_nan(l.x, l.y));
+#pragma unroll
+    for (int o = 1; o <= 4; o <<= 1) {
+      const uint32_t other = __shfl_xor_sync(~0u, *reinterpret_cast<const uint32_t*>(&both), o);
+      both = __hmax2_nan(both, *reinterpret_cast<const T2*>(&other));
+    }
+    hi = to_float<T>(both.x);
+    lo = -to_float<T>(both.y);
+  }
+}
+
 // The four rows of one group of slots, heads [h0, h1).
 template <class T, int BITS>
 __device__ void write_group(const RowArgs& a, int row0, int h0, int h1, int session, int slot0) {
@@ -236,20 +284,8 @@ __device__ void write_group(const RowArgs& a, int row0, int h0, int h1, int sess
         if (in[u]) raw[which][u].load(rows[which] + 64 * u, a.vec);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      float hi = -INFINITY, lo = INFINITY;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (in[u]) {
-          float x[8];
-          raw[which][u].get(x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) hi = max_nan(hi, x[e]), lo = min_nan(lo, x[e]);
-        }
-#pragma unroll
-      for (int o = 1; o <= 4; o <<= 1) {
-        hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
-        lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
-      }
+      float hi, lo;
+      row_extremes<T>(raw[which], in, hi, lo);
       const Quant q = quant_of(hi, lo, BITS);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -310,19 +346,32 @@ __device__ void read_group(const RowArgs& a, int row0, int h0, int h1, int sessi
   T* rows[2] = {static_cast<T*>(a.k.p) + (row0 + s) * a.k.row + h0 * a.k.head + 8 * c0,
                 static_cast<T*>(a.v.p) + (row0 + s) * a.v.row + h0 * a.v.head + 8 * c0};
   const bool in[2] = {c0 < chunks, c0 + 8 < chunks};
-  for (int h = h0; h < h1; ++h) {
-    uint32_t w[2][2][W] = {};
-    uint32_t param[2];
+  // a head's words, loaded while the head before it is decoded
+  uint32_t w[2][2][W] = {}, param[2], w_next[2][2][W] = {}, param_next[2];
+  auto load = [&](const uint32_t* from, uint32_t (&words)[2][2][W], uint32_t (&params)[2]) {
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         if (in[u]) {
 #pragma unroll
-          for (int i = 0; i < W; ++i) w[which][u][i] = block[which ? at.value[u][i] : at.key[u][i]];
+          for (int i = 0; i < W; ++i) words[which][u][i] = __ldg(from + (which ? at.value[u][i] : at.key[u][i]));
         }
-      param[which] = block[param_at + (which ? kBlockSlots * (cb + 4) / 4 : 0)];
+      params[which] = __ldg(from + param_at + (which ? kBlockSlots * (cb + 4) / 4 : 0));
     }
+  };
+  load(block, w_next, param_next);
+  for (int h = h0; h < h1; ++h) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      param[which] = param_next[which];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[which][u][i] = w_next[which][u][i];
+    }
+    block += a.c.region / 4;
+    if (h + 1 < h1) load(block, w_next, param_next);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       // nibbles come as bytes 16c + 8 = 8m, so their scale is an eighth
@@ -352,14 +401,13 @@ __device__ void read_group(const RowArgs& a, int row0, int h0, int h1, int sessi
       }
       rows[which] += which ? a.v.head : a.k.head;
     }
-    block += a.c.region / 4;
   }
 }
 
 // One warp per group of slots and a.warp_heads heads of the segments. Segment b's groups have numbers
 // from start[b] / 4 + 2b on: room for its rows / 4 + 2, and it has no more whatever its first slot.
 template <class T, bool WRITE>
-__global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5) : 6) segment_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5) : 5) segment_kernel(const __grid_constant__ RowArgs a) {
   __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned item = blockIdx.x * (kCacheThreads / 32) + warp;  // fewer than 2^31
@@ -450,6 +498,18 @@ struct mc_kv {
 namespace mc {
 namespace kv {
 
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once for each.
+static cudaError_t allow_smem(const void* f, int device, int bytes) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({f, device})) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.insert({f, device});
+  return e;
+}
+
 static bool rows_ok(const mc_rows* r) { return r && r->data; }
 static Rows rows_of(const mc_rows* r) { return Rows{r->data, (long long)r->row_stride, (long long)r->head_stride}; }
 
@@ -481,8 +541,9 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
   auto aligned = [&](const mc_rows* r) {  // for the 16-byte accesses of eight elements
     return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
   };
-  // Groups of slots pay once a segment has rows to fill them: GROUPS_RULE
-  const bool groups = start && n_rows >= 4ll * n_seg;
+  // Groups of slots pay once segments have two rows on average: write and read of 8192 segments, 8 heads of
+  // 64, in us by groups and row by row: 1.5 rows a segment 204, 183; 2 rows 240, 246; 5 rows 306, 520.
+  const bool groups = start && n_rows >= 2ll * n_seg;
   long long warps = (long long)n_rows * kv->c.heads;
   int warp_heads = 1;
   if (groups) {
@@ -640,6 +701,32 @@ extern "C" int mc_kv_read_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int
                             n_segments, static_cast<cudaStream_t>(stream));
 }
 
+namespace mc {
+namespace kv {
+
+// CTAs that an item's visible slots are split over (0: none, a warp to an item), for `warps` resident
+// warps. A warp costs about as much as 160 slots on top of those it reads (start, query planes, joining);
+// up to three waves count whole. Both sides measured, us, 8 heads of 64 in 8 bits, 1024 slots: 16 sessions
+// 29 with a warp to an item, 12 split; 64: 31, 27; 200: 41, 46; 300 (one item more than a wave): 79, 64;
+// 256 slots: 64 sessions 12, 10; 200: 17, 24.
+static int attend_pieces(long long items, long long slots, long long warps) {
+  auto cost = [&](long long n, double read) {
+    const double waves = (double)n / warps;
+    return (waves <= 3 ? std::ceil(waves) : waves) * (160 + read);
+  };
+  int best = 0;
+  double least = cost(items, (double)slots);
+  const long long most = std::min<long long>({kMaxPieces, kMaxPartials / items, (slots + 127) / 128});
+  for (int p = 1; p <= std::max(1ll, most); ++p) {
+    const double c = cost(items * kAttendWarps * p, (double)slots / (kAttendWarps * p));
+    if (c < least) best = p, least = c;
+  }
+  return best;
+}
+
+}  // namespace kv
+}  // namespace mc
+
 extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out, int dtype, int q_heads,
                                 const int32_t* sessions, const int32_t* lens, int n, int window, float scale,
                                 void* stream) {
@@ -658,13 +745,9 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   const Cache& c = kv->c;
   const int group = q_heads / c.heads, row_groups = (group + kAttendRows - 1) / kAttendRows;
   const long long items = (long long)n * c.heads * row_groups;
-  // CTAs (of four warps) that an item's slots are split over. SLOTS_RULE
-  const int seen = window > 0 ? (int)std::min<long long>(c.slots, (long long)window + c.sinks) : c.slots;
   const AttendVariant f = attend_variant(c.bits, c.dim, dtype == kF32 ? 3 : 2, group);
-  const long long ctas = (long long)f.ctas * kv->n_sm, most = std::min<long long>({(seen + 128 * kAttendWarps - 1) / (128 * kAttendWarps), kMaxPieces, kMaxPartials / std::max(1ll, items)});
-  int pieces = 0;  // 0: an item to a warp
-  if (items < kAttendWarps * ctas && seen > 64)
-    pieces = (int)std::max(1ll, std::min(most, 2 * items <= ctas ? ctas / items : (4 * ctas + items - 1) / items));
+  const long long ctas = (long long)f.ctas * kv->n_sm;
+  const int pieces = attend_pieces(items, window > 0 ? std::min<long long>(c.slots, (long long)window + c.sinks) : c.slots, ctas * kAttendWarps);
   const int size = dtype == kF32 ? 4 : 2;
   auto aligned = [&](const mc_rows* r) {
     return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
@@ -673,7 +756,7 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
                      pieces, sessions, lens, scale * 1.4426950408889634f, kv->partial, kv->arrived};
   if (items > INT_MAX) return set_error(kInvalidArgument, "mc_kv_attend_dev: too many rows");
   const long long blocks = pieces ? items : std::min<long long>((items + kAttendWarps - 1) / kAttendWarps, ctas);
-  MC_CUDA(cudaFuncSetAttribute(f.f, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
+  MC_CUDA(allow_smem(reinterpret_cast<const void*>(f.f), kv->device, f.smem));
   f.f<<<dim3((unsigned)blocks, std::max(1, pieces)), kAttendWarps * 32, f.smem, static_cast<cudaStream_t>(stream)>>>(a);
   MC_CUDA(cudaGetLastError());
   return kOk;

@@ -49,7 +49,9 @@ static int tc_launch(const Args& a, cudaStream_t stream) {
   if (!make_tmap_16(&mk, a.k.p, bf, a.dim, a.heads, a.n_k, 2 * a.k.head, 2 * a.k.row, 1, kTcKeys)) return kCudaError;
   if (!make_tmap_16(&mv, a.v.p, bf, a.dim, a.heads, a.n_k, 2 * a.v.head, 2 * a.v.row, 1, kTcKeys)) return kCudaError;
   const size_t smem = tc_smem(a.dim);
-  MC_CUDA(cudaFuncSetAttribute(tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem(128)));
+  int device = 0;
+  MC_CUDA(cudaGetDevice(&device));
+  MC_CUDA(kv::allow_smem(reinterpret_cast<const void*>(tc_kernel<T>), device, (int)tc_smem(128)));
   const long long tiles = a.n_q / tokens + (long long)a.n_seg;
   if (tiles > INT_MAX || a.heads > 65535) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows or heads");
   tc_kernel<T><<<dim3((unsigned)tiles, a.heads), kTcThreads, smem, stream>>>(mq, mk, mv, args);
@@ -62,7 +64,6 @@ static int tile_launch(const Args& a, cudaStream_t stream) {
   int dimp = 0;
   auto f = tile_variant<T>(a.dim, &dimp);
   const size_t smem = tile_smem(dimp);
-  MC_CUDA(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const long long tiles = a.n_q / (kTileRows / a.group) + (long long)a.n_seg;
   if (tiles > INT_MAX || a.heads > 65535) return set_error(kInvalidArgument, "mc_window_attn_dev: too many rows or heads");
   auto aligned = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.p) % 16 == 0 && r.row % 4 == 0 && r.head % 4 == 0; };
@@ -71,8 +72,11 @@ static int tile_launch(const Args& a, cudaStream_t stream) {
   // Heads one after the other in a CTA hide the start of all but the first (2000 prompts of 16-64 rows, 6
   // heads of 64: 317 us against 338), as long as the tiles, about half of the segments' last ones among
   // them, leave three waves of four CTAs an SM.
-  int heads = 1;
-  while (heads < a.heads && (a.n_q / (kTileRows / a.group) + a.n_seg / 2ll) * ((a.heads + heads) / (heads + 1)) >= 12 * 148ll) ++heads;
+  int device = 0, n_sm = 0, heads = 1;
+  MC_CUDA(cudaGetDevice(&device));
+  MC_CUDA(kv::allow_smem(reinterpret_cast<const void*>(f), device, (int)smem));
+  MC_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, device));
+  while (heads < a.heads && (a.n_q / (kTileRows / a.group) + a.n_seg / 2ll) * ((a.heads + heads) / (heads + 1)) >= 12ll * n_sm) ++heads;
   const TileArgs args{a, quads && aligned(a.k) && aligned(a.v), quads && aligned(a.q), a.dim % 2 == 0 && paired(a.out), heads};
   f<<<dim3((unsigned)tiles, (a.heads + args.heads - 1) / args.heads), kTileThreads, smem, stream>>>(args);
   MC_CUDA(cudaGetLastError());

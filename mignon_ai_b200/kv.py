@@ -84,6 +84,12 @@ def _rows(name: str, x: torch.Tensor, index: int, heads: Optional[int], dim: int
     return x.data_ptr() or 16, stride[0], stride[1]
 
 
+def _address(x: torch.Tensor) -> Tuple[int, int, int]:
+    """_rows of a tensor that was made here."""
+    stride = x.stride()
+    return x.data_ptr() or 16, stride[0], stride[1]
+
+
 def _dtype(x: torch.Tensor) -> int:
     code = _DTYPES.get(x.dtype)
     if code is None:
@@ -169,12 +175,14 @@ class KvCache:
                 n_rows = pos0.shape[0]
             k = torch.empty((n_rows, self.heads, self.head_dim), dtype=dtype, device=self.device)
             v = torch.empty_like(k)
+            k_rows, v_rows = _address(k), _address(v)
         else:
             k, v = out
             n_rows = k.shape[0]
+            k_rows = _rows("out[0]", k, self._index, self.heads, self.head_dim, k.dtype)
+            v_rows = _rows("out[1]", v, self._index, self.heads, self.head_dim, k.dtype, n_rows)
         code, index, s = _dtype(k), self._index, _scratch
-        _pack(s.buf, 0, *_rows("out[0]", k, index, self.heads, self.head_dim, k.dtype),
-              *_rows("out[1]", v, index, self.heads, self.head_dim, k.dtype, n_rows), 0, 0, 0, 0, 0, 0)
+        _pack(s.buf, 0, *k_rows, *v_rows, 0, 0, 0, 0, 0, 0)
         start, sess, pos, n = self._segments(n_rows, pos0, row_start, sessions)
         status = self._lib.mc_kv_read_dev(self._h, s.rows[0], s.rows[1], code, n_rows, start, sess, pos,
                                           _ints("lens", lens, n, index), n, _raw_stream(index))
@@ -192,7 +200,10 @@ class KvCache:
         n, q_heads, _ = q.shape
         if out is None:
             out = torch.empty_like(q)
-        _pack(s.buf, 0, *rows, *_rows("out", out, index, q_heads, self.head_dim, q.dtype, n), 0, 0, 0, 0, 0, 0)
+            out_rows = _address(out)
+        else:
+            out_rows = _rows("out", out, index, q_heads, self.head_dim, q.dtype, n)
+        _pack(s.buf, 0, *rows, *out_rows, 0, 0, 0, 0, 0, 0)
         status = self._lib.mc_kv_attend_dev(
             self._h, s.rows[0], s.rows[1], code, q_heads, _ints("sessions", sessions, n, index),
             _ints("lens", lens, n, index), n, window, self._scale if scale is None else scale, _raw_stream(index))
@@ -212,13 +223,15 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     if index < 0:
         raise ValueError("q: expected a CUDA tensor")
     code = _dtype(q)
-    if out is None:
-        out = torch.empty_like(q)
     q_rows, k_rows = _rows("q", q, index, None, dim, dtype), _rows("k", k, index, None, dim, dtype)
     n_q, q_heads, _ = q.shape
     n_k, heads, _ = k.shape
-    _pack(s.buf, 0, *q_rows, *k_rows, *_rows("v", v, index, heads, dim, dtype, n_k),
-          *_rows("out", out, index, q_heads, dim, dtype, n_q))
+    if out is None:
+        out = torch.empty_like(q)
+        out_rows = _address(out)
+    else:
+        out_rows = _rows("out", out, index, q_heads, dim, dtype, n_q)
+    _pack(s.buf, 0, *q_rows, *k_rows, *_rows("v", v, index, heads, dim, dtype, n_k), *out_rows)
     if k_start is None:
         k_start = q_start
     elif q_start is None:

@@ -460,6 +460,49 @@ def test_the_same_inputs_give_the_same_bits(kv):
     assert torch.equal(first, kv.window_attention(k, k, v, ints([0, 6000, 12000]), window=100))
 
 
+def test_head_major_rows(kv):
+    """Rows as views of [heads, rows, dim] tensors: the head stride above the row stride."""
+    g = gen(13)
+    heads, group, dim, n = 2, 2, 64, 90
+    for dtype in ("f32", "bf16"):
+        x = [torch.randn((h, n, dim), generator=g).to(DTYPES[dtype]).to(DEV).transpose(0, 1) for h in (heads * group, heads, heads)]
+        got = kv.window_attention(*x, window=33, sinks=2)
+        cache = kv.KvCache(1, heads, dim, n, bits=8)
+        cache.write(x[1], x[2], ints([0]), ints([0, n]))
+        rk, rv = cache.read(ints([0]), ints([n]), ints([0, n]), n_rows=n)
+        one = cache.attend(x[0][n - 1:], ints([n]))
+        q, k, v = (y.cpu() for y in x)
+        assert torch.equal(rk.cpu(), ref.value(k, 8).float()) and torch.equal(rv.cpu(), ref.value(v, 8).float())
+        i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+        seen = (j <= i) & ((j < 2) | (j > i - 33))
+        for h in range(heads * group):
+            vmax = v.float().abs().max().item()
+            close(got[:, h], ref.attention(q[:, h], k[:, h // group], v[:, h // group], seen), vmax, dtype)
+            want = ref.attention(q[n - 1:, h], ref.value(k, 8)[:, h // group], ref.value(v, 8)[:, h // group], seen[:1] | True)
+            close(one[:, h], want, vmax, dtype)
+
+
+def test_places_far_into_a_large_cache(kv):
+    """Places more than 2^32 bytes into the cache, and positions above 2^30."""
+    g = gen(14)
+    heads, dim, slots = 8, 128, 1 << 20
+    cache = kv.KvCache(3, heads, dim, slots, bits=8, sinks=3)
+    assert cache.memory.numel() > 1 << 32
+    ring = slots - 3
+    for first in (slots - 70, 3 + ring * 1025 - 40):  # up to the cache's last place; across the ring's end
+        k, v = rows(g, 64, heads, dim, "bf16"), rows(g, 64, heads, dim, "bf16")
+        q = torch.randn((1, heads, dim), generator=g).bfloat16()
+        cache.write(k.to(DEV), v.to(DEV), ints([first]), ints([0, 64]), ints([2]))
+        rk, rv = cache.read(ints([first]), ints([first + 64]), ints([0, 64]), n_rows=64, sessions=ints([2]))
+        assert torch.equal(rk.cpu(), ref.value(k, 8).float()) and torch.equal(rv.cpu(), ref.value(v, 8).float())
+        got = cache.attend(q.to(DEV), ints([first + 64]), sessions=ints([2]), window=64)
+        cache.check()
+        for h in range(heads):  # the three first positions are zeros: codes of nothing written
+            kk, vv = (torch.cat([torch.zeros((3, dim), dtype=torch.float64), ref.value(y, 8)[:, h]]) for y in (k, v))
+            want = ref.attention(q[:, h], kk, vv, torch.ones((1, 67), dtype=torch.bool))
+            close(got[:, h], want, vv.abs().max().item(), "bf16", h)
+
+
 def test_a_cache_in_the_librarys_own_memory(kv):
     """mc_kv_open without memory: the library allocates and frees it."""
     import ctypes
