@@ -27,8 +27,9 @@ constexpr int kCacheThreads = 256;
 // four), eight lanes to a row, a lane eight consecutive dimensions of it (and the eight 64 further
 // on). Then every access is a full word or vector: the keys' words of four rows are 16 consecutive
 // bytes, and the values' words, which hold one dimension of four rows, are made by a byte
-// transpose over the four rows' lanes (two shuffles). Rows that do not fill a group (the ends of a
-// segment, the two sides of a ring's end, single tokens) go one at a time by a whole warp.
+// transpose over the four rows' lanes (two shuffles); at the ends of a segment the values' bytes are
+// written one by one. Rows whose slots do not follow their order in a group (past a ring's end that is
+// not a multiple of four) and single tokens go one at a time by a whole warp.
 //
 // Bound by memory: the rows' bytes and the codes'.
 // ------------------------------------------------------------------------------------------------
@@ -265,23 +266,34 @@ __device__ __forceinline__ void row_extremes(const Raw8<T> (&raw)[2], const bool
   }
 }
 
-// The four rows of one group of slots, heads [h0, h1).
+// The rows of one group of slots, heads [h0, h1): lane (s, c) has the row of slot0 + s, if that is `live`.
 template <class T, int BITS>
-__device__ void write_group(const RowArgs& a, int row0, int h0, int h1, int session, int slot0) {
+__device__ void write_group(const RowArgs& a, int row, bool live, int h0, int h1, int session, int slot0) {
   const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
   const LaneWords<BITS> at(slot0, cb);
   const int param_at = param_word_at(slot0, cb) + s;
   uint32_t* block = reinterpret_cast<uint32_t*>(region_of(a.c, session, h0) + (long long)(slot0 >> 5) * block_bytes(cb));
-  const T* rows[2] = {static_cast<const T*>(a.k.p) + (row0 + s) * a.k.row + h0 * a.k.head + 8 * c0,
-                      static_cast<const T*>(a.v.p) + (row0 + s) * a.v.row + h0 * a.v.head + 8 * c0};
+  const T* rows[2] = {static_cast<const T*>(a.k.p) + row * a.k.row + h0 * a.k.head + 8 * c0,
+                      static_cast<const T*>(a.v.p) + row * a.v.row + h0 * a.v.head + 8 * c0};
   const bool in[2] = {c0 < chunks, c0 + 8 < chunks};
+  const unsigned rows_live = __ballot_sync(~0u, live);  // a row's eight lanes alike
+  // a word of values, one byte a row: whole, or the bytes of the rows there are
+  auto store_values = [&](uint32_t* at_word, uint32_t word) {
+    if (rows_live == ~0u) {
+      *at_word = word;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (rows_live >> (8 * r) & 1) reinterpret_cast<uint8_t*>(at_word)[r] = (uint8_t)(word >> (8 * r));
+    }
+  };
   for (int h = h0; h < h1; ++h) {
     Raw8<T> raw[2][2];
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        if (in[u]) raw[which][u].load(rows[which] + 64 * u, a.vec);
+        if (in[u] && live) raw[which][u].load(rows[which] + 64 * u, a.vec);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       float hi, lo;
@@ -298,8 +310,8 @@ __device__ void write_group(const RowArgs& a, int row0, int h0, int h1, int sess
         const uint32_t b1 = pack_low_bytes(code[4], code[5], code[6], code[7]);
         if (which == 0) {
           if constexpr (BITS == 4) {
-            if (in[u]) block[at.key[u][0]] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
-          } else if (in[u]) {
+            if (in[u] && live) block[at.key[u][0]] = (b0 & 0x0F0F0F0Fu) | ((b1 << 4) & 0xF0F0F0F0u);
+          } else if (in[u] && live) {
             block[at.key[u][0]] = b0;
             block[at.key[u][BITS / 4 - 1]] = b1;
           }
@@ -309,16 +321,16 @@ __device__ void write_group(const RowArgs& a, int row0, int h0, int h1, int sess
           const uint32_t got = __shfl_xor_sync(~0u, odd ? b0 : b1, 1);
           const uint32_t low = odd ? got : b0, high = odd ? b1 : got;
           const uint32_t word = transpose_bytes((low & 0x0F0F0F0Fu) | ((high << 4) & 0xF0F0F0F0u), s);
-          if (in[u]) block[at.value[u][0]] = word;
+          if (in[u]) store_values(block + at.value[u][0], word);
         } else {
           const uint32_t w0 = transpose_bytes(b0, s), w1 = transpose_bytes(b1, s);
           if (in[u]) {
-            block[at.value[u][0]] = w0;
-            block[at.value[u][BITS / 4 - 1]] = w1;
+            store_values(block + at.value[u][0], w0);
+            store_values(block + at.value[u][BITS / 4 - 1], w1);
           }
         }
       }
-      if (c0 == 0) block[param_at + (which ? kBlockSlots * (cb + 4) / 4 : 0)] = param_word(q);
+      if (c0 == 0 && live) block[param_at + (which ? kBlockSlots * (cb + 4) / 4 : 0)] = param_word(q);
       rows[which] += which ? a.v.head : a.k.head;
     }
     block += a.c.region / 4;
@@ -336,15 +348,16 @@ __device__ __forceinline__ void decode4(float* x, uint32_t biased, float2 scale,
   }
 }
 
+// As write_group; a row that is `mine` but not live comes back as zeros.
 template <class T, int BITS>
-__device__ void read_group(const RowArgs& a, int row0, int h0, int h1, int session, int slot0) {
+__device__ void read_group(const RowArgs& a, int row, bool mine, bool live, int h0, int h1, int session, int slot0) {
   constexpr int W = BITS / 4;
   const int lane = threadIdx.x & 31, s = lane >> 3, c0 = lane & 7, chunks = a.c.dim / 8, cb = a.c.cb;
   const LaneWords<BITS> at(slot0, cb);
   const int param_at = param_word_at(slot0, cb) + s;
   const uint32_t* block = reinterpret_cast<const uint32_t*>(region_of(a.c, session, h0) + (long long)(slot0 >> 5) * block_bytes(cb));
-  T* rows[2] = {static_cast<T*>(a.k.p) + (row0 + s) * a.k.row + h0 * a.k.head + 8 * c0,
-                static_cast<T*>(a.v.p) + (row0 + s) * a.v.row + h0 * a.v.head + 8 * c0};
+  T* rows[2] = {static_cast<T*>(a.k.p) + row * a.k.row + h0 * a.k.head + 8 * c0,
+                static_cast<T*>(a.v.p) + row * a.v.row + h0 * a.v.head + 8 * c0};
   const bool in[2] = {c0 < chunks, c0 + 8 < chunks};
   // a head's words, loaded while the head before it is decoded
   uint32_t w[2][2][W] = {}, param[2], w_next[2][2][W] = {}, param_next[2];
@@ -397,7 +410,11 @@ __device__ void read_group(const RowArgs& a, int row0, int h0, int h1, int sessi
         float y[8];
         decode4(y, b0 ^ 0x80808080u, scale2, center2);
         decode4(y + 4, b1 ^ 0x80808080u, scale2, center2);
-        if (in[u]) store8<T>(rows[which] + 64 * u, y, a.vec);
+        if (!live) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        }
+        if (in[u] && mine) store8<T>(rows[which] + 64 * u, y, a.vec);
       }
       rows[which] += which ? a.v.head : a.k.head;
     }
@@ -425,36 +442,43 @@ __global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5
   const long long at = (long long)group - ((first >> 2) + 2ll * b);
   if (rows <= 0 || first < 0 || rows > a.n_rows - first || at < 0) return;
   const int offset = a.pos0[b] >= 0 ? slot_of(a.c, a.pos0[b]) & 3 : 0;  // of the segment's first row in its group
-  const long long begin = max(0ll, 4 * at - offset), end = min((long long)rows, 4 * at - offset + 4);
-  if (begin >= end) return;
-  const int row0 = first + (int)begin, count = (int)(end - begin);
-  // rows by lane: lane 8s + c asks for row s
+  // lane 8s + c asks for the row of the group's slot s
   const int s = lane >> 3;
-  const RowPlace p = place<WRITE>(a, b, first, rows, row0 + min(s, count - 1));
-  const int slot0 = __shfl_sync(~0u, p.slot, 0);
-  if (__all_sync(~0u, count == 4 && slot0 >= 0 && (slot0 & 3) == 0 && p.slot == slot0 + s)) {
+  const long long i = 4 * at - offset + s;
+  const bool mine = i >= 0 && i < rows;
+  const unsigned any = __ballot_sync(~0u, mine);
+  if (!any) return;
+  const int row = mine ? first + (int)i : first;
+  const RowPlace p = place<WRITE>(a, b, first, rows, mine ? row : first);
+  const int slot = mine ? p.slot : -1;
+  const unsigned live = __ballot_sync(~0u, slot >= 0);
+  const int slot0 = live ? __shfl_sync(~0u, slot, __ffs(live) - 1) & ~3 : 0;
+  if (__all_sync(~0u, slot < 0 || slot == slot0 + s)) {
+    if (WRITE && !live) return;
     if (a.c.bits == 4) {
-      if constexpr (WRITE) write_group<T, 4>(a, row0, h0, h1, p.session, slot0);
-      else read_group<T, 4>(a, row0, h0, h1, p.session, slot0);
+      if constexpr (WRITE) write_group<T, 4>(a, row, slot >= 0, h0, h1, p.session, slot0);
+      else read_group<T, 4>(a, row, mine, slot >= 0, h0, h1, p.session, slot0);
     } else {
-      if constexpr (WRITE) write_group<T, 8>(a, row0, h0, h1, p.session, slot0);
-      else read_group<T, 8>(a, row0, h0, h1, p.session, slot0);
+      if constexpr (WRITE) write_group<T, 8>(a, row, slot >= 0, h0, h1, p.session, slot0);
+      else read_group<T, 8>(a, row, mine, slot >= 0, h0, h1, p.session, slot0);
     }
     return;
   }
-  for (int i = 0; i < count; ++i) {
-    const RowPlace q{p.session, __shfl_sync(~0u, p.slot, 8 * i)};
+  for (int r = 0; r < 4; ++r) {
+    if (!(any >> (8 * r) & 1)) continue;
+    const RowPlace q{p.session, __shfl_sync(~0u, slot, 8 * r)};
+    const int at_row = __shfl_sync(~0u, row, 8 * r);
     for (int h = h0; h < h1; ++h) {
       if constexpr (WRITE) {
-        if (q.slot >= 0) write_row<T>(a, row0 + i, h, q, codes[warp]);
+        if (q.slot >= 0) write_row<T>(a, at_row, h, q, codes[warp]);
       } else {
-        read_row<T>(a, row0 + i, h, q);
+        read_row<T>(a, at_row, h, q);
       }
     }
   }
 }
 
-// One warp per (row, head): rows that are a segment of their own (no starts), and short segments.
+// One warp per (row, head): rows that are a segment of their own.
 template <class T, bool WRITE>
 __global__ void __launch_bounds__(kCacheThreads) single_kernel(const __grid_constant__ RowArgs a) {
   __shared__ int8_t codes[WRITE ? kCacheThreads / 32 : 1][kMaxDim];
@@ -498,9 +522,10 @@ struct mc_kv {
 namespace mc {
 namespace kv {
 
-// Lets a kernel use `bytes` of dynamic shared memory on the current device, once for each.
+// Lets a kernel use `bytes` of dynamic shared memory on the current device, once for each. 48 KB need no
+// leave, but what the kernels have besides (at most 8 KB) counts too.
 static cudaError_t allow_smem(const void* f, int device, int bytes) {
-  if (bytes <= 48 * 1024) return cudaSuccess;
+  if (bytes <= 40 * 1024) return cudaSuccess;
   static std::mutex mu;
   static std::set<std::pair<const void*, int>> done;
   std::lock_guard<std::mutex> lock(mu);
@@ -541,9 +566,9 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
   auto aligned = [&](const mc_rows* r) {  // for the 16-byte accesses of eight elements
     return reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride * size % 16 == 0 && r->head_stride * size % 16 == 0;
   };
-  // Groups of slots pay once segments have two rows on average: write and read of 8192 segments, 8 heads of
-  // 64, in us by groups and row by row: 1.5 rows a segment 204, 183; 2 rows 240, 246; 5 rows 306, 520.
-  const bool groups = start && n_rows >= 2ll * n_seg;
+  // Groups of slots pay once segments have more than a row: write and read of 8192 segments, 8 heads of 64,
+  // in us by groups and row by row: 1 row a segment 102, 98; 1.5 rows 117, 182; 5 rows 172, 516.
+  const bool groups = start && n_rows > n_seg;
   long long warps = (long long)n_rows * kv->c.heads;
   int warp_heads = 1;
   if (groups) {
