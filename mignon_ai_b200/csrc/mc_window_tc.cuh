@@ -12,7 +12,12 @@
 //
 // Two CTAs share an SM (96 KB of operands and 256 TMEM columns each), so one's products run
 // under the other's exponentials: per tile the tensor pipe needs about 1000 cycles at dim 128 and
-// the exponentials as many.
+// the exponentials as many. 8192 positions, 32/8 heads of 128, window 1024 with 4 sinks, bfloat16: 243 us,
+// 530 TFLOP/s of the visible pairs (a third more is computed, in tiles that the window cuts); the
+// tensor pipe is 32 % busy. What bounds it is the chain of a tile in one CTA, 6500 cycles: 1700 for
+// the products, 1400 until the maximum is known, 2200 for the weights, 700 of meeting and handing over.
+// One thread a row (4 warps, S read twice) took 250 us; half of the weights by a cubic instead of the
+// exponential unit 240.
 //
 // A hidden key's weight is an exact zero, but zero times an infinity or NaN among its values would
 // still reach the row. A row that comes out non-finite is therefore computed again key by key
