@@ -92,16 +92,6 @@ __device__ __forceinline__ int slot_of(const Cache& c, int pos) {
   return pos < c.sinks ? pos : c.sinks + (pos - c.sinks) % c.ring;
 }
 
-// The position that slot s holds in a session of `len` positions, or -1.
-__device__ __forceinline__ int position_of(const Cache& c, int s, int len) {
-  if (s < c.sinks) return s < len ? s : -1;
-  const int last = len - 1 - c.sinks, j = s - c.sinks;  // ring coordinates of the newest position and of s
-  if (j >= c.ring || last < 0) return -1;
-  const int back = last >= j ? (last - j) % c.ring : c.ring - (j - last);  // j - last < ring
-  const int p = last - back;
-  return p < 0 ? -1 : c.sinks + p;
-}
-
 // Whether a session of `len` positions still holds position pos.
 __device__ __forceinline__ bool is_held(const Cache& c, int pos, int len) {
   return pos >= 0 && pos < len && (pos < c.sinks || pos >= len - c.ring);
