@@ -19,6 +19,12 @@ struct Args {
   float scale;  // of the scores, times log2(e)
 };
 
+// The first key that the window shows a query at position pos. No subtraction leaves 32 bits, whatever the
+// window and for the negative positions of queries before every key.
+__device__ __forceinline__ int window_begin(int window, int pos) {
+  return window > 0 && pos >= window ? pos - window + 1 : 0;
+}
+
 // One query row by one warp, key by key: lane j scores keys j, j + 32, ..; then the lanes own
 // dimensions. Masked keys and values are not read, so whatever they hold reaches nothing.
 template <class T>
@@ -30,7 +36,7 @@ __device__ void row_attention(const Args& a, int row, int h, int k0, int pos, fl
   const T* v = static_cast<const T*>(a.v.p) + k0 * a.v.row + hk * a.v.head;
   for (int d = lane; d < dim; d += 32) qs[d] = to_float<T>(q[d]);
   __syncwarp();
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;  // first key of the window
+  const int lo = window_begin(a.window, pos);
   const int sink_end = min(a.sinks, lo);                        // visible keys before it
   float top = -INFINITY, total = 0.f, acc[kMaxDim / 32] = {};
   const int n = sink_end + (pos + 1 - lo);

@@ -82,7 +82,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
   const int tokens = min(tt, seg.nq - first);
   const int pos0 = seg.nk - seg.nq + first, pos1 = pos0 + tokens - 1;  // positions of the first and last token
   // tiles of keys: the sinks' (below the window) and the window's
-  const int win_lo = a.window > 0 ? max(0, pos0 - a.window + 1) : 0;
+  const int win_lo = window_begin(a.window, pos0);
   const int win_tile = win_lo / kTcKeys;
   const int sink_tiles = pos1 < 0 ? 0 : min(win_tile, (min(a.sinks, win_lo) + kTcKeys - 1) / kTcKeys);
   const int n_tiles = pos1 < 0 ? 0 : sink_tiles + pos1 / kTcKeys - win_tile + 1;
@@ -168,7 +168,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
   } else {
     const int pos = pos0 + row_token;  // of this thread's row
     const bool real = row_token < tokens;
-    const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+    const int lo = window_begin(a.window, pos);
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
     const int c0 = 64 * half;  // this thread's keys of a tile
     auto meet = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };  // the softmax warps

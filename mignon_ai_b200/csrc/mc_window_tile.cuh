@@ -148,15 +148,15 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
     const int i = 16 * warp + r + 8 * e, token = i / a.group;
     real[e] = token < tokens;
     pos[e] = real[e] ? base + token : -1;
-    lo[e] = a.window > 0 ? max(0, pos[e] - a.window + 1) : 0;
+    lo[e] = window_begin(a.window, pos[e]);
     row[e] = seg.q0 + first + token;
     head[e] = i - token * a.group;  // among those that share a key/value head
   }
   // positions of the CTA's and of the warp's first and last real rows
   const int last_token = min(tokens - 1, (16 * warp + 15) / a.group), first_token = 16 * warp / a.group;
   const int w_hi = first_token < tokens ? base + last_token : -1;
-  const int w_lo = a.window > 0 ? max(0, base + first_token - a.window + 1) : 0;  // the warp's first windowed key
-  const int cta_hi = base + tokens - 1, cta_lo = a.window > 0 ? max(0, base - a.window + 1) : 0;
+  const int w_lo = window_begin(a.window, base + first_token);  // the warp's first windowed key
+  const int cta_hi = base + tokens - 1, cta_lo = window_begin(a.window, base);
   const int win_tile = cta_lo / kTileKeys;
   const int sink_tiles = cta_hi < 0 ? 0 : min(win_tile, (min(a.sinks, cta_lo) + kTileKeys - 1) / kTileKeys);
   const int n_tiles = cta_hi < 0 ? 0 : sink_tiles + cta_hi / kTileKeys - win_tile + 1;
