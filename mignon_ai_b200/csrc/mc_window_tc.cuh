@@ -23,6 +23,7 @@
 // still reach the row. A row that comes out non-finite is therefore computed again key by key
 // (row_attention), which reads visible keys only.
 #pragma once
+#include "mc_window_roles.h"
 #include "mc_window_row.cuh"
 
 namespace mc {
@@ -110,60 +111,64 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
 
   if (warp == 8) {
     if (lane == 0 && n_tiles > 0) {
-      bool ok = true;
-      mbar_arrive_expect_tx(q_full, (uint32_t)(blocks * tt * a.group * 128));
-      for (int c = 0; c < blocks; ++c) tma_load_3d(sq + c * kTcBlock, &mq, 64 * c, hk * a.group, seg.q0 + first, q_full);
-      int loads = 0;
-      for (int i = 0; i < n_tiles; ++i) {
-        const int key = seg.k0 + tile_key(i);
-        // the key buffer is free once the products of tile i - 1 are done: s_full's phase i - 1
-        if (i > 0 && !mbar_wait_or_abort(s_full, (i - 1) & 1, kErrWaitEmpty)) ok = false;
-        if (!ok) break;
-        mbar_arrive_expect_tx(k_full, (uint32_t)(blocks * kTcBlock));
-        for (int c = 0; c < blocks; ++c) tma_load_3d(sk + c * kTcBlock, &mk, 64 * c, hk, key, k_full);
-        if (i > 0 && !mbar_wait_or_abort(v_free, (i - 1) & 1, kErrWaitEmpty)) ok = false;
-        ++loads;
-        if (!ok) break;
-        mbar_arrive_expect_tx(v_full, (uint32_t)(blocks * kTcBlock));
-        for (int c = 0; c < blocks; ++c) tma_load_3d(sv + c * kTcBlock, &mv, 64 * c, hk, key, v_full);
-      }
-      // after a wait that gave up: never leave with copies in flight into this CTA's memory
-      if (!ok) {
-        mbar_wait(q_full, 0, kErrWaitFull);
-        if (loads > 0) mbar_wait(k_full, (loads - 1) & 1, kErrWaitFull);
-        if (loads > 1) mbar_wait(v_full, (loads - 2) & 1, kErrWaitFull);
-      }
+      struct {
+        const CUtensorMap *mq, *mk, *mv;
+        uint8_t *sq, *sk, *sv;
+        uint64_t *q_full, *k_full, *v_full, *s_full, *v_free;
+        int blocks, q_bytes, q_head, q_row, hk, k0, win_tile, sink_tiles;
+        __device__ int key(int i) const { return k0 + (i < sink_tiles ? i : win_tile + i - sink_tiles) * kTcKeys; }
+        __device__ void copy_queries() {
+          mbar_arrive_expect_tx(q_full, (uint32_t)q_bytes);
+          for (int c = 0; c < blocks; ++c) tma_load_3d(sq + c * kTcBlock, mq, 64 * c, q_head, q_row, q_full);
+        }
+        __device__ void copy_keys(int i) {
+          mbar_arrive_expect_tx(k_full, (uint32_t)(blocks * kTcBlock));
+          for (int c = 0; c < blocks; ++c) tma_load_3d(sk + c * kTcBlock, mk, 64 * c, hk, key(i), k_full);
+        }
+        __device__ void copy_values(int i) {
+          mbar_arrive_expect_tx(v_full, (uint32_t)(blocks * kTcBlock));
+          for (int c = 0; c < blocks; ++c) tma_load_3d(sv + c * kTcBlock, mv, 64 * c, hk, key(i), v_full);
+        }
+        __device__ bool wait_scores(int phase) { return mbar_wait_or_abort(s_full, phase, kErrWaitEmpty); }
+        __device__ bool wait_values_free(int phase) { return mbar_wait_or_abort(v_free, phase, kErrWaitEmpty); }
+        __device__ void drain_queries(int phase) { mbar_wait(q_full, phase, kErrWaitFull); }
+        __device__ void drain_keys(int phase) { mbar_wait(k_full, phase, kErrWaitFull); }
+        __device__ void drain_values(int phase) { mbar_wait(v_full, phase, kErrWaitFull); }
+      } copier{&mq, &mk, &mv, sq, sk, sv, q_full, k_full, v_full, s_full, v_free, blocks, blocks * tt * a.group * 128,
+               hk * a.group, seg.q0 + first, hk, seg.k0, win_tile, sink_tiles};
+      copy_tiles(copier, n_tiles);
     }
   } else if (warp == 9) {
     if (lane == 0 && n_tiles > 0) {
-      constexpr bool kBf = sizeof(T) == 2 && !std::is_same<T, __half>::value;
-      const uint32_t id_s = idesc_f16(128, kTcKeys, kBf, false), id_o = idesc_f16(128, dim, kBf, true);
-      const uint64_t dq = smem_desc_sw128(sq), dk = smem_desc_sw128(sk), dv = smem_desc_sw128_mn(sv, kTcBlock);
-      auto scores = [&]() {
-        for (int k = 0; k < dim / 16; ++k) {
-          const uint64_t off = (uint64_t)((k >> 2) * (kTcBlock >> 4) + (k & 3) * 2);
-          mma_f16(t_s, dq + off, dk + off, id_s, k > 0);
+      struct {
+        uint64_t *q_full, *k_full, *v_full, *s_full, *p_full, *o_full, *v_free;
+        uint64_t dq, dk, dv;
+        uint32_t t_s, t_o, id_s, id_o;
+        int dim;
+        __device__ void multiply_scores() {
+          for (int k = 0; k < dim / 16; ++k) {
+            const uint64_t off = (uint64_t)((k >> 2) * (kTcBlock >> 4) + (k & 3) * 2);
+            mma_f16(t_s, dq + off, dk + off, id_s, k > 0);
+          }
+          mma_commit(s_full);
         }
-        mma_commit(s_full);
-      };
-      bool ok = mbar_wait_or_abort(q_full, 0, kErrWaitFull) && mbar_wait_or_abort(k_full, 0, kErrWaitFull);
-      if (ok) scores();
-      for (int i = 0; ok && i < n_tiles; ++i) {
-        ok = mbar_wait_or_abort(p_full, i & 1, kErrWaitAccFree) && mbar_wait_or_abort(v_full, i & 1, kErrWaitFull);
-        if (!ok) break;
-        tc_fence_after();
-        for (int k = 0; k < kTcKeys / 16; ++k)
-          mma_f16_ts(t_o, t_s + 8 * k, dv + (uint64_t)k * (2048 >> 4), id_o, i > 0 || k > 0);
-        mma_commit(i + 1 < n_tiles ? v_free : o_full);
-        if (i + 1 < n_tiles) {
-          ok = mbar_wait_or_abort(k_full, (i + 1) & 1, kErrWaitFull);
-          if (ok) scores();  // after the products that read P from the same columns: MMAs run in order
+        __device__ void multiply_values(int i) {
+          tc_fence_after();
+          for (int k = 0; k < kTcKeys / 16; ++k)
+            mma_f16_ts(t_o, t_s + 8 * k, dv + (uint64_t)k * (2048 >> 4), id_o, i > 0 || k > 0);
         }
-      }
-      if (!ok) {  // a wait gave up: the MMAs issued so far end before TMEM is freed
-        mma_commit(o_full);
-        mbar_wait(o_full, 0, kErrWaitAcc);
-      }
+        __device__ void commit_values_free() { mma_commit(v_free); }
+        __device__ void commit_outputs() { mma_commit(o_full); }
+        __device__ bool wait_queries(int phase) { return mbar_wait_or_abort(q_full, phase, kErrWaitFull); }
+        __device__ bool wait_keys(int phase) { return mbar_wait_or_abort(k_full, phase, kErrWaitFull); }
+        __device__ bool wait_values(int phase) { return mbar_wait_or_abort(v_full, phase, kErrWaitFull); }
+        __device__ bool wait_weights(int phase) { return mbar_wait_or_abort(p_full, phase, kErrWaitAccFree); }
+        __device__ void drain_outputs(int phase) { mbar_wait(o_full, phase, kErrWaitAcc); }
+      } multiplier{q_full, k_full, v_full, s_full, p_full, o_full, v_free,
+                   smem_desc_sw128(sq), smem_desc_sw128(sk), smem_desc_sw128_mn(sv, kTcBlock), t_s, t_o,
+                   idesc_f16(128, kTcKeys, !std::is_same<T, __half>::value, false),
+                   idesc_f16(128, dim, !std::is_same<T, __half>::value, true), dim};
+      multiply_tiles(multiplier, n_tiles);
     }
   } else {
     const int pos = pos0 + row_token;  // of this thread's row
