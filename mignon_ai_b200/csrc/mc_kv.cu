@@ -556,12 +556,12 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
                       const int32_t* start, const int32_t* sess, const int32_t* pos0, const int32_t* lens, int n_seg,
                       cudaStream_t stream) {
   clear_error();
-  if (!kv || !rows_ok(k) || !rows_ok(v) || !pos0 || (!write && !lens))
-    return set_error(kInvalidArgument, std::string(name) + ": null argument");
+  if (!kv || !k || !v) return set_error(kInvalidArgument, std::string(name) + ": null argument");
   if (dtype < kF32 || dtype > kBF16) return set_error(kInvalidArgument, std::string(name) + ": unknown dtype");
   if (n_rows < 0 || n_seg < 0 || (!start && n_rows != n_seg))
     return set_error(kInvalidArgument, std::string(name) + ": negative counts, or rows without row_start that are not one per segment");
   if (n_rows == 0 || n_seg == 0) return kOk;
+  if (!k->data || !v->data || !pos0 || (!write && !lens)) return set_error(kInvalidArgument, std::string(name) + ": null argument");
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
   const int size = dtype == kF32 ? 4 : 2;
@@ -760,13 +760,14 @@ extern "C" int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out,
   using namespace mc;
   using namespace mc::kv;
   clear_error();
-  if (!kv || !rows_ok(q) || !rows_ok(out) || !lens) return set_error(kInvalidArgument, "mc_kv_attend_dev: null argument");
+  if (!kv || !q || !out) return set_error(kInvalidArgument, "mc_kv_attend_dev: null argument");
   if (dtype < kF32 || dtype > kBF16) return set_error(kInvalidArgument, "mc_kv_attend_dev: unknown dtype");
   if (n < 0 || window < 0) return set_error(kInvalidArgument, "mc_kv_attend_dev: n and window must not be negative");
   if (q_heads < 1 || q_heads % kv->c.heads)
     return set_error(kInvalidArgument, "mc_kv_attend_dev: q_heads must be a multiple of the cache's heads");
   if (!(scale > 0.f) || !std::isfinite(scale)) return set_error(kInvalidArgument, "mc_kv_attend_dev: scale must be positive");
   if (n == 0) return kOk;
+  if (!q->data || !out->data || !lens) return set_error(kInvalidArgument, "mc_kv_attend_dev: null argument");
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
   const Cache& c = kv->c;

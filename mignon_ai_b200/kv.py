@@ -102,7 +102,7 @@ def _ints(name: str, x: Optional[torch.Tensor], count: int, index: int) -> Optio
         return None
     if x.dtype is not torch.int32 or x.get_device() != index or x.shape != (count,) or not x.is_contiguous():
         raise ValueError(f"{name}: expected {count} contiguous int32 on cuda:{index}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.data_ptr()
+    return x.data_ptr() or 16  # as in _rows: null would mean that none were given
 
 
 class KvCache:

@@ -16,3 +16,33 @@ pytestmark = pytest.mark.gpu
 def test_windows_near_the_largest_number(kv, dtype, dim, window):
     """A window that shows everything, with queries before the first key: their positions are negative."""
     window_case(kv, dtype, dim, 1, 2, [40, 3, 150, 70], [-10, -3, -100, 20], window, 3)
+
+
+def test_calls_without_rows(kv):
+    """Empty batches, whose tensors have no address: nothing to do, and nothing is done."""
+    cache = kv.KvCache(2, 2, 32, 8)
+    x = torch.randn((2, 2, 32), device=DEV)
+    cache.write(x, x, ints([0, 0]))
+    none = ints([])
+    cache.write(x[:0], x[:0], none)
+    cache.write(x[:0], x[:0], none, sessions=none)
+    cache.write(x[:0], x[:0], none, ints([0]))
+    cache.write(x[:0], x[:0], ints([0, 0]), ints([0, 0, 0]))
+    for sessions in (None, none):
+        assert cache.attend(x[:0], none, sessions=sessions).shape == (0, 2, 32)
+        assert cache.read(none, none, sessions=sessions)[0].shape == (0, 2, 32)
+    assert cache.read(none, none, ints([0]), n_rows=0)[1].shape == (0, 2, 32)
+    assert cache.read(ints([0]), ints([1]), ints([0, 0]), n_rows=0)[1].shape == (0, 2, 32)
+    assert kv.window_attention(x[:0], x, x, ints([0]), ints([0])).shape == (0, 2, 32)
+    assert kv.window_attention(x[:0], x[:0], x[:0]).shape == (0, 2, 32)
+    rk, _ = cache.read(ints([0, 0]), ints([1, 1]))
+    assert torch.equal(rk.cpu(), ref.value(x.cpu(), 4).float())
+    cache.check()
+    # the library alone takes null arrays where there is nothing in them
+    L, r = cache._lib, ctypes.byref(kv._Rows(None, 64, 32))
+    assert L.mc_kv_write_dev(cache._h, r, r, 0, 0, None, None, None, 0, None) == 0
+    assert L.mc_kv_read_dev(cache._h, r, r, 0, 0, None, None, None, None, 0, None) == 0
+    assert L.mc_kv_attend_dev(cache._h, r, r, 0, 2, None, None, 0, 0, 1.0, None) == 0
+    # and none where there is something
+    assert L.mc_kv_write_dev(cache._h, r, r, 0, 1, None, None, None, 1, None) == 1
+    assert L.mc_kv_attend_dev(cache._h, r, r, 0, 2, None, None, 1, 0, 1.0, None) == 1
