@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kCacheThreads) single_kernel(const __grid_cons
   RowPlace w{0, -1};
   if (!a.start) {
     w = place<WRITE>(a, row, row, 1, row);
-  } else if (row >= a.start[0] && row < a.start[a.n_seg]) {
+  } else if (a.n_seg > 0 && row >= a.start[0] && row < a.start[a.n_seg]) {
     // where an even spread has the row (decode steps), else by search
     int b = min((int)((float)row * a.spread), a.n_seg - 1);
     if (a.start[b] > row || a.start[b + 1] <= row) b = last_at_most(a.n_seg, [&](int i) { return a.start[i] <= row; });
@@ -560,8 +560,8 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
   if (dtype < kF32 || dtype > kBF16) return set_error(kInvalidArgument, std::string(name) + ": unknown dtype");
   if (n_rows < 0 || n_seg < 0 || (!start && n_rows != n_seg))
     return set_error(kInvalidArgument, std::string(name) + ": negative counts, or rows without row_start that are not one per segment");
-  if (n_rows == 0 || n_seg == 0) return kOk;
-  if (!k->data || !v->data || !pos0 || (!write && !lens)) return set_error(kInvalidArgument, std::string(name) + ": null argument");
+  if (n_rows == 0 || (write && n_seg == 0)) return kOk;
+  if (!k->data || !v->data || (n_seg > 0 && (!pos0 || (!write && !lens)))) return set_error(kInvalidArgument, std::string(name) + ": null argument");
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
   const int size = dtype == kF32 ? 4 : 2;
@@ -570,7 +570,8 @@ static int row_launch(const char* name, bool write, mc_kv* kv, const mc_rows* k,
   };
   // Groups of slots pay once segments have more than a row: write and read of 8192 segments, 8 heads of 64,
   // in us by groups and row by row: 1 row a segment 102, 98; 1.5 rows 117, 182; 5 rows 172, 516.
-  const bool groups = start && n_rows > n_seg;
+  // (rows of no segment at all are read, as zeros, row by row)
+  const bool groups = start && n_rows > n_seg && n_seg > 0;
   long long warps = (long long)n_rows * kv->c.heads;
   int warp_heads = 1;
   if (groups) {

@@ -46,3 +46,16 @@ def test_calls_without_rows(kv):
     # and none where there is something
     assert L.mc_kv_write_dev(cache._h, r, r, 0, 1, None, None, None, 1, None) == 1
     assert L.mc_kv_attend_dev(cache._h, r, r, 0, 2, None, None, 1, 0, 1.0, None) == 1
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_of_no_segment_at_all(kv, dtype):
+    """A read of rows without any segment: all of them come back as zeros."""
+    cache = kv.KvCache(2, 2, 32, 8)
+    some = ints([0, 0])
+    out = torch.full((2, 70, 2, 32), 9.0, dtype=DTYPES[dtype], device=DEV)
+    k, v = (ctypes.byref(kv._Rows(x.data_ptr(), 64, 32)) for x in out)
+    code = {"f32": 0, "bf16": 2}[dtype]
+    assert cache._lib.mc_kv_read_dev(cache._h, k, v, code, 70, some.data_ptr(), None, some.data_ptr(), some.data_ptr(), 0, None) == 0
+    torch.cuda.synchronize()
+    assert not out.any()
