@@ -299,13 +299,15 @@ int mc_kv_open(int device, const mc_kv_spec* spec, void* memory, void* stream, m
 int mc_kv_close(mc_kv* kv);
 /* Waits for the device's work; MC_DEVICE_TIMEOUT if a kernel of this section (window attention
  * included) gave up a wait since the last check; MC_INVALID_ARGUMENT if a call on this cache named a
- * session or a position out of range (such rows are skipped, attention rows written as zero). */
+ * session, a position or a segment out of range (such rows are skipped on writes, and zeros in what
+ * reads and attention give). */
 int mc_kv_error(mc_kv* kv);
 
 /* Quantises rows into the cache. Segment b is rows [row_start[b], row_start[b+1]) and goes to
  * session sessions[b] (NULL: b) at positions pos0[b], pos0[b]+1, ...; row_start == NULL: one row
  * per segment (n_rows == n_segments). Of a segment longer than the ring only the positions that
- * stay are written. Segments of one call must not share a session's places. Arrays of the calls
+ * stay are written. Segments of one call must not share a session's places. Starts must not decrease;
+ * a segment that does not fit the n_rows rows is skipped and reported by mc_kv_error. Arrays of the calls
  * below and this one are device int32. Calls on one cache are ordered by the caller (one stream, or
  * events); no call allocates or synchronizes, so they can be captured into a graph. */
 int mc_kv_write_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int n_rows, const int32_t* row_start,
@@ -313,7 +315,7 @@ int mc_kv_write_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, in
 
 /* Reads positions back as rows, laid out like mc_kv_write_dev's: segment b's rows are positions
  * pos0[b], pos0[b]+1, ... of a session that has lens[b] positions so far. Positions that are not
- * held (past lens[b], or overwritten since) and rows of no segment come back as zeros. */
+ * held (past lens[b], or overwritten since) and rows of no segment that fits come back as zeros. */
 int mc_kv_read_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int n_rows, const int32_t* row_start,
                    const int32_t* sessions, const int32_t* pos0, const int32_t* lens, int n_segments, void* stream);
 

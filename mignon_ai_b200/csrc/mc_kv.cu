@@ -423,6 +423,15 @@ __device__ void read_group(const RowArgs& a, int row, bool mine, bool live, int 
   }
 }
 
+// Reports segments that do not fit the rows there are (a start below zero, past the rows or below the one
+// before it), of which nothing is moved; by the grid's warps together.
+__device__ __forceinline__ void check_starts(const RowArgs& a, unsigned item, unsigned warps) {
+  for (long long b = 32ll * item + (threadIdx.x & 31); b < a.n_seg; b += 32ll * warps) {
+    const int first = a.start[b], end = a.start[b + 1];
+    if (first < 0 || end < first || end > a.n_rows) atomicExch(a.c.error, 1);
+  }
+}
+
 // One warp per group of slots and a.warp_heads heads of the segments. Segment b's groups have numbers
 // from start[b] / 4 + 2b on: room for its rows / 4 + 2, and it has no more whatever its first slot.
 template <class T, bool WRITE>
@@ -432,8 +441,15 @@ __global__ void __launch_bounds__(kCacheThreads, WRITE ? (sizeof(T) == 4 ? 4 : 5
   const unsigned item = blockIdx.x * (kCacheThreads / 32) + warp;  // fewer than 2^31
   const unsigned parts = (unsigned)(a.c.heads + a.warp_heads - 1) / a.warp_heads, group = item / parts;
   const int h0 = (int)(item - group * parts) * a.warp_heads, h1 = min(h0 + a.warp_heads, a.c.heads);
-  if constexpr (!WRITE) {  // rows before the first segment and after the last come back as zeros
-    const int lo = max(0, min(a.start[0], a.n_rows)), hi = max(lo, min(a.start[a.n_seg], a.n_rows));
+  check_starts(a, item, gridDim.x * (kCacheThreads / 32));
+  if constexpr (!WRITE) {  // rows before the first segment and after the last that fit come back as zeros
+    int lo = a.start[0], hi = a.start[a.n_seg];
+    if (lo < 0) lo = a.start[last_at_most(a.n_seg, [&](int i) { return a.start[i] < 0; }) + 1];
+    if (hi > a.n_rows) {
+      const int b = last_at_most(a.n_seg, [&](int i) { return a.start[i] < a.n_rows; });
+      if (a.start[b + 1] > a.n_rows) hi = a.start[b];
+    }
+    lo = max(0, min(lo, a.n_rows)), hi = max(lo, min(hi, a.n_rows));
     for (long long e = item; e < (long long)(lo + a.n_rows - hi) * a.c.heads; e += (long long)gridDim.x * (kCacheThreads / 32)) {
       const int i = (int)(e / a.c.heads);
       read_row<T>(a, i < lo ? i : hi + i - lo, (int)(e % a.c.heads), RowPlace{0, -1});
@@ -487,6 +503,7 @@ __global__ void __launch_bounds__(kCacheThreads) single_kernel(const __grid_cons
   const int warp = threadIdx.x >> 5;
   const unsigned item = blockIdx.x * (kCacheThreads / 32) + warp;  // fewer than 2^31
   const int row = (int)(item / a.c.heads), head = (int)(item - (unsigned)row * a.c.heads);
+  if (a.start) check_starts(a, item, gridDim.x * (kCacheThreads / 32));
   if (row >= a.n_rows) return;
   RowPlace w{0, -1};
   if (!a.start) {
@@ -712,7 +729,7 @@ extern "C" int mc_kv_error(mc_kv* kv) {
   MC_CUDA(cudaMemcpy(&code, kv->c.error, sizeof(int), cudaMemcpyDeviceToHost));
   if (!code) return kOk;
   MC_CUDA(cudaMemset(kv->c.error, 0, sizeof(int)));
-  return set_error(kInvalidArgument, "mc_kv: a session or a position was out of range; its rows were skipped");
+  return set_error(kInvalidArgument, "mc_kv: a session, a position or a segment was out of range; its rows were skipped");
 }
 
 extern "C" int mc_kv_write_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int n_rows,

@@ -138,7 +138,7 @@ class KvCache:
             pass
 
     def check(self):
-        """Waits for the device and raises if a call named a session or position out of range."""
+        """Waits for the device and raises if a call named a session, a position or a segment out of range."""
         _lib.check(_lib.lib().mc_kv_error(self._h))
 
     def _segments(self, n_rows, pos0, row_start, sessions):

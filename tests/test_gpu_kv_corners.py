@@ -59,3 +59,45 @@ def test_rows_of_no_segment_at_all(kv, dtype):
     assert cache._lib.mc_kv_read_dev(cache._h, k, v, code, 70, some.data_ptr(), None, some.data_ptr(), some.data_ptr(), 0, None) == 0
     torch.cuda.synchronize()
     assert not out.any()
+
+
+@pytest.mark.parametrize("dtype,bits", [("f32", 8), ("bf16", 4)])
+@pytest.mark.parametrize("lens,n_rows", [
+    ([4, 16], 10), ([300, 40, 0, 30], 330), ([9, 5], 3), ([1, 1, 3], 3), ([1, 1, 1, 9], 4), ([7, 10 ** 9], 20)])
+def test_starts_past_the_rows(kv, dtype, bits, lens, n_rows):
+    """Starts that go beyond the rows there are: segments that fit are written and read, rows of the others
+    come back as zeros, and the cache reports it. Few and many rows a segment."""
+    heads, dim, g = 3, 48, gen(7)
+    n = len(lens)
+    start = starts(lens)
+    x = rows(g, n_rows, heads, dim, dtype)
+    cache = kv.KvCache(n, heads, dim, 301, bits=bits)
+    cache.write(x.to(DEV), x.to(DEV), ints([0] * n), ints(start))
+    with pytest.raises(Exception, match="out of range"):
+        cache.check()
+    out = tuple(torch.full((n_rows, heads, dim), 9.0, dtype=DTYPES[dtype], device=DEV) for _ in range(2))
+    cache.read(ints([0] * n), ints([300] * n), ints(start), out=out)
+    with pytest.raises(Exception, match="out of range"):
+        cache.check()
+    want = torch.zeros(x.shape)
+    for b in range(n):
+        if start[b + 1] <= n_rows:
+            want[start[b]:start[b + 1]] = ref.value(x[start[b]:start[b + 1]], bits).float()
+    for y in out:
+        assert torch.equal(y.cpu(), want.to(DTYPES[dtype]))
+
+
+@pytest.mark.parametrize("start,n_rows", [([-2, 4, 10], 10), ([-9, -1, 10], 3), ([0, 6, 3, 12], 12), ([3, 2], 5), ([3, 2], 1)])
+def test_starts_below_the_rows_or_out_of_order(kv, start, n_rows):
+    """Negative or decreasing starts are reported too."""
+    n = len(start) - 1
+    cache = kv.KvCache(n, 1, 16, 16, bits=8)
+    x = torch.randn((n_rows, 1, 16), device=DEV)
+    cache.write(x, x, ints([0] * n), ints(start))
+    with pytest.raises(Exception, match="out of range"):
+        cache.check()
+    out = (torch.full_like(x, 9.0), torch.full_like(x, 9.0))
+    cache.read(ints([0] * n), ints([0] * n), ints(start), out=out)
+    with pytest.raises(Exception, match="out of range"):
+        cache.check()
+    assert not out[0].any() and not out[1].any()  # sessions without positions: zeros, whoever's the row is
