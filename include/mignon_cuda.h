@@ -323,7 +323,7 @@ int mc_kv_read_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int
  * [n][q_heads][head_dim] belongs to session sessions[i] (NULL: i), which has lens[i] positions, the
  * query's own the last. It sees the held positions p with p < sinks or p > lens[i] - 1 - window
  * (window 0: every held one). out = softmax(scale q.k) v; query head h uses key/value head
- * h / (q_heads / heads). A row that sees nothing (lens[i] <= 0) is zero. */
+ * h / (q_heads / heads). A row that sees nothing (lens[i] <= 0) is zero. out may be q itself. */
 int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out, int dtype, int q_heads, const int32_t* sessions,
                      const int32_t* lens, int n, int window, float scale, void* stream);
 
@@ -333,8 +333,8 @@ int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out, int dtype,
  * are its last positions: query t of nq is position nk - nq + t. It sees keys j <= position with
  * j < sinks or j > position - window (window 0: all of them). A row that sees nothing is zero;
  * rows outside every segment are not written; a segment whose bounds leave the n_q or n_k rows is
- * skipped. q_start and k_start NULL: one segment of all rows. head_dim 1 to 256. Runs on the
- * current device. */
+ * skipped. q_start and k_start NULL: one segment of all rows. head_dim 1 to 256. out may be q itself,
+ * and shares no memory with k and v. Runs on the current device. */
 int mc_window_attn_dev(const mc_rows* q, const mc_rows* k, const mc_rows* v, const mc_rows* out, int dtype, int q_heads,
                        int kv_heads, int head_dim, int n_q, int n_k, const int32_t* q_start, const int32_t* k_start,
                        int n_segments, int window, int sinks, float scale, void* stream);

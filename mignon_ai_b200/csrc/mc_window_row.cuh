@@ -26,15 +26,15 @@ __device__ __forceinline__ int window_begin(int window, int pos) {
 }
 
 // One query row by one warp, key by key: lane j scores keys j, j + 32, ..; then the lanes own
-// dimensions. Masked keys and values are not read, so whatever they hold reaches nothing.
-template <class T>
-__device__ void row_attention(const Args& a, int row, int h, int k0, int pos, float* qs) {
+// dimensions. Masked keys and values are not read, so whatever they hold reaches nothing. query(d): element
+// d of the row's query, all read before anything is stored.
+template <class T, class Q>
+__device__ void row_attention(const Args& a, int row, int h, int k0, int pos, float* qs, Q query) {
   const int lane = threadIdx.x & 31, dim = a.dim, hk = h / a.group;
-  const T* q = static_cast<const T*>(a.q.p) + row * a.q.row + h * a.q.head;
   T* out = static_cast<T*>(a.out.p) + row * a.out.row + h * a.out.head;
   const T* k = static_cast<const T*>(a.k.p) + k0 * a.k.row + hk * a.k.head;
   const T* v = static_cast<const T*>(a.v.p) + k0 * a.v.row + hk * a.v.head;
-  for (int d = lane; d < dim; d += 32) qs[d] = to_float<T>(q[d]);
+  for (int d = lane; d < dim; d += 32) qs[d] = to_float<T>(query(d));
   __syncwarp();
   const int lo = window_begin(a.window, pos);
   const int sink_end = min(a.sinks, lo);                        // visible keys before it
@@ -82,6 +82,12 @@ __device__ void row_attention(const Args& a, int row, int h, int k0, int pos, fl
     const int d = lane + 32 * u;
     if (d < dim) out[d] = from_float<T>(total == 0.f ? 0.f : __fdiv_rn(acc[u], total));
   }
+}
+
+template <class T>
+__device__ void row_attention(const Args& a, int row, int h, int k0, int pos, float* qs) {
+  const T* q = static_cast<const T*>(a.q.p) + row * a.q.row + h * a.q.head;
+  row_attention<T>(a, row, h, k0, pos, qs, [&](int d) { return q[d]; });
 }
 
 // The segment of row r: the last b with start[b] <= r (null starts: one row per segment), or -1.

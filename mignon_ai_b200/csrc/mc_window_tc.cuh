@@ -289,10 +289,16 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     meet();  // also orders the row's stores before those of a second computation
     if (ok && half == 0) {
       uint32_t again = __ballot_sync(~0u, real && !(exchange[1][0][my_row] == 0.f && exchange[1][1][my_row] == 0.f));
+      // the queries from their tile: outputs may be in place of them. The copy has long landed; this wait is
+      // for its bytes to be seen by this warp.
+      if (again && !__all_sync(~0u, mbar_wait_or_abort(q_full, 0, kErrWaitFull))) again = 0;
       while (again) {
         const int l = __ffs(again) - 1, r = 32 * warp + l;
         again &= again - 1;
-        row_attention<T>(a, seg.q0 + first + r / a.group, hk * a.group + r % a.group, seg.k0, pos0 + r / a.group, redo[warp]);
+        auto query = [&](int d) {
+          return *reinterpret_cast<const T*>(sq + (d >> 6) * kTcBlock + 128 * r + ((((d >> 3) & 7) ^ (r & 7)) << 4) + 2 * (d & 7));
+        };
+        row_attention<T>(a, seg.q0 + first + r / a.group, hk * a.group + r % a.group, seg.k0, pos0 + r / a.group, redo[warp], query);
         __syncwarp();
       }
     }

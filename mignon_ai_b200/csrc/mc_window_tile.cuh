@@ -297,7 +297,8 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
     __syncthreads();
     load(step + 1, true);
   }
-  // ---- the output rows: o[d][2e + u] is row e, dimension 8d + 2c + u
+  // ---- the output rows: o[d][2e + u] is row e, dimension 8d + 2c + u. A row that is not all finite is not
+  // stored: outputs may be in place of the queries, which its second computation reads.
   uint32_t again[2];
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
@@ -306,20 +307,26 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
     sum = __fadd_rn(sum, __shfl_xor_sync(~0u, sum, 2));
     const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.0f, sum);
     float bad = __fmul_rn(sum, 0.f);
+#pragma unroll
+    for (int d = 0; d < DIMP / 8; ++d) {  // NaN once a value is not finite
+      o[d][2 * e] = __fmul_rn(o[d][2 * e], inv);
+      o[d][2 * e + 1] = __fmul_rn(o[d][2 * e + 1], inv);
+      bad = __fmaf_rn(o[d][2 * e], 0.f, __fmaf_rn(o[d][2 * e + 1], 0.f, bad));
+    }
+    again[e] = __ballot_sync(~0u, real[e] && !(bad == 0.f));
+    const bool store = real[e] && !(again[e] & (0xFu << (lane & ~3)));
     T* out = static_cast<T*>(a.out.p) + row[e] * a.out.row + (long long)(hk * a.group + head[e]) * a.out.head;
 #pragma unroll
     for (int d = 0; d < DIMP / 8; ++d) {
-      const float x = __fmul_rn(o[d][2 * e], inv), y = __fmul_rn(o[d][2 * e + 1], inv);
+      const float x = o[d][2 * e], y = o[d][2 * e + 1];
       const int at = 8 * d + 2 * c;
-      bad = __fmaf_rn(x, 0.f, __fmaf_rn(y, 0.f, bad));  // NaN once a value is not finite
-      if (real[e] && args.pairs) {
+      if (store && args.pairs) {
         if (at < a.dim) store_pair<T>(out + at, x, y);
-      } else if (real[e]) {
+      } else if (store) {
         if (at < a.dim) out[at] = from_float<T>(x);
         if (at + 1 < a.dim) out[at + 1] = from_float<T>(y);
       }
     }
-    again[e] = __ballot_sync(~0u, real[e] && !(bad == 0.f));
   }
   // a non-finite row may have met a hidden key's infinity or NaN times its weight of zero: key by key
 #pragma unroll

@@ -101,3 +101,32 @@ def test_starts_below_the_rows_or_out_of_order(kv, start, n_rows):
     with pytest.raises(Exception, match="out of range"):
         cache.check()
     assert not out[0].any() and not out[1].any()  # sessions without positions: zeros, whoever's the row is
+
+
+@pytest.mark.parametrize("dtype,dim,group", [("f32", 64, 2), ("bf16", 64, 2), ("f16", 128, 3), ("f16", 24, 2), ("f32", 192, 2),
+                                             ("bf16", 64, 1)])
+def test_outputs_in_place_of_the_queries(kv, dtype, dim, group):
+    """out=q, with a hidden NaN and infinity that make rows be computed a second time, and a visible one."""
+    g, n, heads = gen(dim), 300, 2
+    q = torch.randn((n, heads * group, dim), generator=g).to(DTYPES[dtype]).to(DEV)
+    k, v = rows(g, n, heads, dim, dtype), rows(g, n, heads, dim, dtype)
+    v[100, 0] = float("nan")
+    v[150, 1, 3] = float("inf")
+    k[290, 1] = float("nan")
+    want = kv.window_attention(q, k.to(DEV), v.to(DEV), window=20, sinks=2)
+    kv.window_attention(q, k.to(DEV), v.to(DEV), window=20, sinks=2, out=q)
+    bad = want.isnan()
+    assert bad[100:120, :group].all() and not bad[120:, :group].any() and not bad[:100].any() and bad[290:, group:].all()
+    assert torch.equal(q.isnan(), bad) and torch.equal(q.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("slots", [70, 9000])
+def test_attend_in_place_of_the_queries(kv, slots):
+    g = gen(slots)
+    cache = kv.KvCache(3, 2, 64, slots, bits=8)
+    k = rows(g, 3 * slots, 2, 64, "bf16").to(DEV)
+    cache.write(k, k.flip(0), ints([0] * 3), ints([0, slots, 2 * slots, 3 * slots]))
+    q = torch.randn((3, 10, 64), generator=g).bfloat16().to(DEV)
+    lens = ints([slots, slots // 2, 1])
+    want = cache.attend(q, lens)
+    assert cache.attend(q, lens, out=q) is q and torch.equal(q, want)
