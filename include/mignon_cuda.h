@@ -297,8 +297,9 @@ int mc_kv_bytes(const mc_kv_spec* spec, size_t* bytes);
 int mc_kv_open(int device, const mc_kv_spec* spec, void* memory, void* stream, mc_kv** out);
 /* Closes the cache; memory of the library's is freed once the device's work is done. */
 int mc_kv_close(mc_kv* kv);
-/* Waits for the device's work; MC_DEVICE_TIMEOUT if a kernel of this section (window attention
- * included) gave up a wait since the last check; MC_INVALID_ARGUMENT if a call on this cache named a
+/* Waits for the device's work; MC_DEVICE_TIMEOUT if a kernel of this section (window attention and
+ * other caches of the device included) gave up a wait since the last check, by whichever of
+ * mc_kv_error and mc_window_error; MC_INVALID_ARGUMENT if a call on this cache named a
  * session, a position or a segment out of range (such rows are skipped on writes, and zeros in what
  * reads and attention give). */
 int mc_kv_error(mc_kv* kv);
@@ -333,11 +334,14 @@ int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out, int dtype,
  * are its last positions: query t of nq is position nk - nq + t. It sees keys j <= position with
  * j < sinks or j > position - window (window 0: all of them). A row that sees nothing is zero;
  * rows outside every segment are not written; a segment whose bounds leave the n_q or n_k rows is
- * skipped. q_start and k_start NULL: one segment of all rows. head_dim 1 to 256. out may be q itself,
+ * skipped and reported by mc_window_error. Starts must not decrease. q_start and k_start NULL: one segment of all rows. head_dim 1 to 256. out may be q itself,
  * and shares no memory with k and v. Runs on the current device. */
 int mc_window_attn_dev(const mc_rows* q, const mc_rows* k, const mc_rows* v, const mc_rows* out, int dtype, int q_heads,
                        int kv_heads, int head_dim, int n_q, int n_k, const int32_t* q_start, const int32_t* k_start,
                        int n_segments, int window, int sinks, float scale, void* stream);
+/* Waits for `device`'s work; MC_DEVICE_TIMEOUT as mc_kv_error, without a cache; MC_INVALID_ARGUMENT if
+ * mc_window_attn_dev was given a segment out of range there since the last check. */
+int mc_window_error(int device);
 
 /* The int8 rate of this device's tensor pipe, the denominator of the INT8 roofline fractions (no
  * counterpart in the reference: a measurement). One CTA per multiprocessor issues back-to-back
@@ -352,6 +356,9 @@ int mc_probe_mma_i8(int device, int iters, int launches, double* tops, double* m
  * device error word and returns. Returns MC_DEVICE_TIMEOUT (any other status means the path is
  * broken); the device stays usable afterwards. */
 int mc_selftest_wait_timeout(int device);
+/* The same for the kernels of the key/value cache and window attention, whose error word it leaves set
+ * for mc_kv_error or mc_window_error to report. */
+int mc_selftest_kv_wait_timeout(int device);
 
 /* The CUDA stream (cudaStream_t) the batch's work on device shard `shard` runs on. */
 int mc_batch_stream(mc_batch* batch, int shard, void** stream);

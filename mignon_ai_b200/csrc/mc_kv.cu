@@ -712,6 +712,44 @@ extern "C" int mc_kv_close(mc_kv* kv) {
   return kOk;
 }
 
+namespace mc {
+namespace kv {
+
+// Reads and clears the current device's error word of this unit's kernels, whose work is done. While it is set, waits
+// that take long give up early.
+static int take_timeout() {
+  int code = 0;
+  MC_CUDA(cudaMemcpyFromSymbol(&code, g_device_error, sizeof(int)));
+  if (!code) return kOk;
+  const int zero = 0;
+  MC_CUDA(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)));
+  MC_CUDA(cudaDeviceSynchronize());
+  return set_error(kDeviceTimeout, "device wait gave up (code " + std::to_string(code) + "); the kernel returned without finishing its work");
+}
+
+// As the engine's, for this unit's error word, which stays set.
+__global__ void selftest_wait_kernel() {
+  __shared__ uint64_t bar;
+  if (threadIdx.x != 0) return;
+  mbar_init(&bar, 1);
+  fence_barrier_init();
+  mbar_wait(&bar, 0, kErrWaitFull);  // phase 0 never completes
+}
+
+}  // namespace kv
+}  // namespace mc
+
+extern "C" int mc_selftest_kv_wait_timeout(int device) {
+  using namespace mc;
+  clear_error();
+  DeviceRestore restore_device;
+  MC_CUDA(cudaSetDevice(device));
+  kv::selftest_wait_kernel<<<1, 32>>>();
+  MC_CUDA(cudaGetLastError());
+  MC_CUDA(cudaDeviceSynchronize());
+  return kOk;
+}
+
 extern "C" int mc_kv_error(mc_kv* kv) {
   using namespace mc;
   clear_error();
@@ -719,16 +757,13 @@ extern "C" int mc_kv_error(mc_kv* kv) {
   DeviceRestore restore_device;
   MC_CUDA(cudaSetDevice(kv->device));
   MC_CUDA(cudaDeviceSynchronize());
+  const int st = kv::take_timeout();
+  if (st != kOk) return st;
   int code = 0;
-  MC_CUDA(cudaMemcpyFromSymbol(&code, g_device_error, sizeof(int)));
-  if (code) {
-    const int zero = 0;
-    MC_CUDA(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)));
-    return set_error(kDeviceTimeout, "device wait gave up (code " + std::to_string(code) + "); the kernel returned without finishing its work");
-  }
   MC_CUDA(cudaMemcpy(&code, kv->c.error, sizeof(int), cudaMemcpyDeviceToHost));
   if (!code) return kOk;
   MC_CUDA(cudaMemset(kv->c.error, 0, sizeof(int)));
+  MC_CUDA(cudaDeviceSynchronize());  // before what other streams do next
   return set_error(kInvalidArgument, "mc_kv: a session, a position or a segment was out of range; its rows were skipped");
 }
 

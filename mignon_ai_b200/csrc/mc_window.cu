@@ -18,6 +18,7 @@ constexpr int kWindowRowThreads = 256;
 template <class T>
 __global__ void __launch_bounds__(kWindowRowThreads) row_kernel(const __grid_constant__ Args a) {
   __shared__ float qs[kWindowRowThreads / 32][kMaxDim];
+  check_segments(a);
   const int warp = threadIdx.x >> 5;
   const long long item = (long long)blockIdx.x * (kWindowRowThreads / 32) + warp;
   const int row = (int)(item / a.q_heads), h = (int)(item % a.q_heads);
@@ -85,6 +86,23 @@ static int tile_launch(const Args& a, cudaStream_t stream) {
 
 }  // namespace win
 }  // namespace mc
+
+extern "C" int mc_window_error(int device) {
+  using namespace mc;
+  clear_error();
+  DeviceRestore restore_device;
+  MC_CUDA(cudaSetDevice(device));
+  MC_CUDA(cudaDeviceSynchronize());
+  const int st = kv::take_timeout();
+  if (st != kOk) return st;
+  int code = 0;
+  MC_CUDA(cudaMemcpyFromSymbol(&code, win::g_window_bounds, sizeof(int)));
+  if (!code) return kOk;
+  const int zero = 0;
+  MC_CUDA(cudaMemcpyToSymbol(win::g_window_bounds, &zero, sizeof(int)));
+  MC_CUDA(cudaDeviceSynchronize());
+  return set_error(kInvalidArgument, "mc_window_attn_dev: a segment was out of range; its rows were skipped");
+}
 
 extern "C" int mc_window_attn_dev(const mc_rows* q, const mc_rows* k, const mc_rows* v, const mc_rows* out, int dtype,
                                   int q_heads, int kv_heads, int head_dim, int n_q, int n_k, const int32_t* q_start,

@@ -106,9 +106,10 @@ __device__ __forceinline__ int segment_of(const int* start, int n, int r) {
 // The segment's queries and keys, with its bounds checked against the rows there are.
 struct Segment {
   int q0, nq, k0, nk;
+  bool fits;
 };
 __device__ __forceinline__ Segment segment(const Args& a, int b) {
-  Segment s{0, a.n_q, 0, a.n_k};
+  Segment s{0, a.n_q, 0, a.n_k, true};
   if (a.q_start) {
     s.q0 = a.q_start[b];
     s.nq = a.q_start[b + 1] - s.q0;
@@ -117,8 +118,19 @@ __device__ __forceinline__ Segment segment(const Args& a, int b) {
     s.k0 = a.k_start[b];
     s.nk = a.k_start[b + 1] - s.k0;
   }
-  if (s.q0 < 0 || s.nq < 0 || s.nq > a.n_q - s.q0 || s.k0 < 0 || s.nk < 0 || s.nk > a.n_k - s.k0) s = Segment{0, 0, 0, 0};
+  if (s.q0 < 0 || s.nq < 0 || s.nq > a.n_q - s.q0 || s.k0 < 0 || s.nk < 0 || s.nk > a.n_k - s.k0) s = Segment{0, 0, 0, 0, false};
   return s;
+}
+
+// Set once a segment did not fit (read and cleared by mc_window_error).
+static __device__ int g_window_bounds = 0;
+
+// Reports the segments that do not fit, of which no row is computed; by the grid's first row of blocks together.
+// A call: in line it made the tcgen05 kernel spill in its loop.
+__device__ __noinline__ void check_segments(const Args& a) {
+  if (!a.q_start || blockIdx.y) return;
+  for (long long b = (long long)blockIdx.x * blockDim.x + threadIdx.x; b < a.n_seg; b += (long long)gridDim.x * blockDim.x)
+    if (!segment(a, (int)b).fits) atomicExch(&g_window_bounds, 1);
 }
 
 // The tiled kernels hand out tiles of tt tokens so that segment b's begin at start[b] / tt + b: each

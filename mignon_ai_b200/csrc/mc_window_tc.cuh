@@ -75,6 +75,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
   uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 2, *s_full = bars + 3, *p_full = bars + 4,
            *o_full = bars + 5, *v_free = bars + 6;
 
+  check_segments(a);
   const int tile_id = gridDim.x - 1 - blockIdx.x, hk = blockIdx.y, tt = args.tokens;
   const int b = a.q_start ? tile_segment(a.q_start, a.n_seg, tt, tile_id) : 0;
   const Segment seg = segment(a, b);

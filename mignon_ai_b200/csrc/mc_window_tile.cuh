@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
   float* sv = sk + kTileKeys * SK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
 
+  check_segments(a);
   const int tt = kTileRows / a.group, tile_id = gridDim.x - 1 - blockIdx.x;
   const int h0 = blockIdx.y * args.heads, n_heads = min(args.heads, a.heads - h0);
   const int b = a.q_start ? tile_segment(a.q_start, a.n_seg, tt, tile_id) : 0;

@@ -12,7 +12,8 @@ All four share one mask: a query at position p sees the positions j <= p with j 
 j > p - window (window 0: every one), as far as the cache still holds them. Rows are
 ``[rows, heads, head_dim]`` float32, float16 or bfloat16 tensors; ragged segments are given by int32
 device tensors of their first rows (n + 1 of them). Calls go to the current stream of the tensors'
-device, allocate at most their output and never synchronize. There is no CPU path.
+device, allocate at most their output and never synchronize; ``KvCache.check`` and ``check`` do, and
+raise what the kernels found. There is no CPU path.
 """
 from __future__ import annotations
 
@@ -42,6 +43,7 @@ _lib.register({
     "mc_kv_open": [_i, ctypes.POINTER(_Spec), c_vp, c_vp, ctypes.POINTER(c_vp)],
     "mc_kv_close": [c_vp],
     "mc_kv_error": [c_vp],
+    "mc_window_error": [_i],
     "mc_kv_write_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, c_vp, _i, c_vp],
     "mc_kv_read_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, c_vp, c_vp, _i, c_vp],
     "mc_kv_attend_dev": [c_vp, c_vp, c_vp, _i, _i, c_vp, c_vp, _i, _i, ctypes.c_float, c_vp],
@@ -138,7 +140,8 @@ class KvCache:
             pass
 
     def check(self):
-        """Waits for the device and raises if a call named a session, a position or a segment out of range."""
+        """Waits for the device and raises if a call named a session, a position or a segment out of range,
+        or a kernel gave up a wait."""
         _lib.check(_lib.lib().mc_kv_error(self._h))
 
     def _segments(self, n_rows, pos0, row_start, sessions):
@@ -212,13 +215,20 @@ class KvCache:
         return out
 
 
+def check(device: Optional[int] = None):
+    """Waits for the device (default: the current one) and raises if ``window_attention`` was given a
+    segment out of range there, or a kernel of this module gave up a wait, since the last check."""
+    _lib.check(_lib.lib().mc_window_error(torch.cuda.current_device() if device is None else device))
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: Optional[torch.Tensor] = None,
                      k_start: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of ragged segments: queries [q_start[b], q_start[b+1]) of q [rows, q_heads,
     head_dim] over keys [k_start[b], k_start[b+1]) of k and v [rows, heads, head_dim]. A segment's
     queries are its last positions (k_start defaults to q_start; both None: one segment). A row
-    that sees nothing is zero; rows of no segment are not written."""
+    that sees nothing is zero; rows of no segment are not written, nor those of a segment out of
+    range, which ``check`` reports."""
     index, dim, dtype, s = q.get_device(), q.shape[-1], q.dtype, _scratch
     if index < 0:
         raise ValueError("q: expected a CUDA tensor")

@@ -1,5 +1,6 @@
 """Corner calls of the quantised key/value cache and window attention, against plain 64-bit
 restatements. Tolerances are those of the ordinary cases unless a test derives its own."""
+import contextlib
 import ctypes
 
 import pytest
@@ -130,3 +131,55 @@ def test_attend_in_place_of_the_queries(kv, slots):
     lens = ints([slots, slots // 2, 1])
     want = cache.attend(q, lens)
     assert cache.attend(q, lens, out=q) is q and torch.equal(q, want)
+
+
+def test_window_segments_out_of_range_are_reported(kv):
+    """Bad starts of window attention: skipped, and reported by a check that needs no cache, once."""
+    x = {d: torch.randn((20, 1, d), device=DEV) for d in (64, 192)}
+    with contextlib.suppress(Exception):
+        kv.check()  # of what ran before
+    for dim, dtype in ((64, torch.float32), (64, torch.bfloat16), (192, torch.float32)):
+        y = x[dim].to(dtype)
+        for q_start, k_start in (([0, 10, 20], [0, 10, 21]), ([0, 10, 21], [0, 10, 20]), ([-1, 10, 20], [0, 10, 20]),
+                                 ([0, 12, 10], [0, 10, 20]), ([0] * 999 + [25], [0] * 999 + [20])):
+            kv.window_attention(y, y, y, ints(q_start), ints(k_start))
+            with pytest.raises(Exception, match="out of range"):
+                kv.check()
+            kv.check()
+        kv.window_attention(y, y, y, ints([0, 10, 20]), ints([0, 10, 20]))
+        kv.check(0)
+    # a cache's own check is about its own indexes
+    cache = kv.KvCache(1, 1, 64, 4)
+    kv.window_attention(x[64], x[64], x[64], ints([0, 21]))
+    cache.check()
+    with pytest.raises(Exception, match="out of range"):
+        kv.check()
+
+
+def test_a_wait_that_ran_out_is_reported_and_cleared(kv):
+    """The error word of a wait that gave up: reported once, with or without a cache, and what is computed after
+    the report is what it was before. A call in between may give up, but ends."""
+    L, g = cache_lib(), gen(21)
+    q = torch.randn((2000, 8, 128), generator=g).bfloat16().to(DEV)
+    k, v = rows(g, 2000, 2, 128, "bf16").to(DEV), rows(g, 2000, 2, 128, "bf16").to(DEV)
+    cache = kv.KvCache(1, 2, 128, 2000, bits=4)
+    cache.write(k, v, ints([0]), ints([0, 2000]))
+    lens = ints([2000])
+    calls = lambda: (kv.window_attention(q, k, v), cache.attend(q[:1], lens))
+    before = calls()
+    for check in (kv.check, cache.check):
+        assert L.mc_selftest_kv_wait_timeout(0) == 0
+        calls()
+        with pytest.raises(Exception, match="gave up"):
+            check()
+        check()
+        assert all(torch.equal(x, y) for x, y in zip(before, calls()))
+        kv.check()
+
+
+def cache_lib():
+    from mignon_ai_b200 import _lib
+    L = _lib.lib()
+    L.mc_selftest_kv_wait_timeout.restype = ctypes.c_int
+    L.mc_selftest_kv_wait_timeout.argtypes = [ctypes.c_int]
+    return L
