@@ -8,7 +8,9 @@
 // The running maximum m is only raised when a row's tile maximum exceeds it by more than 8 (in
 // log2): until then the weights are at most 2^8 and nothing has to be rescaled; a raise rescales
 // O in TMEM. Weights are rounded to the operands' type for the product (as the output is), their sum
-// is not.
+// is not. Float16 weights, and their sum with them, are 2^7 times as large, up to 2^15: so those down to 2^-21
+// of the maximum keep all their bits and those below 2^-32 of it are lost, not 2^-14 and 2^-25, which many
+// small ones behind one large would show.
 //
 // Two CTAs share an SM (96 KB of operands and 256 TMEM columns each), so one's products run
 // under the other's exponentials: per tile the tensor pipe needs about 1000 cycles at dim 128 and
@@ -177,6 +179,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     const int lo = window_begin(a.window, pos);
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
     const int c0 = 64 * half;  // this thread's keys of a tile
+    constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
     auto meet = []() { asm volatile("bar.sync 1, 256;" ::: "memory"); };  // the softmax warps
     float top = -INFINITY;
     float2 total = make_float2(0.f, 0.f);
@@ -226,7 +229,7 @@ tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
         }
       }
       if (ok) {
-        const float shift = top == -INFINITY ? 0.f : top;
+        const float shift = top == -INFINITY ? 0.f : top - kLift;
         const float2 shift2 = make_float2(-shift, -shift);
 #pragma unroll
         for (int c = 0; c < 64; c += 32) {

@@ -183,3 +183,21 @@ def cache_lib():
     L.mc_selftest_kv_wait_timeout.restype = ctypes.c_int
     L.mc_selftest_kv_wait_timeout.argtypes = [ctypes.c_int]
     return L
+
+
+@pytest.mark.parametrize("dtype,most", [("f16", 2.0 ** -8), ("bf16", 2.0 ** -7)])
+@pytest.mark.parametrize("at", [0, 40000, 65536])
+def test_window_small_weights_add_up(kv, dtype, most, at):
+    """One key far above 65,536 others of equal weight, exp(-16.25) of its own or 1.47 * 2^-24, whose share of
+    the output is 0.0057. A float16 weight may be off by 2^-25 of 2^7 times its maximum's, 0.27 % of such a
+    weight, and the output by 2^-11 of itself; bfloat16 ones by 2^-9 and 2^-9."""
+    n, dim = 65537, 64
+    q, k, v = torch.zeros((3, 1, dim)), torch.zeros((n, 1, dim)), torch.ones((n, 1, dim))
+    q[..., 5] = 1
+    k[at, 0, 5] = 16.25
+    v[at] = 0
+    t = DTYPES[dtype]
+    got = kv.window_attention(q.to(t).to(DEV), k.to(t).to(DEV), v.to(t).to(DEV), ints([0, 3]), ints([0, n]), scale=1.0)[-1]
+    share = 65536 * torch.exp(torch.tensor(-16.25, dtype=torch.float64))
+    want = share / (1 + share)
+    assert (got.double().cpu() - want).abs().max() <= most * want
