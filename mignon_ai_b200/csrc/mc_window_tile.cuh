@@ -42,7 +42,8 @@ __device__ __forceinline__ void cut(float x, uint32_t& hi, uint32_t& lo) {
   lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
 }
 // The A operands, fewer than B's, are cut to nearest: their low parts then have either sign, and the
-// low-by-low products that are left out no longer add up.
+// low-by-low products that are left out no longer add up. The carry turns a NaN's high part into anything: its low
+// part is NaN, and where that is not used something else has to be (a row's sum, for weights).
 __device__ __forceinline__ void cut_nearest(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
   lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
@@ -216,8 +217,12 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
         for (int e = 0; e < 2; ++e) {
           const float2 q = *reinterpret_cast<const float2*>(&sq[(16 * warp + r + 8 * e) * SK + 8 * k + 2 * c]);
           // 16-bit values stay exact in tf32: their scores are scaled instead
-          cut_nearest(PRODUCTS == 3 ? __fmul_rn(q.x, a.scale) : q.x, ah[e], al[e]);
-          cut_nearest(PRODUCTS == 3 ? __fmul_rn(q.y, a.scale) : q.y, ah[2 + e], al[2 + e]);
+          if constexpr (PRODUCTS == 3) {
+            cut_nearest(__fmul_rn(q.x, a.scale), ah[e], al[e]);
+            cut_nearest(__fmul_rn(q.y, a.scale), ah[2 + e], al[2 + e]);
+          } else {  // nothing to cut
+            ah[e] = __float_as_uint(q.x), ah[2 + e] = __float_as_uint(q.y);
+          }
         }
         float x[4][2];
 #pragma unroll

@@ -201,3 +201,17 @@ def test_window_small_weights_add_up(kv, dtype, most, at):
     share = 65536 * torch.exp(torch.tensor(-16.25, dtype=torch.float64))
     want = share / (1 + share)
     assert (got.double().cpu() - want).abs().max() <= most * want
+
+
+@pytest.mark.parametrize("dtype,dim", [("f16", 24), ("bf16", 24), ("f32", 24), ("f16", 64), ("bf16", 64), ("f32", 64), ("f32", 192)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_window_queries_that_are_not_finite(kv, dtype, dim, what):
+    """A NaN among a query's elements, or an infinity that meets a positive key, makes its row NaN, and no other."""
+    g = gen(3)
+    q = torch.randn((90, 2, dim), generator=g).to(DTYPES[dtype])
+    k, v = rows(g, 90, 1, dim, dtype).abs() + 1, rows(g, 90, 1, dim, dtype)
+    q[7, 0, 2] = q[70, 1, dim - 1] = what
+    got = kv.window_attention(q.to(DEV), k.to(DEV), v.to(DEV))
+    bad = torch.zeros((90, 2), dtype=torch.bool)
+    bad[7, 0] = bad[70, 1] = True
+    assert torch.equal(got.isnan().all(-1).cpu(), bad) and torch.equal(got.isnan().any(-1).cpu(), bad)
