@@ -340,22 +340,34 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM, PLANES)) a
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          qsum = __fadd_rn(qsum, x[i][e]);
-          big = fmaxf(big, fabsf(x[i][e]));
-        }
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[i][e]));
 #pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        qsum = __fadd_rn(qsum, __shfl_xor_sync(~0u, qsum, x));
-        big = fmaxf(big, __shfl_xor_sync(~0u, big, x));
+      for (int x = 1; x <= 2; x <<= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, x));
+      // rows near the ends of float32's range, whose sum or inverse would leave it, move to its middle by a
+      // power of two, and their scale back
+      float scale = a.scale;
+      if (__any_sync(~0u, big > 0x1p100f || (big < 0x1p-60f && big > 0.f))) {
+        const bool up = big < 0x1p-60f, down = big > 0x1p100f;
+        const float lift = up ? 0x1p64f : down ? 0x1p-64f : 1.f;
+        scale = __fmul_rn(scale, up ? 0x1p-64f : down ? 0x1p64f : 1.f);
+        big = __fmul_rn(big, lift);
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[i][e] = __fmul_rn(x[i][e], lift);
       }
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qsum = __fadd_rn(qsum, x[i][e]);
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) qsum = __fadd_rn(qsum, __shfl_xor_sync(~0u, qsum, x));
       // n = q / step in 16 or 23 bits, cut into signed bytes: adding 0x80 to the lower ones carries into
       // the next what a byte above 127 stands for. 1.5 * 2^23 leaves n in the mantissa's low bits.
       constexpr float kMost = PLANES == 3 ? 4161000.0f : 32600.0f, kBias = PLANES == 3 ? 32896.0f : 128.0f;
-      // below 1e-30 the inverse leaves float32's range: such a row counts as zeros; a non-finite query has
-      // no digits: its scores become NaN by qsum
-      const float inv = big >= 1e-30f ? __fdividef(kMost, big) : 0.f;
-      qstep = __fmul_rn(big >= 1e-30f ? __fmul_rn(big, 1.0f / kMost) : 0.f, __fmul_rn(a.scale, kOne));
+      // a row of zeros has no inverse; a non-finite query has no digits: its scores become NaN by qsum
+      const float inv = big > 0.f ? __fdividef(kMost, big) : 0.f;
+      qstep = __fmul_rn(__fmul_rn(big, 1.0f / kMost), __fmul_rn(scale, kOne));
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -373,7 +385,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM, PLANES)) a
             qa[i][0][e] = ((hi | 0x80808080u) - 0x40404040u) ^ 0x80808080u;
           }
         }
-      qsum = __fmul_rn(qsum, a.scale);
+      qsum = __fmul_rn(qsum, scale);
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i] = make_float2(0.f, 0.f);

@@ -215,3 +215,21 @@ def test_window_queries_that_are_not_finite(kv, dtype, dim, what):
     bad = torch.zeros((90, 2), dtype=torch.bool)
     bad[7, 0] = bad[70, 1] = True
     assert torch.equal(got.isnan().all(-1).cpu(), bad) and torch.equal(got.isnan().any(-1).cpu(), bad)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("q_size,k_size", [(3e38, 1e-25), (5e37, 1e-20), (1e-36, 1e20), (1e-42, 1e25)])
+def test_attend_queries_of_any_size(kv, dtype, bits, q_size, k_size):
+    """Queries near the ends of the type's range, with keys and a scale that bring the scores back to a few."""
+    g, n, dim, group = gen(5), 150, 64, 3
+    q = (torch.rand((1, group, dim), generator=g).double() * 2 - 1).mul(q_size).to(DTYPES[dtype])
+    k = rows(g, n, 1, dim, dtype, size=k_size)
+    v = rows(g, n, 1, dim, dtype)
+    cache = kv.KvCache(1, 1, dim, n, bits=bits)
+    cache.write(k.to(DEV), v.to(DEV), ints([0]), ints([0, n]))
+    scale = 0.1 / (q_size * k_size)
+    got = cache.attend(q.to(DEV), ints([n]), scale=scale)
+    scale = torch.tensor(scale, dtype=torch.float32).double().item()  # as the call takes it
+    want = ref.attention(q[0], ref.value(k, bits)[:, 0], ref.value(v, bits)[:, 0], torch.ones((group, n), dtype=torch.bool), scale)
+    close(got[0], want, v.float().abs().max().item(), dtype)
