@@ -324,7 +324,8 @@ int mc_kv_read_dev(mc_kv* kv, const mc_rows* k, const mc_rows* v, int dtype, int
  * [n][q_heads][head_dim] belongs to session sessions[i] (NULL: i), which has lens[i] positions, the
  * query's own the last. It sees the held positions p with p < sinks or p > lens[i] - 1 - window
  * (window 0: every held one). out = softmax(scale q.k) v; query head h uses key/value head
- * h / (q_heads / heads). A row that sees nothing (lens[i] <= 0) is zero. out may be q itself. */
+ * h / (q_heads / heads). scale must be positive. A row that sees nothing (lens[i] <= 0) is zero; one
+ * whose query is not all finite is NaN. out may be q itself. */
 int mc_kv_attend_dev(mc_kv* kv, const mc_rows* q, const mc_rows* out, int dtype, int q_heads, const int32_t* sessions,
                      const int32_t* lens, int n, int window, float scale, void* stream);
 

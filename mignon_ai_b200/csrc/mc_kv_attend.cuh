@@ -365,9 +365,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, attend_ctas(DIM, PLANES)) a
       // n = q / step in 16 or 23 bits, cut into signed bytes: adding 0x80 to the lower ones carries into
       // the next what a byte above 127 stands for. 1.5 * 2^23 leaves n in the mantissa's low bits.
       constexpr float kMost = PLANES == 3 ? 4161000.0f : 32600.0f, kBias = PLANES == 3 ? 32896.0f : 128.0f;
-      // a row of zeros has no inverse; a non-finite query has no digits: its scores become NaN by qsum
+      // a row of zeros has no inverse; a query that is not all finite has no digits: its scores are NaN, by the
+      // sum that holds a NaN, or by the step where there are infinities (whose signs the digits do not know)
       const float inv = big > 0.f ? __fdividef(kMost, big) : 0.f;
-      qstep = __fmul_rn(__fmul_rn(big, 1.0f / kMost), __fmul_rn(scale, kOne));
+      qstep = big < INFINITY ? __fmul_rn(__fmul_rn(big, 1.0f / kMost), __fmul_rn(scale, kOne)) : __int_as_float(0x7FFF0000);
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll

@@ -233,3 +233,22 @@ def test_attend_queries_of_any_size(kv, dtype, bits, q_size, k_size):
     scale = torch.tensor(scale, dtype=torch.float32).double().item()  # as the call takes it
     want = ref.attention(q[0], ref.value(k, bits)[:, 0], ref.value(v, bits)[:, 0], torch.ones((group, n), dtype=torch.bool), scale)
     close(got[0], want, v.float().abs().max().item(), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [1, 3, 8])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_attend_queries_that_are_not_finite(kv, dtype, group, what):
+    """A query with a NaN or an infinity gives NaN, whatever the signs it meets, and no other row does."""
+    g, n, dim = gen(group), 100, 64
+    for center in (-3.0, 3.0, 0.0):
+        k = (torch.randn((n, 1, dim), generator=g) * 0.1 + center).to(DTYPES[dtype])
+        k[:, 0, 2] = center + 1  # above each row's center
+        cache = kv.KvCache(2, 1, dim, n, bits=8)
+        cache.write(torch.cat([k, k]).to(DEV), torch.cat([k, k]).to(DEV), ints([0, 0]), ints([0, n, 2 * n]))
+        q = torch.randn((2, group, dim), generator=g).to(DTYPES[dtype])
+        q[1, group - 1, 2] = what
+        got = cache.attend(q.to(DEV), ints([n, n])).isnan().cpu()
+        want = torch.zeros((2, group), dtype=torch.bool)
+        want[1, group - 1] = True
+        assert torch.equal(got.all(-1), want) and torch.equal(got.any(-1), want)
