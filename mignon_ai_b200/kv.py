@@ -86,6 +86,13 @@ def _rows(name: str, x: torch.Tensor, index: int, heads: Optional[int], dim: int
     return x.data_ptr() or 16, stride[0], stride[1]
 
 
+def _output(q: torch.Tensor) -> torch.Tensor:
+    """Rows of q's shape, in q's order of strides unless q's rows overlap (then the last dimension's would
+    not be 1)."""
+    out = torch.empty_like(q)
+    return out if out.stride(2) == 1 else torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
 def _address(x: torch.Tensor) -> Tuple[int, int, int]:
     """_rows of a tensor that was made here."""
     stride = x.stride()
@@ -202,7 +209,7 @@ class KvCache:
         rows = _rows("q", q, index, None, self.head_dim, q.dtype)
         n, q_heads, _ = q.shape
         if out is None:
-            out = torch.empty_like(q)
+            out = _output(q)
             out_rows = _address(out)
         else:
             out_rows = _rows("out", out, index, q_heads, self.head_dim, q.dtype, n)
@@ -237,7 +244,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
     n_q, q_heads, _ = q.shape
     n_k, heads, _ = k.shape
     if out is None:
-        out = torch.empty_like(q)
+        out = _output(q)
         out_rows = _address(out)
     else:
         out_rows = _rows("out", out, index, q_heads, dim, dtype, n_q)

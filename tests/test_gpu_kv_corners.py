@@ -252,3 +252,17 @@ def test_attend_queries_that_are_not_finite(kv, dtype, group, what):
         want = torch.zeros((2, group), dtype=torch.bool)
         want[1, group - 1] = True
         assert torch.equal(got.all(-1), want) and torch.equal(got.any(-1), want)
+
+
+def test_queries_whose_rows_overlap(kv):
+    """Rows that share elements (every position of one long row), and rows repeated by a stride of zero: the
+    outputs are rows of their own."""
+    g = gen(15)
+    k, v = rows(g, 40, 1, 64, "f32").to(DEV), rows(g, 40, 1, 64, "f32").to(DEV)
+    cache = kv.KvCache(40, 1, 64, 4, bits=8)
+    cache.write(k, v, ints([0] * 40))
+    q = torch.randn(103, generator=g).to(DEV).unfold(0, 64, 1)[:, None]
+    again = torch.randn((1, 1, 64), generator=g).to(DEV).expand(40, 2, 64)
+    for x in (q, again):
+        assert torch.equal(kv.window_attention(x, k, v), kv.window_attention(x.contiguous(), k, v))
+        assert torch.equal(cache.attend(x, ints([1] * 40)), cache.attend(x.contiguous(), ints([1] * 40)))
