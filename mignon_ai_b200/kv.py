@@ -99,6 +99,13 @@ def _address(x: torch.Tensor) -> Tuple[int, int, int]:
     return x.data_ptr() or 16, stride[0], stride[1]
 
 
+def _int32(name: str, x: int) -> int:
+    """x, which ctypes would cut to 32 bits."""
+    if not -2 ** 31 <= x < 2 ** 31:
+        raise ValueError(f"{name}: {x} does not fit 32 bits")
+    return x
+
+
 def _dtype(x: torch.Tensor) -> int:
     code = _DTYPES.get(x.dtype)
     if code is None:
@@ -124,7 +131,8 @@ class KvCache:
 
     def __init__(self, sessions: int, heads: int, head_dim: int, slots: int, bits: int = 4, sinks: int = 0, device: int = 0):
         self._h = c_vp()
-        spec, n = _Spec(sessions, heads, head_dim, bits, slots, sinks), ctypes.c_size_t()
+        numbers = dict(sessions=sessions, heads=heads, head_dim=head_dim, bits=bits, slots=slots, sinks=sinks)
+        spec, n = _Spec(**{name: _int32(name, x) for name, x in numbers.items()}), ctypes.c_size_t()
         lib = _lib.lib()
         _lib.check(lib.mc_kv_bytes(ctypes.byref(spec), ctypes.byref(n)))
         self.memory = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", device))
@@ -216,7 +224,7 @@ class KvCache:
         _pack(s.buf, 0, *rows, *out_rows, 0, 0, 0, 0, 0, 0)
         status = self._lib.mc_kv_attend_dev(
             self._h, s.rows[0], s.rows[1], code, q_heads, _ints("sessions", sessions, n, index),
-            _ints("lens", lens, n, index), n, window, self._scale if scale is None else scale, _raw_stream(index))
+            _ints("lens", lens, n, index), n, _int32("window", window), self._scale if scale is None else scale, _raw_stream(index))
         if status:
             _lib.check(status)
         return out
@@ -259,7 +267,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
             return window_attention(q, k, v, q_start, k_start, window, sinks, scale, out)
     status = _lib.lib().mc_window_attn_dev(
         *s.rows, code, q_heads, heads, dim, n_q, n_k, _ints("q_start", q_start, n + 1, index),
-        _ints("k_start", k_start, n + 1, index), n, window, sinks, dim ** -0.5 if scale is None else scale,
+        _ints("k_start", k_start, n + 1, index), n, _int32("window", window), _int32("sinks", sinks), dim ** -0.5 if scale is None else scale,
         _raw_stream(index))
     if status:
         _lib.check(status)

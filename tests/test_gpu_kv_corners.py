@@ -266,3 +266,17 @@ def test_queries_whose_rows_overlap(kv):
     for x in (q, again):
         assert torch.equal(kv.window_attention(x, k, v), kv.window_attention(x.contiguous(), k, v))
         assert torch.equal(cache.attend(x, ints([1] * 40)), cache.attend(x.contiguous(), ints([1] * 40)))
+
+
+def test_numbers_that_do_not_fit(kv):
+    """Whole numbers beyond 32 bits are refused, not cut."""
+    cache = kv.KvCache(2, 2, 32, 8)
+    x = torch.randn((2, 2, 32), device=DEV)
+    cache.write(x, x, ints([0, 0]))
+    for n in (2 ** 32, 2 ** 32 + 1, 2 ** 31, -2 ** 32 + 1):
+        for call in (lambda: cache.attend(x, ints([1, 1]), window=n), lambda: kv.window_attention(x, x, x, window=n),
+                     lambda: kv.window_attention(x, x, x, sinks=n), lambda: kv.KvCache(2, 2, 32, n),
+                     lambda: kv.KvCache(2, 2, 32, 8, sinks=n), lambda: kv.KvCache(2, 2, 32, 8, bits=n + 4),
+                     lambda: kv.KvCache(n, 2, 32, 8)):
+            with pytest.raises((ValueError, RuntimeError)):
+                call()
