@@ -76,6 +76,8 @@ def _rows(name: str, x: torch.Tensor, index: int, heads: Optional[int], dim: int
     if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads) or (
             count is not None and shape[0] != count):
         raise ValueError(f"{name}: expected [{'rows' if count is None else count}, {heads or 'heads'}, {dim}], got {tuple(shape)}")
+    if shape[0] >> 31 or shape[1] >> 31:
+        raise ValueError(f"{name}: {tuple(shape)} does not fit 32 bits")
     if x.dtype is not dtype:
         raise TypeError(f"{name}: {x.dtype}, expected {dtype}")
     if x.get_device() != index:
@@ -267,8 +269,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start:
             return window_attention(q, k, v, q_start, k_start, window, sinks, scale, out)
     status = _lib.lib().mc_window_attn_dev(
         *s.rows, code, q_heads, heads, dim, n_q, n_k, _ints("q_start", q_start, n + 1, index),
-        _ints("k_start", k_start, n + 1, index), n, _int32("window", window), _int32("sinks", sinks), dim ** -0.5 if scale is None else scale,
-        _raw_stream(index))
+        _ints("k_start", k_start, n + 1, index), n, _int32("window", window), _int32("sinks", sinks),
+        dim ** -0.5 if scale is None else scale, _raw_stream(index))
     if status:
         _lib.check(status)
     return out

@@ -280,3 +280,17 @@ def test_numbers_that_do_not_fit(kv):
                      lambda: kv.KvCache(n, 2, 32, 8)):
             with pytest.raises((ValueError, RuntimeError)):
                 call()
+
+
+def test_rows_beyond_32_bits(kv):
+    """More rows, or heads, than the library counts (one row seen many times): refused, not cut."""
+    cache = kv.KvCache(2, 1, 32, 8)
+    many = torch.zeros((1, 1, 32), device=DEV).expand(2 ** 32 + 2, 1, 32)
+    heads = torch.zeros((2, 1, 32), device=DEV).expand(2, 2 ** 32 + 1, 32)
+    x = torch.zeros((2, 1, 32), device=DEV)
+    for call in (lambda: cache.write(many, many, ints([0, 0]), ints([0, 1, 2])),
+                 lambda: cache.read(ints([0, 0]), ints([0, 0]), ints([0, 1, 2]), out=(many, many)),
+                 lambda: cache.attend(heads, ints([0, 0]), out=heads),
+                 lambda: kv.window_attention(x, many, many, ints([0, 2]))):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
