@@ -286,8 +286,9 @@ typedef struct mc_kv mc_kv;
 
 /* A cache of keys and values for `sessions` sessions of one layer, in `memory`: device memory of
  * mc_kv_bytes(spec), 256-byte aligned, that the caller owns and leaves to the cache until it is
- * closed and its work is done; NULL: the library allocates it. It is zeroed on `stream`. Position p of a session is held at place p while p < sinks, then in a ring of
- * slots - sinks places: the cache holds the first `sinks` positions and the last slots - sinks.
+ * closed and its work is done; NULL: the library allocates it. It is zeroed on `stream`. Position p
+ * of a session is held at place p while p < sinks, then in a ring of slots - sinks places: the cache
+ * holds the first `sinks` positions and the last slots - sinks.
  * Each row of head_dim values is held as codes of `bits` bits with a scale and a center
  * (bfloat16): center + scale * m, m an odd integer in [-15, 15] (4 bits) or an integer in
  * [-127, 127] (8 bits). The center is the bfloat16 next to the middle of the row's extremes and

@@ -31,9 +31,10 @@ constexpr int kCacheThreads = 256;
 // written one by one. Rows whose slots do not follow their order in a group (past a ring's end that is
 // not a multiple of four) and single tokens go one at a time by a whole warp.
 //
-// What bounds it: reading, memory (65,536 rows of 8 heads of 128 from 4 bits: 63 us, 0.82 of the copy rate);
-// writing, instruction issue, 82 % busy at about seven instructions a value (80,000 such rows: 128 us, memory's
-// share 64). 48 registers for 40 warps an SM: 32 warps took a tenth longer, 24 a half.
+// What bounds it: reading, memory (65,536 rows of 8 heads of 128 from 4 bits: 64 us, 0.81 of the copy rate);
+// writing, instruction issue, 82 % busy at about seven instructions a value (80,000 such rows: 129 us, memory's
+// share 64); single tokens, the latency of a warp's dependent loads and narrow stores (4096 of 4 heads of 32: 12.5 us
+// to write, 9.3 to read). 48 registers for 40 warps an SM: 32 warps took a tenth longer, 24 a half.
 // ------------------------------------------------------------------------------------------------
 struct RowArgs {
   Cache c;

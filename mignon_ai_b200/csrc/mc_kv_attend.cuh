@@ -20,7 +20,7 @@
 // the scores never leave their registers.
 //
 // What bounds it: for long sessions reading the codes, once the loop runs (one session of 262,144
-// positions, 32/8 heads of 128 in 4 bits: 64 us, of which the loop's 285 MB are 43; 9 us go by until the first
+// positions, 32/8 heads of 128 in 4 bits: 66 us, of which the loop's 285 MB are 43; 9 us go by until the first
 // tile is done and 6 for the last join). For short ones instruction issue: about 890 instructions a tile of
 // 64 slots of a 128-wide head, for any number of heads up to four, and 1350 a (session, head) of 64 visible
 // slots at width 32 in float32 (4096 sessions of 4 heads: 41 us, memory's share 7). 16 warps an SM

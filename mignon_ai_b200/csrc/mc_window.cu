@@ -71,7 +71,7 @@ static int tile_launch(const Args& a, cudaStream_t stream) {
   auto paired = [](const Rows& r) { return reinterpret_cast<uintptr_t>(r.p) % (2 * sizeof(T)) == 0 && r.row % 2 == 0 && r.head % 2 == 0; };
   const bool quads = std::is_same<T, float>::value && a.dim % 4 == 0;
   // Heads one after the other in a CTA hide the start of all but the first (2000 prompts of 16-64 rows, 6
-  // heads of 64: 317 us against 338), as long as the tiles, about half of the segments' last ones among
+  // heads of 64: 319 us against 339), as long as the tiles, about half of the segments' last ones among
   // them, leave three waves of four CTAs an SM.
   int device = 0, n_sm = 0, heads = 1;
   MC_CUDA(cudaGetDevice(&device));

@@ -14,16 +14,17 @@
 //
 // Two CTAs share an SM (96 KB of operands and 256 TMEM columns each), so one's products run
 // under the other's exponentials: per tile the tensor pipe needs about 1000 cycles at dim 128 and
-// the exponentials as many. 8192 positions, 32/8 heads of 128, window 1024 with 4 sinks, bfloat16: 243 us,
-// 530 TFLOP/s of the visible pairs (a third more is computed, in tiles that the window cuts); the
+// the exponentials as many. 8192 positions, 32/8 heads of 128, window 1024 with 4 sinks, bfloat16: 245 us,
+// 527 TFLOP/s of the visible pairs (a third more is computed, in tiles that the window cuts); the
 // tensor pipe is 32 % busy. What bounds it is the chain of a tile in one CTA, 6500 cycles: 1700 for
 // the products, 1400 until the maximum is known, 2200 for the weights, 700 of meeting and handing over.
-// One thread a row (4 warps, S read twice) took 250 us; half of the weights by a cubic instead of the
-// exponential unit 240.
+// Other forms, measured beside one of 243 us: one thread a row (4 warps, S read twice) 250; half of the weights by a
+// cubic instead of the exponential unit 240.
 //
 // A hidden key's weight is an exact zero, but zero times an infinity or NaN among its values would
 // still reach the row. A row that comes out non-finite is therefore computed again key by key
-// (row_attention), which reads visible keys only.
+// (row_attention), which reads visible keys only, and its query from the tile in shared memory: outputs may
+// be in place of the queries. What the copying and the multiplying thread do is in mc_window_roles.h.
 #pragma once
 #include "mc_window_roles.h"
 #include "mc_window_row.cuh"

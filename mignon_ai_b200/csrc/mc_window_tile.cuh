@@ -18,7 +18,7 @@
 //
 // What bounds it: for long rows the three products at the legacy tensor rate (275 TFLOP/s of tf32
 // measured, so 92 of float32); for prompts of a tile or less the latency of each phase and the fetching of
-// instructions (2000 prompts of 16-64 rows, 6 heads of 64: 328 us, memory's share of it 75; 128 registers,
+// instructions (2000 prompts of 16-64 rows, 6 heads of 64: 319 us, memory's share of it 75; 128 registers,
 // 16 warps an SM, tensor pipe 17 % busy). Warps skip the columns that none of their 16 rows sees.
 #pragma once
 #include "mc_window_row.cuh"
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kTileThreads, DIMP <= 64 ? 4 : 2) tile_kernel(
     for (int n = 0; n < NK; n += 4) {
       if (n + 4 <= n_begin || n >= n_end) continue;
       float small[4][4] = {};
-      // not unrolled: short CTAs out of step with one another wait for instructions first (2000 prompts: 328 us,
-      // 352 unrolled)
+      // not unrolled: short CTAs out of step with one another wait for instructions first (2000 prompts: 319 us,
+      // 342 unrolled)
 #pragma unroll 1
       for (int k = 0; k < KD; ++k) {
         // step k, thread (r, c): dimensions 8k + 2c (a0, a1) and 8k + 2c + 1 (a2, a3) of rows r and r + 8
